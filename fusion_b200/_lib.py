@@ -91,6 +91,37 @@ class BlockDesc(C.Structure):
     ]
 
 
+class Fp4GemmDesc(C.Structure):
+    """Mirror of ``fus_fp4_gemm_desc``."""
+
+    _fields_ = [
+        ("wq", vp),
+        ("wsf", vp),
+        ("wg", vp),
+        ("n_experts", i32),
+        ("w_rows", i32),
+        ("K", i32),
+        ("fmt", i32),
+        ("xq", vp),
+        ("ldxq", i64),
+        ("xsf", vp),
+        ("xg", vp),
+        ("x_rows", i32),
+        ("block_n", i32),
+        ("expert_ids", vp),
+        ("ntp", vp),
+        ("live_ids", vp),
+        ("live_limit", i32),
+        ("scatter", i32),
+        ("epilogue", i32),
+        ("row_scale", vp),
+        ("out", vp),
+        ("ldo", i64),
+        ("out_rows", i32),
+        ("out_dtype", i32),
+    ]
+
+
 class EPP2PDesc(C.Structure):
     """Mirror of ``fus_ep_p2p_desc``."""
 
@@ -180,6 +211,14 @@ SIGNATURES: dict[str, tuple] = {
     "fus_oproj_finish": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fus_row_rstd": (i32, [vp, i64, i32, i32, f32, vp, vp, vp]),
     "fus_fp8_block_dequant": (i32, [vp, vp, i64, vp, i64, i32, i32, i32, vp, vp]),
+    "fus_fp4_scale_bytes": (sz, [i32, i64, i32, i32]),
+    "fus_fp4_quantize": (i32, [vp, i32, i64, i32, i32, i32, vp, i64, vp, i32, i32, vp, i64, i32,
+                               vp, i64, vp, vp, vp]),
+    "fus_fp4_dequantize": (i32, [vp, i64, vp, i32, i32, i64, i32, vp, i64, vp, i32, i64, vp, vp]),
+    "fus_fp4_weight_scale_bytes": (sz, [i32, i32, i32, i32, i32]),
+    "fus_fp4_pack_scales": (i32, [vp, i32, i32, i32, i32, i32, vp, vp]),
+    "fus_fp4_grouped_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, vp]),
+    "fus_fp4_expert_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, i32, i64, i32, i32, vp, vp]),
     "fus_fold_weight": (i32, [vp, vp, vp, i64, i32, i32, i64, vp, vp]),
     "fus_scale_sum_planes": (i32, [vp, i32, i64, i32, i32, vp, vp, i64, vp, vp]),
     "fus_ep_p2p_decode_forward": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp, vp]),

@@ -1,0 +1,114 @@
+"""Expert products with 4-bit weights: a weight stack, laid out once, and its call.
+
+``ExpertGemmFP4`` is the 4-bit form of one expert projection (w13 with SwiGLU, or w2): it
+quantises bf16 token rows in dispatch order and multiplies them with the packed weights of
+each block's expert (``fus_fp4_expert_gemm``: two overlapping launches, no host
+synchronisation, graph-capturable). Formats "mx" (32 elements share a power of two) and "nv"
+(16 share an e4m3, with one fp32 factor for each expert).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+from . import ops
+
+
+def quantize_weight(w: torch.Tensor, fmt: str):
+    """A bf16 / fp16 / fp32 weight stack [E, N, K] in 4 bits, as a checkpoint would hold it:
+    packed codes [E, N, K/2] uint8, row-major scale bytes [E, N, K/n] uint8 and, for "nv", the
+    experts' fp32 factors [E] (the largest magnitude over 448 * 6), else None."""
+    E, N, K = w.shape
+    q = torch.empty(E, N, K // 2, dtype=torch.uint8, device=w.device)
+    s = torch.empty(E, N, K // ops.FP4_BLOCK[fmt], dtype=torch.uint8, device=w.device)
+    g = torch.empty(E, dtype=torch.float32, device=w.device) if fmt == "nv" else None
+    for e in range(E):  # one expert at a time: no stack-sized temporary
+        if g is not None:
+            top = w[e].abs().amax().float() / (448.0 * 6.0)
+            g[e] = torch.where(top > 0, top, 1.0)
+        ops.fp4_quantize(w[e], q[e], s[e].view(-1), fmt, tile=0,
+                         gscale=g[e : e + 1] if g is not None else None)
+    return q, s, g
+
+
+class ExpertGemmFP4:
+    """Weights of one projection of E experts: q [E, N, K/2] packed codes and scales
+    [E, N, K/n] bytes as ``quantize_weight`` or a checkpoint gives them; ``gscale`` [E] and
+    ``x_gscale`` [1] fp32 factors of the weights and the token rows ("nv"; None: 1).
+    ``gate_up``: rows [0, N/2) gate, [N/2, N) up, SwiGLU in the epilogue, N/2 outputs."""
+
+    def __init__(self, q: torch.Tensor, scales: torch.Tensor, fmt: str, gscale=None,
+                 x_gscale=None, gate_up: bool = False):
+        if fmt not in ops.FP4_FORMATS:
+            raise ValueError(f"format {fmt!r} not in {sorted(ops.FP4_FORMATS)}")
+        if q.dim() != 3:
+            raise ValueError("packed weights are [E, N, K/2]")
+        ops._need(q, torch.uint8, "packed weights")
+        E, N, K = q.shape[0], q.shape[1], q.shape[2] * 2
+        if K % 32 or N % 16:
+            raise ValueError(f"K={K} must be a multiple of 32 and N={N} of 16")
+        ops._need(scales, torch.uint8, "scales", (E, N, K // ops.FP4_BLOCK[fmt]))
+        if fmt == "mx":
+            gscale = x_gscale = None
+        ops._need(gscale, torch.float32, "gscale", (E,))
+        ops._need(x_gscale, torch.float32, "x_gscale")
+        if x_gscale is not None and x_gscale.numel() != 1:
+            raise ValueError("x_gscale: one factor")
+        ops._same_device(q.device, scales, gscale, x_gscale)
+        self.E, self.N, self.K, self.fmt, self.gate_up = E, N, K, fmt, gate_up
+        self.cols = N // 2 if gate_up else N
+        self.device = q.device
+        self._keep = (q, ops.fp4_pack_scales(scales, fmt, gate_up), gscale, x_gscale)
+        d = L.Fp4GemmDesc()
+        d.wq, d.wsf, d.wg, d.xg = (ops._p(t) for t in self._keep[:3] + (x_gscale,))
+        d.n_experts, d.w_rows, d.K, d.fmt = E, N, K, ops.FP4_FORMATS[fmt]
+        d.ldxq = -(-K // 32) * 16
+        d.epilogue = ops.FUS_EPI_SWIGLU if gate_up else ops.FUS_EPI_BF16
+        self._desc = d
+
+    def __call__(self, x, out, sorted_ids, expert_ids, ntp, block_n: int, *, topk: int = 1,
+                 gather: bool = True, scatter: bool = True, row_scale=None):
+        """One projection over a dispatch layout (``ops.moe_align`` with block_n).
+
+        gather: x [T, K] holds tokens, dispatch row p is x[sorted_ids[p] // topk]; else x
+        [capacity, K] is in dispatch order. scatter: out [T * topk, cols] in pair order (row
+        sorted_ids[p]), else out [capacity, cols] in dispatch order; rows of pads are left as
+        they were. out is bf16 or fp32; row_scale: fp32, one for each row of out."""
+        dt, ldx = ops._dtype(x, "x"), ops._rows2d(x, "x")
+        cap = sorted_ids.numel()
+        pairs = x.shape[0] * topk if gather else out.shape[0] if scatter else None
+        if pairs is None:
+            raise ValueError("rows in dispatch order need gather or scatter to name the pairs")
+        if x.shape[1] != self.K or out.shape[1] != self.cols:
+            raise ValueError(f"x [.., {self.K}] and out [.., {self.cols}] required")
+        if out.shape[0] < (pairs if scatter else cap) or (not gather and x.shape[0] < cap):
+            raise ValueError("too few rows")
+        if expert_ids.numel() < cap // block_n or cap % block_n:
+            raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each")
+        if out.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("out is bf16 or fp32")
+        for t, what in ((sorted_ids, "sorted_ids"), (expert_ids, "expert_ids"), (ntp, "ntp")):
+            ops._need(t, torch.int32, what)
+        ops._need(row_scale, torch.float32, "row_scale")
+        if row_scale is not None and row_scale.numel() < out.shape[0]:
+            raise ValueError("row_scale: one for each row of out")
+        ops._same_device(self.device, x, out, sorted_ids, expert_ids, ntp, row_scale)
+        d = L.Fp4GemmDesc.from_buffer_copy(self._desc)
+        # the packed rows: fresh for each call, so calls on other streams and captured graphs
+        # never share them
+        rows = torch.empty(cap * d.ldxq + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n),
+                           dtype=torch.uint8, device=self.device)
+        d.xq = ops._p(rows)
+        d.xsf = d.xq + cap * d.ldxq
+        d.x_rows, d.block_n = cap, block_n
+        d.expert_ids, d.ntp = ops._p(expert_ids), ops._p(ntp)
+        d.live_ids, d.live_limit, d.scatter = ops._p(sorted_ids), pairs, int(scatter)
+        d.row_scale = ops._p(row_scale)
+        d.out, d.ldo = ops._p(out), ops._rows2d(out, "out")
+        d.out_rows, d.out_dtype = out.shape[0], ops.DT[out.dtype]
+        ops._call_on(self.device, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
+                     x.shape[0], topk if gather else 0)
+        return out

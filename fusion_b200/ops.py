@@ -319,6 +319,130 @@ def fp8_block_dequant(src, scale, dst, block=(128, 128)):
            block[0], block[1], _stream(), _sp())
 
 
+# -------------------------------------------------------------------------------------
+# operators over tensors of any device: the call runs on that device, on its current stream
+DT = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}  # FUS_DT_*
+FP4_FORMATS = {"mx": 0, "nv": 1}  # FUS_FP4_*
+FP4_BLOCK = {"mx": 32, "nv": 16}  # elements that share a scale
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: bf16, fp16 or fp32 required, not {t.dtype}")
+    return code
+
+
+def _need(t, dtype, what: str, shape=None) -> None:
+    """`t` (may be None) has this element type, this shape and contiguous elements."""
+    if t is None:
+        return
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {dtype} required, not {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, not {tuple(shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous elements required")
+
+
+def _rows2d(t: torch.Tensor, what: str) -> int:
+    """Row stride of a [rows, columns] tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what}: two dimensions with contiguous rows required")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """The entry point with `device`'s current stream and status word, that device current."""
+    if device.type != "cuda":
+        raise ValueError(f"{name}: tensors must be on a CUDA device, not {device}")
+    if device.index == torch.cuda.current_device():
+        L.call(name, *args, torch.cuda.current_stream(device).cuda_stream,
+               status_tensor(device.index).data_ptr())
+    else:
+        with torch.cuda.device(device):
+            L.call(name, *args, torch.cuda.current_stream(device).cuda_stream,
+                   status_tensor(device.index).data_ptr())
+
+
+def _same_device(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+
+
+def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
+    """Bytes of the scales of `rows` rows; ``tile`` is the dispatch block of a product's rows
+    (or 0: row-major)."""
+    n = int(L.lib().fus_fp4_scale_bytes(FP4_FORMATS[fmt], rows, K, tile))
+    if n == 0 and rows > 0:
+        raise ValueError(f"fp4_scale_bytes: K={K} (multiples of 32) or tile={tile} not possible")
+    return n
+
+
+def _fp4_args(q, sf, rows: int, K: int, fmt: str, tile: int, gscale, what: str) -> tuple:
+    if fmt not in FP4_FORMATS:
+        raise ValueError(f"{what}: format {fmt!r} not in {sorted(FP4_FORMATS)}")
+    if q.dtype != torch.uint8 or sf.dtype != torch.uint8:
+        raise TypeError(f"{what}: packed values and scales are uint8")
+    if tuple(q.shape) != (rows, K // 2):
+        raise ValueError(f"{what}: packed values of shape {tuple(q.shape)}, not {(rows, K // 2)}")
+    if not sf.is_contiguous() or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile):
+        raise ValueError(f"{what}: scales need {fp4_scale_bytes(rows, K, fmt, tile)} contiguous bytes")
+    _need(gscale, torch.float32, f"{what}: gscale")
+    per = 0
+    if gscale is not None:
+        if gscale.numel() < 1 or rows % gscale.numel():
+            raise ValueError(f"{what}: {gscale.numel()} factors for {rows} rows")
+        per = rows // gscale.numel() if gscale.numel() > 1 else 0
+    return _rows2d(q, what), per
+
+
+def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, id_div: int = 1,
+                 id_limit: int = 0, ntp=None):
+    """Rows of x [R, K] (bf16, fp16 or fp32) to 4 bits: q [rows, K/2] uint8, sf their scales
+    (``fp4_scale_bytes``). ``fmt`` "mx" or "nv"; gscale (nv): fp32 factors, one or one for each
+    equal run of rows. With ``ids`` (int32, one for each row of q) row p is x[ids[p] // id_div];
+    rows whose id is not in [0, id_limit) keep what they held, as do rows from ntp[0] on."""
+    dt, ldx = _dtype(x, "fp4_quantize"), _rows2d(x, "fp4_quantize: x")
+    K, rows = x.shape[1], q.shape[0]
+    _same_device(x.device, q, sf, gscale, ids, ntp)
+    ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_quantize")
+    _need(ids, torch.int32, "fp4_quantize: ids", (rows,))
+    _need(ntp, torch.int32, "fp4_quantize: ntp")
+    _call_on(x.device, "fus_fp4_quantize", _p(x), dt, ldx, x.shape[0], K, FP4_FORMATS[fmt],
+             _p(gscale), per, _p(ids), id_div, id_limit, _p(ntp), rows, tile, _p(q), ldq, _p(sf))
+
+
+def fp4_dequantize(q, sf, out, fmt: str, *, tile: int = 128, gscale=None):
+    """The values of packed rows: out [rows, K] (bf16, fp16 or fp32) = q * scale (* factor)."""
+    dt, ldo = _dtype(out, "fp4_dequantize"), _rows2d(out, "fp4_dequantize: out")
+    rows, K = out.shape
+    _same_device(out.device, q, sf, gscale)
+    ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_dequantize")
+    _call_on(out.device, "fus_fp4_dequantize", _p(q), ldq, _p(sf), FP4_FORMATS[fmt], tile, rows, K,
+             _p(gscale), per, _p(out), dt, ldo)
+
+
+def fp4_pack_scales(scales, fmt: str, gate_up: bool = False) -> torch.Tensor:
+    """Row-major scales [E, N, K/n] (or [N, K/n]) of a weight stack, as a checkpoint stores
+    them, in the product's weight layout; ``gate_up`` for a w13 stack multiplied with SwiGLU."""
+    if fmt not in FP4_FORMATS:
+        raise ValueError(f"fp4_pack_scales: format {fmt!r} not in {sorted(FP4_FORMATS)}")
+    s = scales if scales.dim() == 3 else scales[None]
+    _need(s, torch.uint8, "fp4_pack_scales")
+    E, N, n = s.shape
+    K = n * FP4_BLOCK[fmt]
+    need = int(L.lib().fus_fp4_weight_scale_bytes(FP4_FORMATS[fmt], E, N, K, int(gate_up)))
+    sf = torch.empty(need, dtype=torch.uint8, device=s.device)
+    if s.device.type != "cuda":
+        raise ValueError("fp4_pack_scales: CUDA tensors required")
+    with torch.cuda.device(s.device):
+        L.call("fus_fp4_pack_scales", _p(s), FP4_FORMATS[fmt], E, N, K, int(gate_up), _p(sf),
+               _stream())
+    return sf
+
+
 def add(a, b, o):
     M, N = a.shape
     L.call("fus_add", _p(a), _ld(a), _p(b), _ld(b), _p(o), _ld(o), M, N, _stream(), _sp())

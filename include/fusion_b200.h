@@ -36,6 +36,11 @@ extern "C" {
 #define FUS_E_LAUNCH (-2)      /* CUDA reported an error when launching */
 #define FUS_E_UNSUPPORTED (-3) /* shape outside what the kernels implement */
 
+/* element types of the entry points that take more than bf16 */
+#define FUS_DT_BF16 0
+#define FUS_DT_F32 1
+#define FUS_DT_F16 2
+
 /* device status bits */
 #define FUS_ERR_TIMEOUT 0x1    /* a pipeline wait exceeded its time budget */
 #define FUS_ERR_BAD_EXPERT 0x2 /* an expert id outside [0, E) was seen */
@@ -329,6 +334,80 @@ int fus_scale_sum_planes(const float* partial, int nsplit, long plane, int T, in
  * rows x cols row-major, cols % 8 == 0, bc % 8 == 0. */
 int fus_fp8_block_dequant(const void* src, const float* scale, long scale_ld, void* dst, long rows,
                           int cols, int br, int bc, void* stream, int* status);
+
+/* ---------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (no counterpart in the reference). Values are e2m1
+ * (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign), two in a byte, the even element in the low four
+ * bits; consecutive elements along K share a scale byte:
+ *   FUS_FP4_MX: 32 elements, e8m0, s = 2^(floor(log2 amax) - 2)
+ *   FUS_FP4_NV: 16 elements, e4m3, s = e4m3(amax / (6 g)), with one fp32 factor g > 0 of
+ *               the tensor (of each `rows_per_g` rows when that is not 0; NULL: g = 1)
+ * q = e2m1(x / s) (/ (s g)), to the nearest, ties to even, at most 6; every code is the one
+ * of exact arithmetic. A block with an infinity or a NaN gets the NaN scale. K % 32 == 0.
+ * Scale layouts: tile = 0 row-major [rows, K / n] bytes, as checkpoints store them; tile in
+ * {16, 32, 64, 128, 256}: the atoms the tensor cores read, one run for each `tile` rows (a
+ * dispatch block), fus_fp4_scale_bytes(fmt, rows, K, tile) bytes, 16-byte aligned.
+ *
+ * fus_fp4_quantize: row p of q [rows, ldq bytes] = x[ids ? ids[p] / id_div : p]; rows with
+ *   ids[p] outside [0, id_limit) (dispatch pads) and rows from ntp[0] on keep what they
+ *   held. x [x_rows, K] of `dtype`, any alignment (32-byte rows are faster).
+ * fus_fp4_dequantize: out[p, k] = q * s (* g), rounded to `dtype`.
+ * fus_fp4_pack_scales: row-major scales [n_experts, w_rows, K / n] of an expert stack ->
+ *   weight scale tiles (fus_fp4_weight_scale_bytes). gate_up = 1 for a w13 stack that
+ *   FUS_EPI_SWIGLU multiplies. */
+#define FUS_FP4_MX 0
+#define FUS_FP4_NV 1
+size_t fus_fp4_scale_bytes(int fmt, long rows, int K, int tile);
+int fus_fp4_quantize(const void* x, int dtype, long ldx, int x_rows, int K, int fmt,
+                     const float* gscale, long rows_per_g, const int* ids, int id_div,
+                     int id_limit, const int* ntp, long rows, int tile, void* q, long ldq,
+                     void* sf, void* stream, int* status);
+int fus_fp4_dequantize(const void* q, long ldq, const void* sf, int fmt, int tile, long rows,
+                       int K, const float* gscale, long rows_per_g, void* out, int dtype,
+                       long ldo, void* stream, int* status);
+size_t fus_fp4_weight_scale_bytes(int fmt, int n_experts, int w_rows, int K, int gate_up);
+int fus_fp4_pack_scales(const void* scales, int fmt, int n_experts, int w_rows, int K,
+                        int gate_up, void* sf, void* stream);
+
+/* Grouped product of 4-bit rows with 4-bit expert weights on the block-scaled tensor
+ * cores, the 4-bit form of fus_grouped_gemm: rows of xq in dispatch order, block b of
+ * `block_n` rows meets expert expert_ids[b] (NULL: one expert); rows from ntp[0] on and
+ * rows whose live_ids entry is not below live_limit (pads, which end a block) give no output.
+ *   FUS_EPI_BF16   out[r, n] = wg[e] * xg * row_scale[r] * acc      n < w_rows
+ *   FUS_EPI_SWIGLU out[r, f] = row_scale[r] * silu(y[r, f]) * y[r, w_rows/2 + f],
+ *                  y = wg[e] * xg * acc in fp32; f < w_rows / 2
+ * r = live_ids[p] with scatter, p without. K % 32 == 0, w_rows % 16 == 0, block_n in {16,
+ * 32, 64, 128, 256}, 16-byte aligned rows. Rows of out outside [0, out_rows) are dropped.
+ * fus_fp4_expert_gemm quantises the rows first, into the descriptor's xq and xsf (then
+ * workspaces, not inputs): dispatch row p is x[live_ids[p] / gather_div], or x[p] with
+ * gather_div 0. The two kernels overlap (the weights are requested while rows are
+ * quantised). */
+typedef struct fus_fp4_gemm_desc {
+  const void* wq;         /* [n_experts, w_rows, K / 2] packed weights                      */
+  const void* wsf;        /* their scale tiles (fus_fp4_pack_scales)                        */
+  const float* wg;        /* [n_experts] factors (FUS_FP4_NV) or NULL                       */
+  int n_experts, w_rows, K, fmt;
+  const void* xq;         /* [x_rows, ldxq bytes] packed rows in dispatch order             */
+  long ldxq;
+  const void* xsf;        /* their scales, tile = block_n                                   */
+  const float* xg;        /* one factor (FUS_FP4_NV) or NULL                                */
+  int x_rows;
+  int block_n;
+  const int* expert_ids;
+  const int* ntp;
+  const int* live_ids;    /* optional (scatter and gather need it)                          */
+  int live_limit;
+  int scatter;
+  int epilogue;           /* FUS_EPI_BF16 or FUS_EPI_SWIGLU                                 */
+  const float* row_scale; /* optional, by output row                                        */
+  void* out;
+  long ldo;
+  int out_rows;
+  int out_dtype;          /* FUS_DT_BF16 or FUS_DT_F32                                      */
+} fus_fp4_gemm_desc;
+int fus_fp4_grouped_gemm(const fus_fp4_gemm_desc* d, void* stream, int* status);
+int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, int x_dtype, long ldx,
+                        int src_rows, int gather_div, void* stream, int* status);
 
 /* ---------------------------------------------------------------------------------
  * Element-wise / merge kernels

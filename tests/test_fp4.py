@@ -1,0 +1,125 @@
+"""Microscaled 4-bit floating point without a GPU: sizes, refusals, and the oracle itself."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import fp4_oracle as Q
+from fusion_b200 import _lib as L
+from fusion_b200 import fp4, ops
+
+P = 0x10000  # a 256-byte aligned address that host checks never read
+
+
+def test_oracle_grids():
+    assert list(Q.E2M1) == [0, 0.5, 1, 1.5, 2, 3, 4, 6]
+    assert Q.E4M3[126] == 448 and Q.E4M3[1] == 2.0 ** -9
+    # ties to the even code, saturation at the top
+    assert list(Q.nearest(Q.E2M1, np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 9.0]))) == [0, 2, 2, 4, 4, 6, 6, 7]
+
+
+@pytest.mark.parametrize("fmt,n", [("mx", 32), ("nv", 16)])
+def test_scale_bytes(fmt, n):
+    assert ops.fp4_scale_bytes(5, 96, fmt, 0) == 5 * 96 // n
+    for tile in (16, 32, 64, 128, 256):
+        for rows in (1, 16, 257):
+            for K in (32, 256, 6144):
+                pos = Q.scale_positions(fmt, rows, K, tile)
+                size = ops.fp4_scale_bytes(rows, K, fmt, tile)
+                assert size > pos.max() and len(np.unique(pos)) == pos.size
+    with pytest.raises(ValueError):
+        ops.fp4_scale_bytes(4, 40, fmt)
+    with pytest.raises(ValueError):
+        ops.fp4_scale_bytes(4, 64, fmt, tile=48)
+
+
+def _refused(rc, text):
+    assert rc in (-1, -3) and text in L.last_error(), L.last_error()
+
+
+def test_quantize_refusals():
+    def call(x=P, dtype=0, ldx=64, x_rows=4, K=64, fmt=1, g=None, per=0, ids=None, div=1, limit=0,
+             rows=4, tile=16, q=P, ldq=32, sf=P):
+        return L.lib().fus_fp4_quantize(x, dtype, ldx, x_rows, K, fmt, g, per, ids, div, limit, None,
+                                        rows, tile, q, ldq, sf, None, None)
+
+    assert call(rows=0) == 0
+    _refused(call(K=40), "multiple of 32")
+    _refused(call(K=0), "multiple of 32")
+    _refused(call(fmt=2), "format")
+    _refused(call(dtype=7), "dtype")
+    _refused(call(tile=24), "tile")
+    _refused(call(rows=-1), "row count")
+    _refused(call(rows=5), "5 rows of 4")
+    _refused(call(ldx=63), "source rows")
+    _refused(call(q=P + 8), "16-byte")
+    _refused(call(ldq=24), "16-byte")
+    _refused(call(sf=P + 4), "16-byte")
+    _refused(call(x=P + 1), "misaligned")
+    _refused(call(x=None), "null")
+    _refused(call(ids=P, div=0), "id_div")
+    _refused(call(fmt=0, g=P), "no factor")
+
+
+def test_dequantize_and_pack_refusals():
+    def call(q=P, ldq=32, sf=P, fmt=0, tile=16, rows=4, K=64, g=None, out=P, dtype=0, ldo=64):
+        return L.lib().fus_fp4_dequantize(q, ldq, sf, fmt, tile, rows, K, g, 0, out, dtype, ldo, None, None)
+
+    assert call(rows=0) == 0
+    _refused(call(ldo=63), "output rows")
+    _refused(call(ldq=28), "8-byte")
+    _refused(call(g=P), "no factor")
+    _refused(call(out=None), "null")
+    _refused(L.lib().fus_fp4_pack_scales(P, 0, 2, 32, 33, 0, P, None), "sizes")
+    _refused(L.lib().fus_fp4_pack_scales(None, 0, 2, 32, 64, 0, P, None), "null")
+
+
+def test_gemm_refusals():
+    def desc(**kw):
+        d = L.Fp4GemmDesc(wq=P, wsf=P, n_experts=2, w_rows=64, K=64, fmt=1, xq=P, ldxq=32, xsf=P,
+                          x_rows=32, block_n=16, expert_ids=P, ntp=P, live_ids=P, live_limit=20,
+                          scatter=1, epilogue=0, out=P, ldo=64, out_rows=20, out_dtype=0)
+        for k, v in kw.items():
+            setattr(d, k, v)
+        return d
+
+    def call(**kw):
+        return L.lib().fus_fp4_grouped_gemm(ctypes.byref(desc(**kw)), None, None)
+
+    assert call(x_rows=0) == 0 and call(out_rows=0) == 0
+    for kw, text in (({"K": 48}, "multiple of 32"), ({"w_rows": 40}, "multiple of 16"),
+                     ({"block_n": 48}, "block_n"), ({"epilogue": 2}, "epilogue"), ({"fmt": 3}, "format"),
+                     ({"out_dtype": 2}, "output is"), ({"wq": None}, "null"), ({"xsf": P + 8}, "aligned"),
+                     ({"ldo": 56}, "output rows"), ({"ldo": 68}, "output rows"),
+                     ({"live_ids": None}, "live_ids"), ({"expert_ids": None}, "expert_ids"),
+                     ({"n_experts": 0}, "n_experts"), ({"fmt": 0, "xg": P}, "no factors"),
+                     ({"ldxq": 16}, "aligned"), ({"x_rows": -1}, "row counts")):
+        _refused(call(**kw), text)
+    d = desc(live_ids=None, scatter=0)
+    _refused(L.lib().fus_fp4_expert_gemm(ctypes.byref(d), P, 0, 64, 4, 8, None, None), "live_ids")
+    _refused(L.lib().fus_fp4_expert_gemm(None, P, 0, 64, 4, 8, None, None), "null descriptor")
+
+
+def test_python_refusals():
+    q = torch.zeros(2, 32, 32, dtype=torch.uint8)
+    s = torch.zeros(2, 32, 2, dtype=torch.uint8)
+    for bad in (dict(fmt="fp8"), dict(scales=s[:, :, :1]), dict(q=q.int()), dict(q=q[0]),
+                dict(q=q[:, :24]), dict(q=q[:, :, :20])):
+        with pytest.raises((ValueError, TypeError)):
+            fp4.ExpertGemmFP4(**{"q": q, "scales": s, "fmt": "mx", **bad})
+    x = torch.zeros(4, 64)
+    ok = (torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4096, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.fp4_quantize(x, *ok, "mx")
+    with pytest.raises(TypeError):
+        ops.fp4_quantize(x.int(), *ok, "mx")
+    with pytest.raises(ValueError):
+        ops.fp4_quantize(x, ok[0][:, :31], ok[1], "mx")
+    with pytest.raises(ValueError):
+        ops.fp4_quantize(x, ok[0], ok[1][:8], "mx")
+    with pytest.raises(ValueError):
+        ops.fp4_quantize(x.T, *ok, "mx")
