@@ -211,6 +211,10 @@ SIGNATURES: dict[str, tuple] = {
     "fus_oproj_finish": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fus_row_rstd": (i32, [vp, i64, i32, i32, f32, vp, vp, vp]),
     "fus_fp8_block_dequant": (i32, [vp, vp, i64, vp, i64, i32, i32, i32, vp, vp]),
+    "fus_norm_gate_residual": (i32, [vp, i64, vp, i64, vp, vp, i64, i32, i32, f32, vp, i64, vp, vp,
+                                     i64, i32, i32, i32, f32, vp, vp]),
+    "fus_route_topk": (i32, [vp, i32, i64, vp, i32, i32, i32, vp, vp, i32, i32, i32, f32, i32, vp,
+                             vp]),
     "fus_fp4_scale_bytes": (sz, [i32, i64, i32, i32]),
     "fus_fp4_quantize": (i32, [vp, i32, i64, i32, i32, i32, vp, i64, vp, i32, i32, vp, i64, i32,
                                vp, i64, vp, vp, vp]),

@@ -10,6 +10,7 @@
 // twice, a little smaller and a little larger (1 -+ 2^-21), and only where the two codes
 // differ (some 10^-6 of the blocks) it is decided by products of at most 31 bits in fp64.
 // A block with an infinity or a NaN gets the NaN scale: the product shows it.
+#include "dtype.cuh"
 #include "fp4.cuh"
 #include "host_util.h"
 
@@ -22,18 +23,6 @@ FUS_DEVICE void ld32(const void* p, uint32_t* r) {  // 32 bytes in one load, rea
                  "=r"(r[6]), "=r"(r[7])
                : "l"(p));
 }
-
-FUS_DEVICE float to_f(float v) { return v; }
-FUS_DEVICE float to_f(__half v) { return __half2float(v); }
-FUS_DEVICE float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-FUS_DEVICE T from_f(float v);
-template <>
-FUS_DEVICE float from_f<float>(float v) { return v; }
-template <>
-FUS_DEVICE __half from_f<__half>(float v) { return __float2half_rn(v); }
-template <>
-FUS_DEVICE __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // 16 consecutive elements as fp32; vec: p is 32-byte aligned
 template <typename T>
@@ -264,8 +253,6 @@ bool valid_tile(int tile) {
   return tile == 16 || tile == 32 || tile == 64 || tile == 128 || tile == 256;
 }
 
-int dtype_size(int dtype) { return dtype == FUS_DT_F32 ? 4 : 2; }
-
 template <int FMT>
 int quantize_launch(const void* x, int dtype, long ldx, int x_rows, long rows, const int* ntp,
                     const int* ids, int id_div, int id_limit, int K, const float* gscale,
@@ -307,7 +294,7 @@ void dequantize_launch(const void* q, long ldq, const void* sf, int tile, long r
 int check_common(const char* what, int fmt, int dtype, long rows, int K, int tile) {
   if (fmt != FUS_FP4_MX && fmt != FUS_FP4_NV)
     return set_error(FUS_E_INVALID, "%s: unknown format %d", what, fmt);
-  if (dtype != FUS_DT_BF16 && dtype != FUS_DT_F16 && dtype != FUS_DT_F32)
+  if (!dtype_known(dtype))
     return set_error(FUS_E_INVALID, "%s: unknown dtype %d", what, dtype);
   if (rows < 0 || rows > 0x7fffffffL) return set_error(FUS_E_INVALID, "%s: bad row count", what);
   if (K <= 0 || K % 32)

@@ -371,6 +371,63 @@ def _same_device(device: torch.device, *tensors) -> None:
             raise ValueError(f"tensors on {device} and {t.device}")
 
 
+GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
+SCORES = {"sigmoid": 0, "softmax": 1}
+
+
+def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
+                       gate_act: str = "none", alpha: float = 1.0, eps: float = 1e-5):
+    """h = res + alpha * act(gate) * norm(y) * post_w and x = norm(h) * pre_w, RMS norms of
+    [T, N] rows (bf16, fp16 or fp32 throughout). post_w None: y unnormalised; x None: h only.
+    gate: [T, 1], [1, N] or [N], or [T, N]; gate_act "none", "sigmoid" or "tanh". h may be res
+    or y itself, x may be y."""
+    what = "norm_gate_residual"
+    dt = _dtype(y, what)
+    T, N = y.shape
+    for t, name in ((res, "res"), (h, "h"), (x, "x")):
+        if t is not None and (t.dtype != y.dtype or t.shape != y.shape):
+            raise ValueError(f"{what}: {name} must have y's type and shape")
+    _need(post_w, y.dtype, f"{what}: post_w", (N,))
+    _need(pre_w, y.dtype, f"{what}: pre_w", (N,))
+    kind, ldg = 0, 0
+    if gate is not None:
+        if gate.dtype != y.dtype:
+            raise TypeError(f"{what}: gate must have y's type")
+        if gate.dim() == 1:
+            gate = gate[None]
+        if gate.shape == (T, N):
+            kind, ldg = 3, _rows2d(gate, f"{what}: gate")
+        elif gate.shape == (1, N):
+            kind = 2
+            _rows2d(gate, f"{what}: gate")
+        elif gate.shape == (T, 1):
+            kind, ldg = 1, gate.stride(0)
+        else:
+            raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} for {(T, N)}")
+    _same_device(y.device, res, h, x, post_w, pre_w, gate)
+    _call_on(y.device, "fus_norm_gate_residual", _p(y), _rows2d(y, what), _p(res),
+             _rows2d(res, what), _p(post_w), _p(gate), ldg, kind, GATE_ACTS[gate_act], alpha,
+             _p(h), _rows2d(h, what), _p(pre_w), _p(x), _rows2d(x, what) if x is not None else 0,
+             T, N, dt, eps)
+
+
+def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group: int = 1,
+               topk_group: int = 1, renorm: bool = True, scale: float = 1.0):
+    """Experts of each token from router logits [T, E] (bf16, fp16 or fp32): topi [T, k] int32
+    and their weights topw [T, k] fp32. score "sigmoid" or "softmax"; bias [E] fp32 counts in the
+    choice only; n_group / topk_group limit the choice to the best groups; renorm divides by the
+    chosen weights' sum. -inf or NaN logits mask experts; slots left over get id -1, weight 0."""
+    T, E = logits.shape
+    k = topi.shape[1] if topi.dim() == 2 else 0
+    dt, ld = _dtype(logits, "route_topk"), _rows2d(logits, "route_topk: logits")
+    _need(topi, torch.int32, "route_topk: topi", (T, k))
+    _need(topw, torch.float32, "route_topk: topw", (T, k))
+    _need(bias, torch.float32, "route_topk: bias", (E,))
+    _same_device(logits.device, topw, topi, bias)
+    _call_on(logits.device, "fus_route_topk", _p(logits), dt, ld, _p(bias), SCORES[score], n_group,
+             topk_group, _p(topw), _p(topi), T, E, k, scale, int(renorm))
+
+
 def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
     """Bytes of the scales of `rows` rows; ``tile`` is the dispatch block of a product's rows
     (or 0: row-major)."""

@@ -87,6 +87,28 @@ int fus_add_rmsnorm(const void* x, long ldx, const void* res, long ldr, const vo
                     void* h1, long ldh, void* out, long ldo, int T, int N, float eps,
                     int do_add, int do_norm, void* stream, int* status);
 
+/* The norms after a block and before the next, with the block's gate and residual scale (no
+ * counterpart in the reference, whose layer has no norm after a block):
+ *   v = y * rsqrt(mean(y^2) + eps) * post_w      (post_w NULL: v = y)
+ *   h = res + alpha * act(gate) * v
+ *   x = h * rsqrt(mean(h^2) + eps) * pre_w       (x and pre_w NULL: not computed)
+ * [T, N] rows, all of `dtype`, any N to 32768 (16384 fp32) and any alignment (16-byte rows are
+ * fastest); fp32 arithmetic, h and x rounded once each, x from the unrounded h. gate: none,
+ * one for a token (gate[t * ldg]), for a channel (gate[n]) or for an element. h may be res
+ * or y, x may be y (the same rows and strides). */
+#define FUS_GATE_NONE 0
+#define FUS_GATE_TOKEN 1
+#define FUS_GATE_CHANNEL 2
+#define FUS_GATE_FULL 3
+#define FUS_GATE_LINEAR 0  /* act */
+#define FUS_GATE_SIGMOID 1
+#define FUS_GATE_TANH 2
+int fus_norm_gate_residual(const void* y, long ldy, const void* res, long ldr,
+                           const void* post_w, const void* gate, long ldg, int gate_kind,
+                           int gate_act, float alpha, void* h, long ldh, const void* pre_w,
+                           void* x, long ldx, int T, int N, int dtype, float eps, void* stream,
+                           int* status);
+
 /* ---------------------------------------------------------------------------------
  * Router weights. The router GEMM runs on the tensor cores in bf16 with fp32
  * accumulation over `nplanes` bf16 planes whose sum is the weight:
@@ -126,6 +148,23 @@ int fus_router_topk_grouped(const float* partial, int nsplit, const float* bias,
                             float* logits_out, float* topw, int* topi, int T, int E, int topk,
                             int n_group, int topk_group, float scale, int renorm, void* stream,
                             int* status);
+
+/* Routing from logits of any router (no counterpart in the reference, whose router is the
+ * sigmoid of fus_router_topk): logits [T, E] of `dtype`, E <= 1024 (with groups: E / n_group
+ * <= 32 * 2^floor(log2(32 / n_group))), topk <= 32.
+ *   s = sigmoid(l) (FUS_SCORE_SIGMOID) or softmax(l) (FUS_SCORE_SOFTMAX);  c = s + bias
+ *   n_group > 1: only experts of the topk_group groups (consecutive ids) with the largest
+ *   sum of their two largest c may be chosen (ties: lower group; fus_router_topk_grouped
+ *   keeps the others with choice 0, this one never chooses them)
+ *   ids = top-k of c, descending, ties to the lower id, as exact arithmetic orders them;
+ *   w = s[ids]; if renorm: w /= max(sum(w), 1e-20); w *= scale
+ * A logit of -infinity or NaN masks its expert. Slots without an expert left: id -1 (a hole
+ * of fus_moe_align), weight 0. bias [E] fp32 or NULL, finite. */
+#define FUS_SCORE_SIGMOID 0
+#define FUS_SCORE_SOFTMAX 1
+int fus_route_topk(const void* logits, int dtype, long ld, const float* bias, int score,
+                   int n_group, int topk_group, float* topw, int* topi, int T, int E, int topk,
+                   float scale, int renorm, void* stream, int* status);
 
 /* ---------------------------------------------------------------------------------
  * Dispatch layout (glm52/reference.py:85-128 moe_align_block_size, sglang layout):

@@ -1,0 +1,166 @@
+"""Routing from logits on the GPU against its definition in 64 bits: ids exactly, weights within
+the rounding of fp32 sums and exponentials."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from fusion_b200 import ops
+from gpu_util import finish
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _oracle(l, bias, score, n_group, topk_group, k, renorm, scale):
+    T, E = l.shape
+    l = np.where(np.isnan(l), -np.inf, np.minimum(l, np.finfo(np.float32).max))
+    with np.errstate(all="ignore"):
+        if score == "sigmoid":
+            s = 1 / (1 + np.exp(-l))
+        else:
+            e = np.where(l > -np.inf, np.exp(l - l.max(1, keepdims=True)), 0.0)
+            s = e / e.sum(1, keepdims=True)
+    c = np.where(l > -np.inf, s + (0.0 if bias is None else bias), -np.inf)
+    if n_group > 1:
+        g = c.reshape(T, n_group, -1)
+        two = -np.sort(-g, -1)[..., :2]
+        best = np.where(np.isfinite(two).any(-1), np.where(np.isfinite(two), two, 0.0).sum(-1), -np.inf)
+        keep = np.argsort(-best, 1, kind="stable")[:, :topk_group]
+        mask = np.zeros((T, n_group), bool)
+        np.put_along_axis(mask, keep, True, 1)
+        c = np.where(mask[..., None], g, -np.inf).reshape(T, E)
+    # a plain choice ranks the logits: the score is monotone in them, and exact
+    rank = l if bias is None and n_group == 1 else c
+    ids = np.argsort(-rank, 1, kind="stable")[:, :k]
+    ok = np.take_along_axis(rank, ids, 1) > -np.inf
+    w = np.where(ok, np.take_along_axis(np.nan_to_num(s), ids, 1), 0.0)
+    if renorm:
+        w = w / np.maximum(w.sum(1, keepdims=True), 1e-20)
+    return np.where(ok, ids, -1), w * scale
+
+
+def _run(logits, k, bias=None, score="sigmoid", n_group=1, topk_group=1, renorm=True, scale=1.0):
+    T = logits.shape[0]
+    w = torch.full((T, k), 9.0, device="cuda")
+    i = torch.full((T, k), 9, dtype=torch.int32, device="cuda")
+    ops.route_topk(logits, w, i, score=score, bias=bias, n_group=n_group, topk_group=topk_group,
+                   renorm=renorm, scale=scale)
+    finish()
+    ids, want = _oracle(logits.double().cpu().numpy(), None if bias is None else bias.double().cpu().numpy(),
+                        score, n_group, topk_group, k, renorm, scale)
+    np.testing.assert_array_equal(i.cpu().numpy(), ids)
+    # (E / 32 + 5) roundings of the sum, 25 of an exponential of -20, ten more: below 2^-17
+    got = w.double().cpu().numpy()
+    assert (np.abs(got - want) <= 2.0 ** -17 * np.abs(want) + 1e-30).all()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("T,E,k,n_group,topk_group", [
+    (1, 256, 8, 1, 1), (1, 1, 1, 1, 1), (7, 8, 8, 1, 1), (33, 33, 5, 1, 1), (130, 162, 6, 1, 1),
+    (65, 256, 8, 8, 4), (19, 104, 3, 8, 2), (40, 512, 8, 4, 1), (9, 1024, 32, 1, 1),
+    (21, 60, 4, 5, 2), (17, 64, 8, 32, 8), (300, 48, 24, 3, 3), (5, 1000, 10, 1, 1)])
+def test_matches_definition(score, dtype, with_bias, T, E, k, n_group, topk_group):
+    gen = torch.Generator(device="cuda").manual_seed(T * E + k)
+    logits = torch.randn(T, E, device="cuda", generator=gen).to(DTYPES[dtype])
+    bias = 0.1 * torch.randn(E, device="cuda", generator=gen) if with_bias else None
+    _run(logits, k, bias, score, n_group, topk_group, renorm=bool(E % 3), scale=2.5)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_long_batch(score):
+    """Enough rows that some decisions hang on the last bits of fp32 scores."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    logits = 0.02 * torch.randn(20000, 256, device="cuda", generator=gen)
+    bias = 1e-4 * torch.randn(256, device="cuda", generator=gen)
+    _run(logits, 8, bias, score)
+    _run(logits, 8, bias, score, n_group=8, topk_group=4)
+    _run(logits, 8, None, score, n_group=8, topk_group=4)
+
+
+def test_ties_go_to_the_lower_id():
+    logits = torch.zeros(4, 200, device="cuda")
+    logits[1] = torch.arange(200, device="cuda") // 40
+    logits[2, ::7] = 1.0
+    logits[3] = 3.0
+    for bias in (None, torch.zeros(200, device="cuda"), torch.full((200,), 0.5, device="cuda")):
+        for score in ("sigmoid", "softmax"):
+            _run(logits, 8, bias, score)
+            _run(logits, 8, bias, score, n_group=4, topk_group=2)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("bias", [False, True])
+def test_masked_experts_and_empty_rows(score, bias):
+    """-inf and NaN mask; rows left with fewer than k experts, with one, with none; the lowest
+    finite value is a logit like any other; +inf is the largest."""
+    logits = torch.randn(9, 96, device="cuda")
+    inf = float("inf")
+    logits[0] = -inf
+    logits[1] = float("nan")
+    logits[2, 1:] = -inf
+    logits[3, 5:] = float("nan")
+    logits[4, ::2] = -inf
+    logits[5] = torch.finfo(torch.float32).min
+    logits[6, 3] = inf
+    logits[6, 50] = inf
+    logits[7, 4:90] = torch.finfo(torch.float32).min
+    b = 0.3 * torch.randn(96, device="cuda") if bias else None
+    for groups in (1, 4):
+        _run(logits, 6, b, score, n_group=groups, topk_group=max(1, groups // 2))
+
+
+def test_large_bias_and_logits():
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    logits = 60 * torch.randn(50, 128, device="cuda", generator=gen)
+    bias = 100 * torch.randn(128, device="cuda", generator=gen).round()
+    _run(logits, 8, bias)
+    _run(logits.clamp(-8, 8), 8, -bias, n_group=8, topk_group=3)
+
+
+def test_strided_logits_and_rows_behind():
+    buf = torch.randn(10, 300, device="cuda")
+    for off in (0, 1, 4):
+        _run(buf[:, off:off + 250], 8, torch.randn(250, device="cuda"))
+    w = torch.full((12, 8), 7.0, device="cuda")
+    i = torch.full((12, 8), 7, dtype=torch.int32, device="cuda")
+    ops.route_topk(buf, w[:10], i[:10])
+    finish()
+    assert (w[10:] == 7).all() and (i[10:] == 7).all()
+
+
+def test_stream_graph_and_empty_batch():
+    logits = torch.randn(64, 256, device="cuda")
+    w, i = torch.empty(64, 8, device="cuda"), torch.empty(64, 8, dtype=torch.int32, device="cuda")
+    ops.route_topk(logits, w, i)
+    w2, i2 = torch.zeros_like(w), torch.zeros_like(i)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.route_topk(logits, w2, i2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g.replay()
+    finish()
+    assert torch.equal(w, w2) and torch.equal(i, i2)
+    ops.route_topk(logits[:0], w[:0], i[:0])
+    finish()
+
+
+def test_feeds_the_dispatch_layout():
+    """Holes of masked rows are not placed."""
+    logits = torch.randn(12, 16, device="cuda")
+    logits[3] = -float("inf")
+    w, i = torch.empty(12, 4, device="cuda"), torch.empty(12, 4, dtype=torch.int32, device="cuda")
+    ops.route_topk(logits, w, i, score="softmax")
+    sorted_ids = torch.empty(48 + 16 * 16, dtype=torch.int32, device="cuda")
+    eids = torch.empty(19, dtype=torch.int32, device="cuda")
+    ntp = torch.empty(1, dtype=torch.int32, device="cuda")
+    ops.moe_align(i, 16, 16, sorted_ids, eids, ntp)
+    finish()
+    placed = sorted_ids[: int(ntp.item())].cpu().numpy()
+    assert sorted(placed[placed < 48]) == [p for p in range(48) if p // 4 != 3]
