@@ -57,7 +57,7 @@ class ExpertGemmFP4:
         ops._need(x_gscale, torch.float32, "x_gscale")
         if x_gscale is not None and x_gscale.numel() != 1:
             raise ValueError("x_gscale: one factor")
-        ops._same_device(q.device, scales, gscale, x_gscale)
+        self._dev = ops._device_of(q, scales, gscale, x_gscale)
         self.E, self.N, self.K, self.fmt, self.gate_up = E, N, K, fmt, gate_up
         self.cols = N // 2 if gate_up else N
         self.device = q.device
@@ -95,7 +95,8 @@ class ExpertGemmFP4:
         ops._need(row_scale, torch.float32, "row_scale")
         if row_scale is not None and row_scale.numel() < out.shape[0]:
             raise ValueError("row_scale: one for each row of out")
-        ops._same_device(self.device, x, out, sorted_ids, expert_ids, ntp, row_scale)
+        if ops._device_of(x, out, sorted_ids, expert_ids, ntp, row_scale) != self._dev:
+            raise ValueError(f"tensors must be on {self.device}, with the weights")
         d = L.Fp4GemmDesc.from_buffer_copy(self._desc)
         # the packed rows: fresh for each call, so calls on other streams and captured graphs
         # never share them
@@ -109,6 +110,6 @@ class ExpertGemmFP4:
         d.row_scale = ops._p(row_scale)
         d.out, d.ldo = ops._p(out), ops._rows2d(out, "out")
         d.out_rows, d.out_dtype = out.shape[0], ops.DT[out.dtype]
-        ops._call_on(self.device, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
+        ops._call_on(self._dev, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
                      x.shape[0], topk if gather else 0)
         return out

@@ -32,14 +32,15 @@ def _p(t: torch.Tensor | None) -> int | None:
     library's empty-size early return instead of its null-pointer check."""
     if t is None:
         return None
-    if t.numel() == 0 and t.is_cuda:
+    ptr = t.data_ptr()
+    if ptr == 0 and t.numel() == 0 and t.is_cuda:
         idx = t.device.index if t.device.index is not None else torch.cuda.current_device()
         a = _empty_anchor.get(idx)
         if a is None:
             a = torch.zeros(256, dtype=torch.uint8, device=t.device)
             _empty_anchor[idx] = a
         return a.data_ptr()
-    return t.data_ptr()
+    return ptr
 
 
 def _stream() -> int:
@@ -320,10 +321,15 @@ def fp8_block_dequant(src, scale, dst, block=(128, 128)):
 
 
 # -------------------------------------------------------------------------------------
-# operators over tensors of any device: the call runs on that device, on its current stream
+# operators over tensors of any device: the call runs on that device, on its current stream.
+# At a few tokens the host's work is what a call costs, so the checks read each property of
+# a tensor once and the stream and status word are looked up without building objects.
 DT = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}  # FUS_DT_*
 FP4_FORMATS = {"mx": 0, "nv": 1}  # FUS_FP4_*
 FP4_BLOCK = {"mx": 32, "nv": 16}  # elements that share a scale
+
+_fns: dict = {}
+_status_ptr: dict[int, int] = {}
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -339,7 +345,7 @@ def _need(t, dtype, what: str, shape=None) -> None:
         return
     if t.dtype != dtype:
         raise TypeError(f"{what}: {dtype} required, not {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, not {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: contiguous elements required")
@@ -347,28 +353,37 @@ def _need(t, dtype, what: str, shape=None) -> None:
 
 def _rows2d(t: torch.Tensor, what: str) -> int:
     """Row stride of a [rows, columns] tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    st = t.stride()
+    if len(st) != 2 or (st[1] != 1 and t.shape[1] > 1):
         raise ValueError(f"{what}: two dimensions with contiguous rows required")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return st[0] if t.shape[0] > 1 else t.shape[1]
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """The entry point with `device`'s current stream and status word, that device current."""
-    if device.type != "cuda":
-        raise ValueError(f"{name}: tensors must be on a CUDA device, not {device}")
-    if device.index == torch.cuda.current_device():
-        L.call(name, *args, torch.cuda.current_stream(device).cuda_stream,
-               status_tensor(device.index).data_ptr())
-    else:
-        with torch.cuda.device(device):
-            L.call(name, *args, torch.cuda.current_stream(device).cuda_stream,
-                   status_tensor(device.index).data_ptr())
+def _device_of(t: torch.Tensor, *others) -> int:
+    """Index of the CUDA device that holds `t` and the others (None: absent)."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"tensors must be on a CUDA device, not {t.device}")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError(f"tensors on {t.device} and {o.device}")
+    return dev
 
 
-def _same_device(device: torch.device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
+def _call_on(dev: int, name: str, *args) -> None:
+    """The entry point with device `dev` current, on its current stream, with its status word."""
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return _call_on(dev, name, *args)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(L.lib(), name)
+    status = _status_ptr.get(dev)
+    if status is None:
+        status = _status_ptr[dev] = status_tensor(dev).data_ptr()
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev), status)
+    if rc != 0:
+        raise RuntimeError(f"{name} failed ({rc}): {L.last_error()}")
 
 
 GATE_ACTS = {"none": 0, "sigmoid": 1, "tanh": 2}
@@ -383,12 +398,13 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
     or y itself, x may be y."""
     what = "norm_gate_residual"
     dt = _dtype(y, what)
-    T, N = y.shape
-    for t, name in ((res, "res"), (h, "h"), (x, "x")):
-        if t is not None and (t.dtype != y.dtype or t.shape != y.shape):
-            raise ValueError(f"{what}: {name} must have y's type and shape")
-    _need(post_w, y.dtype, f"{what}: post_w", (N,))
-    _need(pre_w, y.dtype, f"{what}: pre_w", (N,))
+    shape, dtype = y.shape, y.dtype
+    T, N = shape
+    for t in (res, h, x):
+        if t is not None and (t.dtype != dtype or t.shape != shape):
+            raise ValueError(f"{what}: res, h and x must have y's type and shape")
+    for w in (post_w, pre_w):
+        _need(w, dtype, "norm_gate_residual: weight", (N,))
     kind, ldg = 0, 0
     if gate is not None:
         if gate.dtype != y.dtype:
@@ -404,8 +420,8 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
             kind, ldg = 1, gate.stride(0)
         else:
             raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} for {(T, N)}")
-    _same_device(y.device, res, h, x, post_w, pre_w, gate)
-    _call_on(y.device, "fus_norm_gate_residual", _p(y), _rows2d(y, what), _p(res),
+    dev = _device_of(y, res, h, x, post_w, pre_w, gate)
+    _call_on(dev, "fus_norm_gate_residual", _p(y), _rows2d(y, what), _p(res),
              _rows2d(res, what), _p(post_w), _p(gate), ldg, kind, GATE_ACTS[gate_act], alpha,
              _p(h), _rows2d(h, what), _p(pre_w), _p(x), _rows2d(x, what) if x is not None else 0,
              T, N, dt, eps)
@@ -423,18 +439,21 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
     _need(topi, torch.int32, "route_topk: topi", (T, k))
     _need(topw, torch.float32, "route_topk: topw", (T, k))
     _need(bias, torch.float32, "route_topk: bias", (E,))
-    _same_device(logits.device, topw, topi, bias)
-    _call_on(logits.device, "fus_route_topk", _p(logits), dt, ld, _p(bias), SCORES[score], n_group,
+    dev = _device_of(logits, topw, topi, bias)
+    _call_on(dev, "fus_route_topk", _p(logits), dt, ld, _p(bias), SCORES[score], n_group,
              topk_group, _p(topw), _p(topi), T, E, k, scale, int(renorm))
 
 
 def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
     """Bytes of the scales of `rows` rows; ``tile`` is the dispatch block of a product's rows
     (or 0: row-major)."""
-    n = int(L.lib().fus_fp4_scale_bytes(FP4_FORMATS[fmt], rows, K, tile))
-    if n == 0 and rows > 0:
+    n = FP4_BLOCK[fmt]
+    if K <= 0 or K % 32 or rows < 0 or tile not in (0, 16, 32, 64, 128, 256):
         raise ValueError(f"fp4_scale_bytes: K={K} (multiples of 32) or tile={tile} not possible")
-    return n
+    if tile == 0:
+        return rows * (K // n)
+    # whole 512-byte atoms of 128 rows x 4 scales, 256 elements of K at a time
+    return -(-rows // tile) * -(-K // 256) * (64 // n) * (tile // 128 or 1) * 512
 
 
 def _fp4_args(q, sf, rows: int, K: int, fmt: str, tile: int, gscale, what: str) -> tuple:
@@ -442,11 +461,12 @@ def _fp4_args(q, sf, rows: int, K: int, fmt: str, tile: int, gscale, what: str) 
         raise ValueError(f"{what}: format {fmt!r} not in {sorted(FP4_FORMATS)}")
     if q.dtype != torch.uint8 or sf.dtype != torch.uint8:
         raise TypeError(f"{what}: packed values and scales are uint8")
-    if tuple(q.shape) != (rows, K // 2):
+    if q.shape != (rows, K // 2):
         raise ValueError(f"{what}: packed values of shape {tuple(q.shape)}, not {(rows, K // 2)}")
-    if not sf.is_contiguous() or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile):
-        raise ValueError(f"{what}: scales need {fp4_scale_bytes(rows, K, fmt, tile)} contiguous bytes")
-    _need(gscale, torch.float32, f"{what}: gscale")
+    need = fp4_scale_bytes(rows, K, fmt, tile)
+    if not sf.is_contiguous() or sf.numel() < need:
+        raise ValueError(f"{what}: scales need {need} contiguous bytes")
+    _need(gscale, torch.float32, what)
     per = 0
     if gscale is not None:
         if gscale.numel() < 1 or rows % gscale.numel():
@@ -463,11 +483,12 @@ def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, 
     rows whose id is not in [0, id_limit) keep what they held, as do rows from ntp[0] on."""
     dt, ldx = _dtype(x, "fp4_quantize"), _rows2d(x, "fp4_quantize: x")
     K, rows = x.shape[1], q.shape[0]
-    _same_device(x.device, q, sf, gscale, ids, ntp)
+    dev = _device_of(x, q, sf, gscale, ids, ntp)
     ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_quantize")
-    _need(ids, torch.int32, "fp4_quantize: ids", (rows,))
+    if ids is not None:
+        _need(ids, torch.int32, "fp4_quantize: ids", (rows,))
     _need(ntp, torch.int32, "fp4_quantize: ntp")
-    _call_on(x.device, "fus_fp4_quantize", _p(x), dt, ldx, x.shape[0], K, FP4_FORMATS[fmt],
+    _call_on(dev, "fus_fp4_quantize", _p(x), dt, ldx, x.shape[0], K, FP4_FORMATS[fmt],
              _p(gscale), per, _p(ids), id_div, id_limit, _p(ntp), rows, tile, _p(q), ldq, _p(sf))
 
 
@@ -475,9 +496,9 @@ def fp4_dequantize(q, sf, out, fmt: str, *, tile: int = 128, gscale=None):
     """The values of packed rows: out [rows, K] (bf16, fp16 or fp32) = q * scale (* factor)."""
     dt, ldo = _dtype(out, "fp4_dequantize"), _rows2d(out, "fp4_dequantize: out")
     rows, K = out.shape
-    _same_device(out.device, q, sf, gscale)
+    dev = _device_of(out, q, sf, gscale)
     ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_dequantize")
-    _call_on(out.device, "fus_fp4_dequantize", _p(q), ldq, _p(sf), FP4_FORMATS[fmt], tile, rows, K,
+    _call_on(dev, "fus_fp4_dequantize", _p(q), ldq, _p(sf), FP4_FORMATS[fmt], tile, rows, K,
              _p(gscale), per, _p(out), dt, ldo)
 
 

@@ -31,6 +31,7 @@ def test_scale_bytes(fmt, n):
                 pos = Q.scale_positions(fmt, rows, K, tile)
                 size = ops.fp4_scale_bytes(rows, K, fmt, tile)
                 assert size > pos.max() and len(np.unique(pos)) == pos.size
+                assert size == L.lib().fus_fp4_scale_bytes(ops.FP4_FORMATS[fmt], rows, K, tile)
     with pytest.raises(ValueError):
         ops.fp4_scale_bytes(4, 40, fmt)
     with pytest.raises(ValueError):
