@@ -38,27 +38,56 @@ FUS_DEVICE float cta_sum(float v, float* red) {
   return warp_sum(v);
 }
 
+template <typename T, int V>
+FUS_DEVICE void unpack_v(const uint4& u, float* f) {
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = to_f(e[j]);
+}
+template <typename T, int V>
+FUS_DEVICE uint4 pack_v(const float* f) {
+  uint4 u;
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int j = 0; j < V; ++j) e[j] = from_f<T>(f[j]);
+  return u;
+}
+
 // V elements (16 bytes) from p + i for i in [i0, i0 + V) within [0, N); whole: one load
 template <typename T, int V>
 FUS_DEVICE void load_v(const T* p, int i0, int N, bool whole, float* f) {
   if (whole) {
-    const uint4 u = ldg_stream(p + i0);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = to_f(e[j]);
+    unpack_v<T, V>(ldg_stream(p + i0), f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = i0 + j >= 0 && i0 + j < N ? to_f(p[i0 + j]) : 0.f;
   }
 }
-// the same for the weights, which every row reads (kept in L1)
+// The same for the weights, which every row reads (kept in L1). They start on 16 bytes but
+// the row does not: element i0 is `off` short of a 16-byte line, so two lines are read and
+// shifted together.
 template <typename T, int V>
-FUS_DEVICE void load_w(const T* p, int i0, int N, bool whole, float* f) {
-  if (whole) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + i0));
-    const T* e = reinterpret_cast<const T*>(&u);
+FUS_DEVICE void load_w(const T* p, int i0, int N, bool whole, int off, float* f) {
+  if (whole && off == 0) {
+    unpack_v<T, V>(__ldg(reinterpret_cast<const uint4*>(p + i0)), f);
+  } else if (whole && i0 + off + V <= N) {
+    const uint4* line = reinterpret_cast<const uint4*>(p + i0 + off - V);
+    const uint4 a = __ldg(line), b = __ldg(line + 1);
+    uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const int bytes = (V - off) * (int)sizeof(T);  // 2 .. 14, a multiple of sizeof(T)
+    if (bytes & 8) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = to_f(e[j]);
+      for (int j = 0; j < 6; ++j) r[j] = r[j + 2];
+    }
+    if (bytes & 4) {
+#pragma unroll
+      for (int j = 0; j < 5; ++j) r[j] = r[j + 1];
+    }
+    if (bytes & 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = __funnelshift_r(r[j], r[j + 1], 16);
+    }
+    unpack_v<T, V>(make_uint4(r[0], r[1], r[2], r[3]), f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = i0 + j >= 0 && i0 + j < N ? to_f(p[i0 + j]) : 0.f;
@@ -67,11 +96,7 @@ FUS_DEVICE void load_w(const T* p, int i0, int N, bool whole, float* f) {
 template <typename T, int V>
 FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, const float* f) {
   if (whole) {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = from_f<T>(f[j]);
-    *reinterpret_cast<uint4*>(p + i0) = u;
+    *reinterpret_cast<uint4*>(p + i0) = pack_v<T, V>(f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -81,8 +106,7 @@ FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, const float* f) {
 
 // One CTA for a row, VPT 16-byte vectors for a thread. MODE 0: every row of every tensor starts
 // on 16 bytes. 1: rows start anywhere, but alike in all row tensors (odd widths): vectors
-// follow the 16-byte lines of memory, the two at the ends and the weights go by element. 2: by
-// element.
+// follow the 16-byte lines of memory, the ones at the ends go by element. 2: by element.
 template <typename T, int VPT, int MODE>
 __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(T);
@@ -125,14 +149,14 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
     if (i >= N) continue;
     if (a.post_w) {
       float w[V];
-      load_w<T, V>(reinterpret_cast<const T*>(a.post_w), i, N, MODE == 0 && whole(i), w);
+      load_w<T, V>(reinterpret_cast<const T*>(a.post_w), i, N, whole(i), off, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) f[v][j] *= w[j];
     }
     if (a.gate_kind >= 2) {
       float g[V];
       if (a.gate_kind == 2)
-        load_w<T, V>(reinterpret_cast<const T*>(a.gate), i, N, MODE == 0 && whole(i), g);
+        load_w<T, V>(reinterpret_cast<const T*>(a.gate), i, N, whole(i), off, g);
       else
         load_v<T, V>(reinterpret_cast<const T*>(a.gate) + t * a.ldg, i, N, whole(i), g);
 #pragma unroll
@@ -154,11 +178,145 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
     const int i = start(v);
     if (i >= N) continue;
     float w[V];
-    load_w<T, V>(reinterpret_cast<const T*>(a.pre_w), i, N, MODE == 0 && whole(i), w);
+    load_w<T, V>(reinterpret_cast<const T*>(a.pre_w), i, N, whole(i), off, w);
 #pragma unroll
     for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
     store_v<T, V>(x, i, N, whole(i), w);
   }
+}
+
+// Many rows: persistent CTAs, each with a ring of rows that bulk copies fill ahead of the
+// arithmetic, so that loads never wait for a row's two sums and barriers. The weights (and a
+// channel gate) stay in registers over all rows.
+constexpr int kRingThreads = 256;
+
+template <typename T, int VPT, bool FULL>
+__global__ void __launch_bounds__(kRingThreads, 2)
+    norm_gate_residual_ring_kernel(const NormArgs a, int rows, int stages, int* status) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float red[2][32];
+  __shared__ uint64_t bars[8];
+  __shared__ volatile int abort_flag;
+  extern __shared__ uint8_t ring[];  // stages x (y row | res row | gate row)
+  const int N = a.N, nv = N / V;
+  const uint32_t row_bytes = (uint32_t)N * sizeof(T);
+  const uint32_t stage_bytes = row_bytes * (FULL ? 3 : 2);
+  const uint32_t bar = smem_u32(bars);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(bar + 8 * s, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  auto load_row = [&](long t, int s) {
+    const uint64_t pol = policy_evict_first();
+    const uint32_t dst = smem_u32(ring) + s * stage_bytes;
+    mbar_arrive_expect_tx(bar + 8 * s, stage_bytes);
+    bulk_load(dst, reinterpret_cast<const T*>(a.y) + t * a.ldy, row_bytes, bar + 8 * s, pol);
+    bulk_load(dst + row_bytes, reinterpret_cast<const T*>(a.res) + t * a.ldr, row_bytes,
+              bar + 8 * s, pol);
+    if (FULL)
+      bulk_load(dst + 2 * row_bytes, reinterpret_cast<const T*>(a.gate) + t * a.ldg, row_bytes,
+                bar + 8 * s, pol);
+  };
+  if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s) {
+      const long t = blockIdx.x + (long)s * gridDim.x;
+      if (t < rows) load_row(t, s);
+    }
+  uint4 post[VPT], pre[VPT], gch[VPT];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int i = threadIdx.x + v * kRingThreads;
+    post[v] = pre[v] = gch[v] = make_uint4(0, 0, 0, 0);
+    if (i < nv) {
+      if (a.post_w) post[v] = __ldg(reinterpret_cast<const uint4*>(a.post_w) + i);
+      if (a.pre_w) pre[v] = __ldg(reinterpret_cast<const uint4*>(a.pre_w) + i);
+      if (a.gate_kind == 2) gch[v] = __ldg(reinterpret_cast<const uint4*>(a.gate) + i);
+    }
+  }
+  int n = 0;
+  for (long t = blockIdx.x; t < rows; t += gridDim.x, ++n) {
+    const int s = n % stages;
+    float scale = a.alpha;
+    if (a.gate_kind == 1)
+      scale *= gate_act(to_f(reinterpret_cast<const T*>(a.gate)[t * a.ldg]), a.act);
+    if (!mbar_wait_bounded(bar + 8 * s, (n / stages) & 1, &abort_flag, status)) break;
+    const uint4* sy = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
+    const uint4* sr = sy + nv;
+    const uint4* sg = sr + nv;
+    float f[VPT][V];
+    uint4 r[VPT], g[VPT];
+    float ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int i = threadIdx.x + v * kRingThreads;
+      uint4 u = make_uint4(0, 0, 0, 0);
+      r[v] = g[v] = u;
+      if (i < nv) {
+        u = sy[i];
+        r[v] = sr[i];
+        if (FULL) g[v] = sg[i];
+      }
+      unpack_v<T, V>(u, f[v]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) ss += f[v][j] * f[v][j];
+    }
+    ss = cta_sum(ss, red[0]);  // its barrier: the whole CTA has read the stage
+    if (threadIdx.x == 0) {
+      const long next = t + (long)stages * gridDim.x;
+      if (next < rows) load_row(next, s);
+    }
+    if (a.post_w) scale *= 1.0f / sqrtf(ss / (float)N + a.eps);
+    float sh = 0.f;
+    T* h = reinterpret_cast<T*>(a.h) + t * a.ldh;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int i = threadIdx.x + v * kRingThreads;
+      float w[V];
+      if (a.post_w) {
+        unpack_v<T, V>(post[v], w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[v][j] *= w[j];
+      }
+      if (FULL || a.gate_kind == 2) {
+        unpack_v<T, V>(FULL ? g[v] : gch[v], w);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[v][j] *= gate_act(w[j], a.act);
+      }
+      unpack_v<T, V>(r[v], w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        f[v][j] = w[j] + scale * f[v][j];
+        sh += f[v][j] * f[v][j];
+      }
+      if (i < nv) reinterpret_cast<uint4*>(h)[i] = pack_v<T, V>(f[v]);
+    }
+    if (!a.x) continue;
+    sh = cta_sum(sh, red[1]);
+    const float rstd = 1.0f / sqrtf(sh / (float)N + a.eps);
+    T* x = reinterpret_cast<T*>(a.x) + t * a.ldx;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int i = threadIdx.x + v * kRingThreads;
+      float w[V];
+      unpack_v<T, V>(pre[v], w);
+#pragma unroll
+      for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
+      if (i < nv) reinterpret_cast<uint4*>(x)[i] = pack_v<T, V>(w);
+    }
+  }
+}
+
+template <typename T, int VPT, bool FULL>
+int launch_ring(const NormArgs& a, int rows, int stages, cudaStream_t st, int* status) {
+  auto fn = norm_gate_residual_ring_kernel<T, VPT, FULL>;
+  const int bytes = stages * (FULL ? 3 : 2) * a.N * (int)sizeof(T);
+  // the limit is set once, to what two CTAs of an SM may have
+  if (int rc = ensure_smem_attr((const void*)fn, 110 * 1024, "norm_gate_residual")) return rc;
+  const int grid = 2 * num_sms();
+  fn<<<grid < rows ? grid : rows, kRingThreads, bytes, st>>>(a, rows, stages, status);
+  return check_launch("norm_gate_residual");
 }
 
 template <typename T, int VPT>
@@ -172,7 +330,7 @@ void launch_mode(const NormArgs& a, int T_, int threads, int mode, cudaStream_t 
 }
 
 template <typename T>
-int launch_norm(const NormArgs& a, int rows, cudaStream_t st) {
+int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
   constexpr int V = 16 / sizeof(T);
   // alignment of the row tensors: mode 0 wants all on 16 bytes (weights too), mode 1 alike
   const void* rowp[5] = {a.y, a.res, a.h, a.x, a.gate_kind == 3 ? a.gate : nullptr};
@@ -188,6 +346,21 @@ int launch_norm(const NormArgs& a, int rows, cudaStream_t st) {
   for (const void* p : wp) on16 = on16 && (!p || aligned16(p));
   const int mode = on16 ? 0 : alike ? 1 : 2;
   const int nv = (a.N + V - 1) / V + (mode == 1 ? 1 : 0);
+  const bool full = a.gate_kind == 3;
+  // the ring wants whole aligned rows, some rows for each CTA and two stages at least
+  if (mode == 0 && a.N % V == 0 && rows >= 4 * 148 && nv > kRingThreads / 2 &&
+      nv <= 3 * kRingThreads) {
+    int stages = 108 * 1024 / ((full ? 3 : 2) * a.N * (int)sizeof(T));
+    if (stages > 8) stages = 8;
+    if (stages >= 2) {
+      const int vpt = (nv + kRingThreads - 1) / kRingThreads;
+#define FUS_RING(P) \
+  (full ? launch_ring<T, P, true>(a, rows, stages, st, status) \
+        : launch_ring<T, P, false>(a, rows, stages, st, status))
+      return vpt == 1 ? FUS_RING(1) : vpt == 2 ? FUS_RING(2) : FUS_RING(3);
+#undef FUS_RING
+    }
+  }
   // few rows: as many threads as there are vectors (latency); many: four vectors for each
   int vpt = rows <= 2 * 148 ? 1 : 4;
   while (vpt > 1 && nv < 32 * vpt) vpt >>= 1;
@@ -212,7 +385,6 @@ extern "C" int fus_norm_gate_residual(const void* y, long ldy, const void* res, 
                                       int gate_kind, int gate_act, float alpha, void* h, long ldh,
                                       const void* pre_w, void* x, long ldx, int T, int N,
                                       int dtype, float eps, void* stream, int* status) {
-  (void)status;
   if (T < 0 || N < 1) return set_error(FUS_E_INVALID, "norm_gate_residual: bad sizes");
   if (!dtype_known(dtype)) return set_error(FUS_E_INVALID, "norm_gate_residual: dtype %d", dtype);
   if (gate_kind < FUS_GATE_NONE || gate_kind > FUS_GATE_FULL || gate_act < FUS_GATE_LINEAR ||
@@ -233,7 +405,7 @@ extern "C" int fus_norm_gate_residual(const void* y, long ldy, const void* res, 
   NormArgs a{y, res, post_w, pre_w, gate_kind ? gate : nullptr, h, x, ldy, ldr, ldh, ldx, ldg,
              N, gate_kind, gate_act, alpha, eps};
   cudaStream_t st = as_stream(stream);
-  if (dtype == FUS_DT_BF16) return launch_norm<__nv_bfloat16>(a, T, st);
-  if (dtype == FUS_DT_F16) return launch_norm<__half>(a, T, st);
-  return launch_norm<float>(a, T, st);
+  if (dtype == FUS_DT_BF16) return launch_norm<__nv_bfloat16>(a, T, st, status);
+  if (dtype == FUS_DT_F16) return launch_norm<__half>(a, T, st, status);
+  return launch_norm<float>(a, T, st, status);
 }

@@ -280,6 +280,17 @@ FUS_DEVICE void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, in
       : "memory");
 }
 
+// untiled copy global -> shared, completion counted on an mbarrier; addresses and size are
+// multiples of 16 bytes
+FUS_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
+                          uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
+      "[%1], %2, [%3], %4;" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+      : "memory");
+}
+
 // 4 rows (one 128-byte box row each) gathered by row index into consecutive smem rows;
 // the tensor map's box is one row high. Rows past the tensor's extent read zeros.
 FUS_DEVICE void tma_gather4(uint32_t dst, const CUtensorMap* m, uint32_t bar, int c0, int r0,

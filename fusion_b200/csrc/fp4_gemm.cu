@@ -118,15 +118,6 @@ FUS_DEVICE void tc_cp_scales(uint32_t taddr, uint32_t saddr) {
                : "memory");
 }
 
-FUS_DEVICE void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
-                          uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
-      "[%1], %2, [%3], %4;" ::"r"(dst),
-      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
-      : "memory");
-}
-
 template <int BN, int FMT, bool SWIGLU>
 __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
