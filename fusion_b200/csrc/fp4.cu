@@ -6,9 +6,12 @@
 //   NV  s = e4m3(a / (6 g)), to the nearest, ties to even, at most 448
 //   q = e2m1(x / s) or e2m1(x / (s g)), to the nearest, ties to even, at most 6
 // Every code is the one of exact arithmetic. MX only scales by powers of two, which fp32 does
-// exactly. NV divides: fp32 leaves a relative error below 2^-22, so the quotient is rounded
-// twice, a little smaller and a little larger (1 -+ 2^-21), and only where the two codes
-// differ (some 10^-6 of the blocks) it is decided by products of at most 31 bits in fp64.
+// exactly. NV divides: fp32 leaves a relative error below 2^-21, so the quotient is rounded
+// twice, a little smaller and a little larger (1 -+ 2^-21); where the two codes differ, the
+// value is compared with the border between them times s g, a product and its rounding error.
+// That is not rare: a factor taken from a bf16 maximum makes exact ties of bf16 values (half
+// of the warps of a 8192 x 6144 tensor meet one), so it must be cheap (the comparison in
+// fp64 cost 19 of 57 us there).
 // A block with an infinity or a NaN gets the NaN scale: the product shows it.
 #include "dtype.cuh"
 #include "fp4.cuh"
@@ -24,22 +27,24 @@ FUS_DEVICE void ld32(const void* p, uint32_t* r) {  // 32 bytes in one load, rea
                : "l"(p));
 }
 
-// 16 consecutive elements as fp32 and the largest magnitude's bits; vec: p is 32-byte aligned.
-// Magnitudes compare as integers: an infinity or NaN comes out on top.
+// 16 consecutive elements; vec: p is 32-byte aligned
 template <typename T>
-FUS_DEVICE uint32_t load16(const T* p, bool vec, float* f) {
-  uint32_t r[8 * sizeof(T) / 2];
-  T* e = reinterpret_cast<T*>(r);
+FUS_DEVICE void load16(const T* p, bool vec, uint32_t* r) {
   if (vec) {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i)
       ld32(reinterpret_cast<const char*>(p) + 32 * i, r + 8 * i);
   } else {
+    T* e = reinterpret_cast<T*>(r);
 #pragma unroll
     for (int i = 0; i < 16; ++i) e[i] = p[i];
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) f[i] = to_f(e[i]);
+}
+
+// the largest magnitude's bits (fp32). Magnitudes compare as integers: an infinity or NaN comes
+// out on top.
+template <typename T>
+FUS_DEVICE uint32_t top16(const uint32_t* r) {
   uint32_t top = 0;
   if (sizeof(T) == 2) {  // two 16-bit magnitudes at a time
 #pragma unroll
@@ -48,12 +53,30 @@ FUS_DEVICE uint32_t load16(const T* p, bool vec, float* f) {
     return __float_as_uint(to_f(*reinterpret_cast<const T*>(&m)));
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+  for (int i = 0; i < 16; ++i) top = max(top, r[i] & 0x7fffffffu);
   return top;
 }
 
+// element j, by selection (no indexed registers)
+template <typename T>
+FUS_DEVICE float pick16(const uint32_t* r, int j) {
+  constexpr int W = 8 * sizeof(T) / 2;  // words
+  const int w = sizeof(T) == 2 ? j >> 1 : j;
+  uint32_t v[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] = r[i];
+#pragma unroll
+  for (int n = W / 2, bit = W / 2; n > 0; n >>= 1, bit >>= 1)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = w & bit ? v[i + n] : v[i];
+  if (sizeof(T) == 2) v[0] >>= 16 * (j & 1);
+  return to_f(*reinterpret_cast<const T*>(v));
+}
+
 // eight e2m1 codes of f * m, the first in the low four bits
-FUS_DEVICE uint32_t cvt8(const float* f, float m) {
+template <typename T>
+FUS_DEVICE uint32_t cvt8(const uint32_t* r, float m) {
+  const T* f = reinterpret_cast<const T*>(r);
   uint32_t v;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -62,122 +85,194 @@ FUS_DEVICE uint32_t cvt8(const float* f, float m) {
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(v)
-      : "f"(f[0] * m), "f"(f[1] * m), "f"(f[2] * m), "f"(f[3] * m), "f"(f[4] * m), "f"(f[5] * m),
-        "f"(f[6] * m), "f"(f[7] * m));
+      : "f"(to_f(f[0]) * m), "f"(to_f(f[1]) * m), "f"(to_f(f[2]) * m), "f"(to_f(f[3]) * m),
+        "f"(to_f(f[4]) * m), "f"(to_f(f[5]) * m), "f"(to_f(f[6]) * m), "f"(to_f(f[7]) * m));
   return v;
 }
 
-// e2m1 code of x over scale s*g, decided in fp64 (all products exact)
-FUS_DEVICE uint32_t code_exact(float x, double p) {
-  const double a = fabs((double)x);
-  uint32_t c = (a > 0.25 * p) + (a >= 0.75 * p) + (a > 1.25 * p) + (a >= 1.75 * p) +
-               (a > 2.5 * p) + (a >= 3.5 * p) + (a > 5.0 * p);
-  return c | (__float_as_uint(x) >> 31 << 3);
+// a > u g, or a = u g and `tie`: exact in fp32 where a is within 2^-20 of u g, u has a few
+// bits and u g is far from fp32's ends (the product's rounding error is one more fp32 number,
+// the difference is exact)
+FUS_DEVICE bool above(float a, float u, float g, bool tie) {
+  const float prod = u * g, err = fmaf(u, g, -prod), d = a - prod;
+  return d > err || (d == err && tie);
 }
 
-// eight of them
-FUS_DEVICE uint32_t code8_exact(const float* f, double p) {
-  uint32_t v = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) v |= code_exact(f[j], p) << (4 * j);
-  return v;
+FUS_DEVICE float rcp_approx(float v) {  // within 2^-23 of 1 / v
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
-// e4m3 byte nearest to a / (6 g), ties to even
-FUS_DEVICE uint32_t nv_scale(float a, float g) {
-  const float t = __fdividef(a, 6.0f * g);
+// e4m3 byte nearest to a / (6 g), ties to even; g is far from fp32's ends, inv6g = 1 / (6 g)
+FUS_DEVICE uint32_t nv_scale(float a, float g, float inv6g) {
+  const float t = a * inv6g;
   constexpr float kEps = 1.0f / (1 << 21);
   const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(t - t * kEps, t + t * kEps),
                                                 __NV_SATFINITE, __NV_E4M3);
-  uint32_t b0 = two & 0xff, b1 = two >> 8;
-  if (b0 != b1) {
-    const double m = 0.5 * ((double)fp4_scale_value<FUS_FP4_NV>(b0) +
-                            (double)fp4_scale_value<FUS_FP4_NV>(b1));
-    const double want = m * 6.0 * (double)g;
-    if ((double)a > want || ((double)a == want && (b1 & 1) == 0)) b0 = b1;
+  const uint32_t b0 = two & 0xff, b1 = two >> 8;
+  if (b0 == b1) return b0;
+  const float u = 3.0f * (fp4_scale_value<FUS_FP4_NV>(b0) + fp4_scale_value<FUS_FP4_NV>(b1));
+  return above(a, u, g, b0 & 1) ? b1 : b0;
+}
+// Byte and sixteen codes for a factor near fp32's ends (or not positive: zeros), in fp64: all
+// products below are exact there.
+template <typename T>
+FUS_DEVICE uint64_t nv_exact(const uint32_t* r, float a, float g, uint32_t* byte) {
+  uint32_t b = 126;  // the grid is monotone in the byte: step down to the nearest
+  while (b > 0) {
+    const double m = 3.0 * (double)g * ((double)fp4_scale_value<FUS_FP4_NV>(b) +
+                                        (double)fp4_scale_value<FUS_FP4_NV>(b - 1));
+    if ((double)a > m || ((double)a == m && (b & 1) == 0)) break;
+    --b;
   }
-  return b0;
+  *byte = b;
+  const double p = (double)fp4_scale_value<FUS_FP4_NV>(b) * (double)g;
+  uint64_t codes = 0;
+#pragma unroll 1
+  for (int j = 0; j < 16 && p > 0.0; ++j) {
+    const float f = pick16<T>(r, j);
+    const double v = fabs((double)f);
+    uint64_t c = (v > 0.25 * p) + (v >= 0.75 * p) + (v > 1.25 * p) + (v >= 1.75 * p) +
+                 (v > 2.5 * p) + (v >= 3.5 * p) + (v > 5.0 * p);
+    c |= (uint64_t)(__float_as_uint(f) >> 31) << 3;
+    codes |= c << (4 * j);
+  }
+  return codes;
 }
 
-// One thread quantises 16 elements; blockDim (UX, 256 / UX), UX a power of two >= 16 that
-// divides the row's padded K / 16, so a row's 256 elements are 16 neighbouring lanes and the
-// scale bytes of a cell, in four (NV) or eight (MX) of them, leave as one 4-byte store.
-// Bound: HBM (2.56 bytes an element from bf16); no index is divided, the tile is a shift.
+// sixteen codes of x / (s g): `lo` and `hi` are the codes a little below and above; where they
+// differ (by one) the border between them decides. A thread has one such element, rarely two:
+// they are visited one by one, not in sixteen tests.
+template <typename T>
+FUS_DEVICE uint64_t resolve16(uint64_t lo, uint64_t hi, const uint32_t* r, float s, float g) {
+  uint64_t differ = lo ^ hi;
+  while (differ) {
+    const int sh = (__ffsll((long long)differ) - 1) & ~3;
+    const uint32_t c = (uint32_t)(lo >> sh) & 7u;
+    const float border = c < 4 ? 0.25f + 0.5f * (float)c : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
+    const uint64_t mask = (uint64_t)15 << sh;
+    if (above(fabsf(pick16<T>(r, sh >> 2)), border * s, g, c & 1)) lo = (lo & ~mask) | (hi & mask);
+    differ &= ~mask;
+  }
+  return lo;
+}
+
+// One thread quantises 16 elements of `iters` rows; blockDim (UX, 256 / UX), UX a power of two
+// >= 16 that divides the row's padded K / 16, so a row's 256 elements are 16 neighbouring lanes
+// and the scale bytes of a cell, in four (NV) or eight (MX) of them, leave as one 4-byte store.
+// Bound: HBM (2.56 bytes an element from bf16) and, close behind, instruction issue: what
+// does not depend on the row is computed once for several rows.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
-    fp4_quantize_kernel(const T* __restrict__ x, long ldx, int x_rows, int rows,
+    fp4_quantize_kernel(const T* __restrict__ x, int ldx, int x_rows, int rows, int iters,
                         const int* __restrict__ ntp, const int* __restrict__ ids, int id_div,
                         int id_limit, int K, const float* __restrict__ gscale, int rows_per_g,
-                        int tile_log2, uint8_t* __restrict__ q, long ldq,
+                        int tile_log2, uint8_t* __restrict__ q, int ldq,
                         uint8_t* __restrict__ sf, int vec, int* status) {
   pdl_allow_dependents();
-  const int p = blockIdx.x * blockDim.y + threadIdx.y;
   const int k = (blockIdx.y * blockDim.x + threadIdx.x) * 16;
   const int used = ntp ? min(__ldg(ntp), rows) : rows;
-  bool live = p < used;
-  int src = p;
-  if (live && ids) {
-    const int id = __ldg(ids + p);
-    live = id >= 0 && id < id_limit;  // dispatch pads keep what their rows held
-    src = id_div > 1 ? id / id_div : id;
-    if (live && src >= x_rows) {
-      raise_status(status, FUS_ERR_CAPACITY);
-      live = false;
-    }
-  }
-  const bool data = live && k < K;
-  float f[16];
-  uint32_t top = 0;
-  if (data) {
-    top = load16(x + (long)src * ldx + k, vec, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = 0.f;
-  }
-  if (FMT == FUS_FP4_MX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  const bool bad = top >= 0x7f800000u;  // infinity or NaN in the block
-  uint32_t byte;
-  uint2 c;
-  if (FMT == FUS_FP4_MX) {
-    const int e = (int)(top >> 23) - 2;
-    byte = e > 0 ? e : 0;
-    const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
-    c = make_uint2(cvt8(f, inv), cvt8(f + 8, inv));
-    if (bad) byte = 255;
-  } else {
-    const float g =
-        gscale ? __ldg(gscale + (rows_per_g ? p / rows_per_g : 0)) : 1.0f;
-    byte = bad ? 0x7f : nv_scale(__uint_as_float(top), g);
-    const float s = fp4_scale_value<FUS_FP4_NV>(byte);
-    const float pr = s * g;
-    const float inv = __frcp_rn(pr);
-    constexpr float kLo = 1.0f - 1.0f / (1 << 21), kHi = 1.0f + 1.0f / (1 << 21);
-    c = make_uint2(cvt8(f, inv * kLo), cvt8(f + 8, inv * kLo));
-    const uint2 up = make_uint2(cvt8(f, inv * kHi), cvt8(f + 8, inv * kHi));
-    // next to a border, or a product near fp32's ends: decided in fp64
-    if (c.x != up.x || c.y != up.y || !(pr > 1e-30f && pr < 1e30f)) {
-      const double pd = (double)s * (double)g;
-      c = s > 0.f ? make_uint2(code8_exact(f, pd), code8_exact(f + 8, pd)) : make_uint2(0, 0);
-    }
-  }
-  if (bad) c = make_uint2(0, 0);
-  if (data) *reinterpret_cast<uint2*>(q + (long)p * ldq + k / 2) = c;
-  // scales: NV one byte of each lane, MX one of each lane pair; zeros past K
+  const int j0 = k / fp4_block(FMT);  // this thread's scale
+  const int tile = 1 << tile_log2;
+  const long per_tile = (long)gridDim.y * blockDim.x / 16 * fp4_stage_scale_bytes(FMT, tile);
   constexpr int kLanes = FMT == FUS_FP4_MX ? 8 : 4;
-  if (!data) byte = 0;
-  uint32_t word = byte << (8 * ((threadIdx.x / (kLanes / 4)) & 3));
+  const int shift = 8 * ((threadIdx.x / (kLanes / 4)) & 3);
+  uint8_t* cells = sf + fp4_scale_offset(tile, 0, j0 & ~3);
+  x += k;
+  q += k / 2;
+  float g = gscale && rows_per_g == 0 ? __ldg(gscale) : 1.0f;
+  float inv6g = 1.0f / (6.0f * g);
+  const int p0 = blockIdx.x * blockDim.y * iters + threadIdx.y;
+  constexpr int W = 8 * sizeof(T) / 2;
+  constexpr int HALF = W / 2;
+  // MX: the row after the one at work is on its way (24.8 -> 22.9 us at 8192 x 6144). NV needs the
+  // registers for occupancy instead (48.4 -> 40 us from fp32).
+  constexpr bool kAhead = FMT == FUS_FP4_MX;
+  uint32_t next[W];
+  bool next_live = false;
+  auto fetch = [&](int p) {
+    next_live = p < used;
+    int src = p;
+    if (next_live && ids) {
+      const int id = __ldg(ids + p);
+      next_live = id >= 0 && id < id_limit;  // dispatch pads keep what their rows held
+      src = id_div > 1 ? id / id_div : id;
+      if (next_live && src >= x_rows) {
+        raise_status(status, FUS_ERR_CAPACITY);
+        next_live = false;
+      }
+    }
+    if (next_live && k < K) {
+      load16(x + (long)src * ldx, vec, next);
+    } else {
 #pragma unroll
-  for (int o = kLanes / 4; o < kLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-  if (!live) return;
-  const int j0 = k / fp4_block(FMT);  // this block's scale
-  if (tile_log2 == 0) {
-    if (k < K && (FMT == FUS_FP4_NV || (threadIdx.x & 1) == 0))
-      sf[(long)p * (K / fp4_block(FMT)) + j0] = (uint8_t)byte;
-  } else if ((threadIdx.x & (kLanes - 1)) == 0) {
-    const int tile = 1 << tile_log2;
-    const long per_tile = (long)gridDim.y * blockDim.x / 16 * fp4_stage_scale_bytes(FMT, tile);
-    *reinterpret_cast<uint32_t*>(sf + (p >> tile_log2) * per_tile +
-                                 fp4_scale_offset(FMT, tile, p & (tile - 1), j0 & ~3)) = word;
+      for (int j = 0; j < W; ++j) next[j] = 0;
+    }
+  };
+  if (kAhead) fetch(p0);
+#pragma unroll 1
+  for (int i = 0; i < iters; ++i) {
+    const int p = p0 + i * blockDim.y;
+    if (!kAhead) fetch(p);
+    uint32_t f[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) f[j] = next[j];
+    const bool live = next_live;
+    const bool data = live && k < K;
+    if (kAhead && i + 1 < iters) fetch(p + blockDim.y);
+    uint32_t top = top16<T>(f);
+    if (FMT == FUS_FP4_MX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const bool bad = top >= 0x7f800000u;  // infinity or NaN in the block
+    uint32_t byte = 0;
+    uint2 c = make_uint2(0, 0);
+    if (FMT == FUS_FP4_MX) {
+      const int e = (int)(top >> 23) - 2;
+      byte = e > 0 ? e : 0;
+      const float inv = __uint_as_float((254u - byte) << 23);  // 2^(127 - byte)
+      c = make_uint2(cvt8<T>(f, inv), cvt8<T>(f + HALF, inv));
+    } else if (data) {
+      if (rows_per_g) {
+        g = __ldg(gscale + p / rows_per_g);
+        inv6g = 1.0f / (6.0f * g);
+      }
+      const float a = bad ? 0.f : __uint_as_float(top);
+      if (g > 1e-30f && g < 1e30f) {
+        byte = nv_scale(a, g, inv6g);
+        const float s = fp4_scale_value<FUS_FP4_NV>(byte);
+        // s = 0 only for magnitudes below 6 g 2^-10: their codes are zeros
+        const float inv = s > 0.f ? rcp_approx(s * g) : 0.f;
+        constexpr float kLo = 1.0f - 1.0f / (1 << 21), kHi = 1.0f + 1.0f / (1 << 21);
+        c = make_uint2(cvt8<T>(f, inv * kLo), cvt8<T>(f + HALF, inv * kLo));
+        const uint2 up = make_uint2(cvt8<T>(f, inv * kHi), cvt8<T>(f + HALF, inv * kHi));
+        if ((c.x != up.x || c.y != up.y) && !bad) {
+          const uint64_t r = resolve16<T>((uint64_t)c.y << 32 | c.x,
+                                          (uint64_t)up.y << 32 | up.x, f, s, g);
+          c = make_uint2((uint32_t)r, (uint32_t)(r >> 32));
+        }
+      } else {
+        const uint64_t r = nv_exact<T>(f, a, g, &byte);
+        c = make_uint2((uint32_t)r, (uint32_t)(r >> 32));
+      }
+    }
+    if (bad) {
+      byte = FMT == FUS_FP4_MX ? 255 : 127;
+      c = make_uint2(0, 0);
+    }
+    if (data) *reinterpret_cast<uint2*>(q + (long)p * ldq) = c;
+    // scales: NV one byte of each lane, MX one of each lane pair; zeros past K
+    if (!data) byte = 0;
+    uint32_t word = byte << shift;
+#pragma unroll
+    for (int o = kLanes / 4; o < kLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+    if (!live) continue;
+    if (tile_log2 == 0) {
+      if (k < K && (FMT == FUS_FP4_NV || (threadIdx.x & 1) == 0))
+        sf[(long)p * (K / fp4_block(FMT)) + j0] = (uint8_t)byte;
+    } else if ((threadIdx.x & (kLanes - 1)) == 0) {
+      *reinterpret_cast<uint32_t*>(cells + (p >> tile_log2) * per_tile +
+                                   fp4_row_offset(p & (tile - 1))) = word;
+    }
   }
 }
 
@@ -190,41 +285,57 @@ FUS_DEVICE void st32(void* p, const uint32_t* r) {  // 32 bytes in one store
 // The reverse, by the same threads.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256)
-    fp4_dequantize_kernel(const uint8_t* __restrict__ q, long ldq, const uint8_t* __restrict__ sf,
-                          int tile_log2, int rows, int K, const float* __restrict__ gscale,
-                          int rows_per_g, T* __restrict__ out, long ldo, int vec) {
-  const int p = blockIdx.x * blockDim.y + threadIdx.y;
+    fp4_dequantize_kernel(const uint8_t* __restrict__ q, int ldq, const uint8_t* __restrict__ sf,
+                          int tile_log2, int rows, int iters, int K,
+                          const float* __restrict__ gscale, int rows_per_g, T* __restrict__ out,
+                          int ldo, int vec) {
   const int k = (blockIdx.y * blockDim.x + threadIdx.x) * 16;
-  if (p >= rows || k >= K) return;
-  const uint2 v = *reinterpret_cast<const uint2*>(q + (long)p * ldq + k / 2);
+  if (k >= K) return;
   const int j0 = k / fp4_block(FMT);
   const int tile = 1 << tile_log2;
   const long per_tile = (long)gridDim.y * blockDim.x / 16 * fp4_stage_scale_bytes(FMT, tile);
-  const uint32_t byte =
-      tile_log2 == 0 ? sf[(long)p * (K / fp4_block(FMT)) + j0]
-                     : sf[(p >> tile_log2) * per_tile +
-                          fp4_scale_offset(FMT, tile, p & (tile - 1), j0)];
-  const float s = fp4_scale_value<FMT>(byte);
-  const float g =
-      FMT == FUS_FP4_NV && gscale ? __ldg(gscale + (rows_per_g ? p / rows_per_g : 0)) : 1.0f;
-  uint32_t o[8 * sizeof(T) / 2];
-  T* e = reinterpret_cast<T*>(o);
+  const int n_scales = K / fp4_block(FMT);
+  sf += tile_log2 ? fp4_scale_offset(tile, 0, j0) : j0;
+  q += k / 2;
+  out += k;
+  float m = FMT == FUS_FP4_NV && gscale && rows_per_g == 0 ? __ldg(gscale) : 1.0f;
+  const int p0 = blockIdx.x * blockDim.y * iters + threadIdx.y;
+#pragma unroll 2
+  for (int i = 0; i < iters; ++i) {
+    const int p = p0 + i * blockDim.y;
+    if (p >= rows) return;
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(q + (long)p * ldq));
+    const uint32_t byte = __ldg(sf + (tile_log2 ? (p >> tile_log2) * per_tile + fp4_row_offset(p & (tile - 1))
+                                                : (long)p * n_scales));
+    uint32_t o[8 * sizeof(T) / 2];
+    T* e = reinterpret_cast<T*>(o);
+    __half2 hs;
+    if (FMT == FUS_FP4_MX) {
+      m = fp4_scale_value<FMT>(byte);
+    } else {
+      if (rows_per_g) m = __ldg(gscale + p / rows_per_g);
+      const __half_raw r = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
+      hs = __half2half2(*reinterpret_cast<const __half*>(&r));
+    }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(
-        (__nv_fp4x2_storage_t)((j < 4 ? v.x >> (8 * j) : v.y >> (8 * (j - 4))) & 0xff), __NV_E2M1);
-    const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    // value x scale has at most 6 bits: exact; the factor rounds once, the type once
-    e[2 * j] = from_f<T>(w.x * s * g);
-    e[2 * j + 1] = from_f<T>(w.y * s * g);
-  }
-  T* dst = out + (long)p * ldo + k;
-  if (vec) {
+    for (int j = 0; j < 8; ++j) {
+      const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(
+          (__nv_fp4x2_storage_t)((j < 4 ? v.x >> (8 * j) : v.y >> (8 * (j - 4))) & 0xff), __NV_E2M1);
+      __half2 w = *reinterpret_cast<const __half2*>(&h);
+      // value x scale is exact (NV: 6 bits, in fp16); the factor rounds once, the type once
+      if (FMT == FUS_FP4_NV) w = __hmul2(w, hs);
+      const float2 wf = __half22float2(w);
+      e[2 * j] = from_f<T>(wf.x * m);
+      e[2 * j + 1] = from_f<T>(wf.y * m);
+    }
+    T* dst = out + (long)p * ldo;
+    if (vec) {
 #pragma unroll
-    for (int j = 0; j < (int)sizeof(T) / 2; ++j) st32(reinterpret_cast<char*>(dst) + 32 * j, o + 8 * j);
-  } else {
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) st32(reinterpret_cast<char*>(dst) + 32 * j, o + 8 * j);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) dst[j] = e[j];
+      for (int j = 0; j < 16; ++j) dst[j] = e[j];
+    }
   }
 }
 
@@ -268,13 +379,18 @@ int log2_of(int tile) {
   return n;
 }
 
-// threads over the rows, padded to whole stages of K: (UX, 256 / UX), see the kernel
-void shape_of(long rows, int K, dim3& grid, dim3& block) {
+// Threads over the rows, padded to whole stages of K: (UX, 256 / UX), see the kernel. Up to
+// eight rows for a thread while eight CTAs remain for each SM.
+int shape_of(long rows, int K, dim3& grid, dim3& block) {
   const int per_row = (int)(fp4_stages(K) * (kFp4StageK / 16));
   int ux = 16;
   while (ux < 128 && per_row % (2 * ux) == 0) ux *= 2;
   block = dim3(ux, 256 / ux);
-  grid = dim3((unsigned)((rows + block.y - 1) / block.y), per_row / ux);
+  const long blocks = (rows + block.y - 1) / block.y;
+  int iters = 1;
+  while (iters < 8 && blocks * (per_row / ux) / (2 * iters) >= 8 * 148) iters *= 2;
+  grid = dim3((unsigned)((blocks + iters - 1) / iters), per_row / ux);
+  return iters;
 }
 
 template <typename T>
@@ -283,13 +399,13 @@ int quantize_launch(const void* x, long ldx, int x_rows, long rows, const int* n
                     long rows_per_g, int tile, void* q, long ldq, void* sf, cudaStream_t st,
                     int* status) {
   dim3 grid, block;
-  shape_of(rows, K, grid, block);
+  const int iters = shape_of(rows, K, grid, block);
   const int vec = (reinterpret_cast<uintptr_t>(x) % 32) == 0 && (ldx * (long)sizeof(T)) % 32 == 0;
   auto fn = fmt == FUS_FP4_MX ? fp4_quantize_kernel<T, FUS_FP4_MX> : fp4_quantize_kernel<T, FUS_FP4_NV>;
-  fn<<<grid, block, 0, st>>>(reinterpret_cast<const T*>(x), ldx, x_rows, (int)rows, ntp, ids, id_div,
-                             id_limit, K, gscale, (int)rows_per_g, log2_of(tile),
-                             reinterpret_cast<uint8_t*>(q), ldq, reinterpret_cast<uint8_t*>(sf), vec,
-                             status);
+  fn<<<grid, block, 0, st>>>(reinterpret_cast<const T*>(x), (int)ldx, x_rows, (int)rows, iters, ntp,
+                             ids, id_div, id_limit, K, gscale, (int)rows_per_g, log2_of(tile),
+                             reinterpret_cast<uint8_t*>(q), (int)ldq,
+                             reinterpret_cast<uint8_t*>(sf), vec, status);
   return check_launch("fp4_quantize");
 }
 
@@ -297,12 +413,12 @@ template <typename T>
 int dequantize_launch(const void* q, long ldq, const void* sf, int fmt, int tile, long rows, int K,
                       const float* gscale, long rows_per_g, void* out, long ldo, cudaStream_t st) {
   dim3 grid, block;
-  shape_of(rows, K, grid, block);
+  const int iters = shape_of(rows, K, grid, block);
   const int vec = (reinterpret_cast<uintptr_t>(out) % 32) == 0 && (ldo * (long)sizeof(T)) % 32 == 0;
   auto fn = fmt == FUS_FP4_MX ? fp4_dequantize_kernel<T, FUS_FP4_MX> : fp4_dequantize_kernel<T, FUS_FP4_NV>;
-  fn<<<grid, block, 0, st>>>(reinterpret_cast<const uint8_t*>(q), ldq,
-                             reinterpret_cast<const uint8_t*>(sf), log2_of(tile), (int)rows, K, gscale,
-                             (int)rows_per_g, reinterpret_cast<T*>(out), ldo, vec);
+  fn<<<grid, block, 0, st>>>(reinterpret_cast<const uint8_t*>(q), (int)ldq,
+                             reinterpret_cast<const uint8_t*>(sf), log2_of(tile), (int)rows, iters, K,
+                             gscale, (int)rows_per_g, reinterpret_cast<T*>(out), (int)ldo, vec);
   return check_launch("fp4_dequantize");
 }
 
@@ -338,14 +454,14 @@ extern "C" int fus_fp4_quantize(const void* x, int dtype, long ldx, int x_rows, 
   if (int rc = check_common("fp4_quantize", fmt, dtype, rows, K, tile)) return rc;
   if (rows == 0) return FUS_OK;
   if (!x || !q || !sf) return set_error(FUS_E_INVALID, "fp4_quantize: null pointer");
-  if (x_rows < 1 || ldx < K) return set_error(FUS_E_INVALID, "fp4_quantize: bad source rows");
+  if (x_rows < 1 || ldx < K || ldx > 0x7fffffffL) return set_error(FUS_E_INVALID, "fp4_quantize: bad source rows");
   if (!ids && rows > x_rows)
     return set_error(FUS_E_INVALID, "fp4_quantize: %ld rows of %d", rows, x_rows);
   if (ids && (id_div < 1 || id_limit < 0))
     return set_error(FUS_E_INVALID, "fp4_quantize: bad id_div / id_limit");
   if (reinterpret_cast<uintptr_t>(x) % dtype_size(dtype))
     return set_error(FUS_E_INVALID, "fp4_quantize: misaligned source");
-  if (ldq < K / 2 || ldq % 16 || !aligned16(q) || !aligned16(sf))
+  if (ldq < K / 2 || ldq > 0x7fffffffL || ldq % 16 || !aligned16(q) || !aligned16(sf))
     return set_error(FUS_E_INVALID, "fp4_quantize: packed rows must be 16-byte aligned");
   if (rows_per_g < 0 || rows_per_g > 0x7fffffffL) return set_error(FUS_E_INVALID, "fp4_quantize: bad rows_per_g");
   if (fmt == FUS_FP4_MX && gscale)
@@ -367,9 +483,9 @@ extern "C" int fus_fp4_dequantize(const void* q, long ldq, const void* sf, int f
   if (int rc = check_common("fp4_dequantize", fmt, dtype, rows, K, tile)) return rc;
   if (rows == 0) return FUS_OK;
   if (!q || !sf || !out) return set_error(FUS_E_INVALID, "fp4_dequantize: null pointer");
-  if (ldq < K / 2 || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8)
+  if (ldq < K / 2 || ldq > 0x7fffffffL || ldq % 8 || reinterpret_cast<uintptr_t>(q) % 8)
     return set_error(FUS_E_INVALID, "fp4_dequantize: packed rows must be 8-byte aligned");
-  if (ldo < K || reinterpret_cast<uintptr_t>(out) % dtype_size(dtype))
+  if (ldo < K || ldo > 0x7fffffffL || reinterpret_cast<uintptr_t>(out) % dtype_size(dtype))
     return set_error(FUS_E_INVALID, "fp4_dequantize: bad output rows");
   if (rows_per_g < 0 || rows_per_g > 0x7fffffffL) return set_error(FUS_E_INVALID, "fp4_dequantize: bad rows_per_g");
   if (fmt == FUS_FP4_MX && gscale)

@@ -40,10 +40,13 @@ __host__ __device__ constexpr int fp4_atoms(int tile) { return tile > 128 ? tile
 __host__ __device__ constexpr int fp4_stage_scale_bytes(int fmt, int tile) {
   return fp4_cells(fmt) * fp4_atoms(tile) * 512;
 }
-// byte offset of scale j (of the whole row) of row r within its tile
-FUS_DEVICE long fp4_scale_offset(int fmt, int tile, int r, int j) {
-  const int A = fp4_atoms(tile);
-  return ((long)(j >> 2) * A + (r >> 7)) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4 + (j & 3);
+// byte offset of scale j (of the whole row) of row r within its tile: a row's part and a
+// scale's part
+FUS_DEVICE int fp4_row_offset(int r) {
+  return (r >> 7) * 512 + (r & 31) * 16 + ((r & 127) >> 5) * 4;
+}
+FUS_DEVICE long fp4_scale_offset(int tile, int r, int j) {
+  return (long)(j >> 2) * fp4_atoms(tile) * 512 + fp4_row_offset(r) + (j & 3);
 }
 
 // value of a scale byte, fp32 (exact)
