@@ -12,11 +12,15 @@
 //
 // A CTA loops over (block, weight tile) units with one continuous ring of stages (256 K
 // elements = 128 bytes of a row):
-//   warp 0  : producer, one lane: TMA boxes of weights and token rows (128-byte swizzle), one
-//             bulk copy each of their scale atoms
-//   warp 1  : TMEM owner; one lane copies a stage's scales into tensor memory (tcgen05.cp, in
-//             order with the MMAs of the same thread) and issues four K = 64 MMAs
-//   warps 2-5: epilogue, TMEM -> registers -> shared (token-major) -> 16-byte stores
+//   warp 0  : producer, one lane: TMA boxes of weights and token rows (128-byte swizzle; only
+//             the 64-row boxes that hold live rows), one bulk copy each of their scale atoms
+//   warp 1  : TMEM owner; one lane issues a stage's four K = 64 MMAs
+//   warp 2  : one lane copies a stage's scales into tensor memory (tcgen05.cp) ahead of the
+//             MMAs, into one of two buffers. Issued by the MMA thread they would run in order
+//             with the MMAs, about 55 cycles each: 12 of them for 512 cycles of MMA (dense
+//             8192 x 4096 x 6144 NV: 290 -> 230 us with 128-token blocks)
+//   warps 4-11 (4-7 up to 64 token columns): epilogue, two groups that take chunks of 32 columns
+//             in turn, TMEM -> registers -> shared (token-major) -> 16-byte stores
 // Up to 128 token columns the accumulator is double-buffered: the next unit's MMAs run while
 // the epilogue drains.
 #include "fp4.cuh"
@@ -52,8 +56,7 @@ struct Fp4Args {
   int* status;
 };
 
-constexpr int kThreads = 192;
-constexpr int kEpiThreads = 128;
+constexpr int kGroupThreads = 128;  // an epilogue group: the four lane quarters of TMEM
 
 template <int BN, int FMT>
 struct Cfg {
@@ -65,15 +68,19 @@ struct Cfg {
   static constexpr int SFB_BYTES = CELLS * ATOMS * 512;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int CHUNK = BN < 32 ? BN : 32;  // token columns of an epilogue step
-  static constexpr int EPI_BYTES = CHUNK * 128 * 4;
+  static constexpr int GROUPS = BN > 64 ? 2 : 1;
+  static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
+  static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);  // staging, row numbers
+  static constexpr int BOX = BN < 64 ? BN : 64;  // token rows of a TMA box
   // two CTAs for an SM up to 64 token columns (TMEM 256 columns each), else one
   static constexpr int CTAS = BN <= 64 ? 2 : 1;
   static constexpr int RING_TARGET = (CTAS == 2 ? 112 : 226) * 1024 - EPI_BYTES - 1280;
   static constexpr int STAGES = RING_TARGET / STAGE_BYTES > 8 ? 8 : RING_TARGET / STAGE_BYTES;
   static constexpr int ACCS = BN <= 128 ? 2 : 1;
-  static constexpr int SFA_COL = ACCS * BN;
-  static constexpr int SFB_COL = SFA_COL + CELLS * 4;
-  static constexpr int COLS = SFB_COL + CELLS * ATOMS * 4;
+  static constexpr int SFB_OFF = CELLS * 4;                      // token scales, after the weights'
+  static constexpr int SF_COLS = SFB_OFF + CELLS * ATOMS * 4;    // one of two scale buffers
+  static constexpr int SF_COL = ACCS * BN;
+  static constexpr int COLS = SF_COL + 2 * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
   static_assert(STAGES >= 3 && CTAS * TMEM_COLS <= 512 && COLS <= 512, "resources");
@@ -119,7 +126,7 @@ FUS_DEVICE void tc_cp_scales(uint32_t taddr, uint32_t saddr) {
 }
 
 template <int BN, int FMT, bool SWIGLU>
-__global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
+__global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
                     const __grid_constant__ Fp4Args a) {
   using C = Cfg<BN, FMT>;
@@ -131,13 +138,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
   const uint32_t sB = sA + STAGES * C::A_BYTES;
   const uint32_t sSA = sB + STAGES * C::B_BYTES;
   const uint32_t sSB = sSA + STAGES * C::SFA_BYTES;
-  float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES);  // [CHUNK][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + C::EPI_BYTES);
   const uint32_t bar_full = smem_u32(bars);
   const uint32_t bar_empty = bar_full + 8 * STAGES;
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // accumulator finished
   const uint32_t bar_free = bar_acc + 8 * C::ACCS;   // accumulator drained
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * C::ACCS);
+  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // scales are in tensor memory
+  const uint32_t bar_sf_free = bar_sf + 16;          // their MMAs are done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * C::ACCS + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -148,7 +156,11 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(bar_acc + 8 * b, 1);
-      mbar_init(bar_free + 8 * b, 4);
+      mbar_init(bar_free + 8 * b, 4 * C::GROUPS);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_sf + 8 * b, 1);
+      mbar_init(bar_sf_free + 8 * b, 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -173,23 +185,35 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
     raise_status(a.status, FUS_ERR_BAD_EXPERT);
     return -1;
   };
+  // live columns of a block (whole warp): dispatch pads end it
+  auto live_of = [&](int blk) {
+    int live = 0;
+    for (int j = lane; j < BN; j += 32) {
+      const int pos = blk * BN + j;
+      live += pos < rows_used && (!a.live_ids || __ldg(a.live_ids + pos) < a.live_limit);
+    }
+    return __reduce_add_sync(0xffffffffu, live);
+  };
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint64_t pol_w = a.stream_w ? policy_evict_first() : policy_evict_normal();
-      const uint64_t pol_x = policy_evict_last();
-      int it = 0;  // stages issued
-      bool waited = a.pdl == 0;
-      bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
-        const int e = expert_of(blk);
-        if (e < 0) continue;
+    const uint64_t pol_w = a.stream_w ? policy_evict_first() : policy_evict_normal();
+    const uint64_t pol_x = policy_evict_last();
+    int it = 0;  // stages issued
+    bool waited = a.pdl == 0;
+    int ok = 1;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
+      const int e = expert_of(blk);
+      if (e < 0) continue;
+      const int boxes = BN > 64 ? max(1, (live_of(blk) + 63) / 64) : 1;
+      if (lane == 0) {
         const uint8_t* wsf = a.wsf + ((long)e * a.m_tiles + mt) * a.nst * C::SFA_BYTES;
         const uint8_t* xsf = a.xsf + (long)blk * a.nst * C::SFB_BYTES;
+        const uint32_t bytes =
+            C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + boxes * C::BOX * 128;
         auto load_w = [&](int s, int k) {
           const uint32_t full = bar_full + 8 * s;
-          mbar_arrive_expect_tx(full, C::STAGE_BYTES);
+          mbar_arrive_expect_tx(full, bytes);
           if (SWIGLU) {
             const int r = e * a.w_rows + mt * 64;
             tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, r, pol_w);
@@ -202,7 +226,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
         };
         auto load_x = [&](int s, int k) {
           const uint32_t full = bar_full + 8 * s;
-          tma_load_2d(sB + s * C::B_BYTES, &tx, full, k * 128, blk * BN, pol_x);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(sB + s * C::B_BYTES + b * C::BOX * 128, &tx, full, k * 128,
+                        blk * BN + b * C::BOX, pol_x);
           bulk_load(sSB + s * C::SFB_BYTES, xsf + (long)k * C::SFB_BYTES, C::SFB_BYTES, full, pol_x);
         };
         int k0 = 0;
@@ -219,45 +245,35 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
         for (int k = k0; k < a.nst; ++k, ++it) {
           const int s = it % STAGES;
           if (!mbar_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
-            ok = false;
+            ok = 0;
             break;
           }
           load_w(s, k);
           load_x(s, k);
         }
       }
-      if (!waited) pdl_wait();
+      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
+    if (lane == 0 && !waited) pdl_wait();
   } else if (warp == 1) {
     int it = 0, n = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    int ok = 1;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const int blk = u / a.m_tiles;
       if (expert_of(blk) < 0) continue;
-      // live columns: dispatch pads end a block
-      int live = 0;
-      for (int j = lane; j < BN; j += 32) {
-        const int pos = blk * BN + j;
-        live += pos < rows_used && (!a.live_ids || __ldg(a.live_ids + pos) < a.live_limit);
-      }
-      live = __reduce_add_sync(0xffffffffu, live);
-      const int nm = max(16, (live + 15) & ~15);
-      int ok = 1;
+      const int nm = max(16, (live_of(blk) + 15) & ~15);
       if (lane == 0) {
         const int buf = n % C::ACCS;
         ok = mbar_wait_bounded(bar_free + 8 * buf, ((n / C::ACCS) & 1) ^ 1, abort_flag, a.status);
         tc_fence_after();
         const uint32_t acc = tmem + buf * BN;
         for (int k = 0; k < a.nst && ok; ++k, ++it) {
-          const int s = it % STAGES;
-          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+          const int s = it % STAGES, b = it & 1;
+          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
+               mbar_wait_bounded(bar_sf + 8 * b, (it >> 1) & 1, abort_flag, a.status);
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < C::CELLS; ++c)
-            tc_cp_scales(tmem + C::SFA_COL + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
-#pragma unroll
-          for (int c = 0; c < C::CELLS * C::ATOMS; ++c)
-            tc_cp_scales(tmem + C::SFB_COL + 4 * c, sSB + s * C::SFB_BYTES + 512 * c);
+          const uint32_t sf = tmem + C::SF_COL + b * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -266,57 +282,92 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
               const int id = FMT == FUS_FP4_MX ? (j % 2) * 2 : 0;
               tc_mma_fp4<FMT>(acc, sw128_desc(sA + s * C::A_BYTES + 32 * j),
                               sw128_desc(sB + s * C::B_BYTES + 32 * j), fp4_idesc<FMT>(nm, id),
-                              tmem + C::SFA_COL + 4 * cell,
-                              tmem + C::SFB_COL + 4 * C::ATOMS * cell, (k | j) != 0);
+                              sf + 4 * cell, sf + C::SFB_OFF + 4 * C::ATOMS * cell, (k | j) != 0);
             }
           }
           tc_commit(bar_empty + 8 * s);
+          tc_commit(bar_sf_free + 8 * b);
         }
         if (ok) tc_commit(bar_acc + 8 * buf);
       }
       ++n;
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
     }
-  } else {
+  } else if (warp == 2) {
+    int it = 0;
+    int ok = 1;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+      const int blk = u / a.m_tiles;
+      if (expert_of(blk) < 0) continue;
+      // atoms of token scales that hold live rows
+      const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
+      if (lane == 0) {
+        for (int k = 0; k < a.nst; ++k, ++it) {
+          const int s = it % STAGES, b = it & 1;
+          ok = mbar_wait_bounded(bar_sf_free + 8 * b, ((it >> 1) & 1) ^ 1, abort_flag, a.status) &&
+               mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sf = tmem + C::SF_COL + b * C::SF_COLS;
+#pragma unroll
+          for (int c = 0; c < C::CELLS; ++c) {
+            tc_cp_scales(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
+#pragma unroll
+            for (int t = 0; t < C::ATOMS; ++t)
+              if (t < atoms)
+                tc_cp_scales(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
+                             sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
+          }
+          tc_commit(bar_sf + 8 * b);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+  } else if (warp >= 4) {
     const int q4 = warp & 3;  // the TMEM lanes this warp may read
+    const int grp = (warp - 4) >> 2;
     const int m = q4 * 32 + lane;
-    const int et = threadIdx.x - 64;
+    const int et = threadIdx.x - 128 - grp * kGroupThreads;
+    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
+    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
+                                        C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
     int n = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
       const int e = expert_of(blk);
       if (e < 0) continue;
-      int live = 0;
-      for (int j = lane; j < BN; j += 32) {
+      const int live = live_of(blk);
+      // output rows, out of range: -1 (read by this group only, after its barrier below)
+      for (int j = et; j < live; j += kGroupThreads) {
         const int pos = blk * BN + j;
-        live += pos < rows_used && (!a.live_ids || __ldg(a.live_ids + pos) < a.live_limit);
+        const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
+        s_row[j] = row < a.out_rows ? row : -1;
       }
-      live = __reduce_add_sync(0xffffffffu, live);
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
       const int buf = n % C::ACCS;
       if (!mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q4 * 32) << 16);
-      for (int c0 = 0; c0 < live; c0 += C::CHUNK) {
+      for (int c0 = grp * C::CHUNK; c0 < live; c0 += C::GROUPS * C::CHUNK) {
+        uint32_t v[C::CHUNK];
 #pragma unroll
-        for (int c = 0; c < C::CHUNK; c += 16) {
-          float v[16];
-          tmem_ld16(acc + c0 + c, v);
+        for (int c = 0; c < C::CHUNK; c += 16) tmem_ld16_issue(acc + c0 + c, v + c);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) S[(c + j) * 128 + m] = v[j] * alpha;
-        }
-        named_bar_sync(1, kEpiThreads);
+        for (int c = 0; c < C::CHUNK; c += 16) tmem_ld_wait(v + c);
+#pragma unroll
+        for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[j]) * alpha;
+        named_bar_sync(1 + grp, kGroupThreads);
         constexpr int PER = SWIGLU ? 8 : 16;  // threads of a token row, 8 features each
         const int nj = min(C::CHUNK, live - c0);
-        for (int i = et; i < nj * PER; i += kEpiThreads) {
-          const int j = i / PER, f = (i % PER) * 8;
-          const int pos = blk * BN + c0 + j;
-          const int id = a.live_ids ? __ldg(a.live_ids + pos) : pos;
-          const int row = a.scatter ? id : pos;
-          const int col = mt * (SWIGLU ? 64 : 128) + f;
-          if (col >= a.out_cols || row < 0 || row >= a.out_rows) continue;
+        const int f = (et % PER) * 8;
+        const int col = mt * (SWIGLU ? 64 : 128) + f;
+#pragma unroll
+        for (int j0 = 0; j0 < C::CHUNK; j0 += kGroupThreads / PER) {
+          const int j = j0 + et / PER;
+          if (j >= nj || col >= a.out_cols) continue;
+          const int row = s_row[c0 + j];
+          if (row < 0) continue;
           float o[8];
           *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(S + j * 128 + f);
           *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<const float4*>(S + j * 128 + f + 4);
@@ -343,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<BN, FMT>::CTAS))
                                       (long)row * a.ldo + col) = pack8(o);
           }
         }
-        named_bar_sync(1, kEpiThreads);
+        named_bar_sync(1 + grp, kGroupThreads);
       }
       tc_fence_before();
       __syncwarp();
@@ -369,7 +420,7 @@ int launch(const CUtensorMap& tw, const CUtensorMap& tx, const Fp4Args& a, long 
   const long slots = (long)num_sms() * C::CTAS;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units < slots ? units : slots));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -470,7 +521,7 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
                            (uint64_t)d->K / 2, 128, sw ? 64 : 128);
   if (!rc)
     rc = make_tmap_u8_2d(&tx, d->xq, (uint64_t)d->K / 2, (uint64_t)d->x_rows, (uint64_t)d->ldxq,
-                         128, d->block_n);
+                         128, d->block_n < 64 ? d->block_n : 64);
   if (rc) return rc;
   cudaStream_t st = as_stream(stream);
   if (d->fmt == FUS_FP4_MX)
