@@ -13,8 +13,9 @@
 // The ids are those of exact arithmetic on the logits. Without bias and groups the logits are
 // ranked themselves (the score is monotone in them). Otherwise fp32 scores rank, and where two
 // choices that decide something lie within their error of each other (a few tokens in a
-// thousand) the warp does the row again in fp64. The same path takes rows with more than 32
-// candidates (ties) or fewer than k finite choices.
+// thousand) the warp decides again in fp64: the groups from all choices, the experts from the
+// candidates alone, one for each lane. Rows with more than 32 candidates (ties) or fewer than k
+// finite choices go through k plain rounds in fp64.
 //
 // A logit of -infinity or NaN masks its expert; a slot for which no expert is left gets id -1
 // (a hole of the dispatch layout) and weight 0.
@@ -34,7 +35,8 @@ struct RouteArgs {
   int softmax;
   int n_group, topk_group;
   int gsz;   // experts of a group
-  int lpg;   // lanes of a group (a power of two)
+  int lpg;   // lanes of a group, 2^lpg_log2
+  int lpg_log2;
   int npl;   // experts of a lane
   float scale;
   int renorm;
@@ -43,7 +45,18 @@ struct RouteArgs {
 constexpr int kWarps = 4;
 constexpr unsigned kAll = 0xffffffffu;
 
-FUS_DEVICE float sigmoid_fast(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
+constexpr float kLog2e = 1.4426950408889634f;
+FUS_DEVICE float ex2(float v) {  // 2^v, within 2 ulp
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+FUS_DEVICE float rcp(float v) {  // 1 / v, within 1 ulp
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+FUS_DEVICE float sigmoid_fast(float l) { return rcp(1.0f + ex2(-kLog2e * l)); }
 
 // order-preserving unsigned key of a float
 FUS_DEVICE uint32_t key_of(float v) {
@@ -56,16 +69,15 @@ FUS_DEVICE float value_of(uint32_t k) {
 
 // a logit as the routing sees it: NaN and -infinity mask, +infinity is the largest number
 FUS_DEVICE float clean(float l) {
-  if (!(l > -INFINITY)) return -INFINITY;
-  return fminf(l, 3.402823466e38f);
+  return fminf(fmaxf(l, -INFINITY), 3.402823466e38f);  // fmaxf drops a NaN
 }
 
 // the whole row in fp64, k rounds; every lane returns after the row's outputs are written
 template <typename T>
 __device__ __noinline__ void route_row_exact(const RouteArgs& a, long t, int lane) {
   const T* row = reinterpret_cast<const T*>(a.logits) + t * a.ld;
-  const int group = lane / a.lpg;
-  const int e0 = group * a.gsz + (lane % a.lpg) * a.npl;
+  const int group = lane >> a.lpg_log2;
+  const int e0 = group * a.gsz + (lane & (a.lpg - 1)) * a.npl;
   const int n = group < a.n_group ? max(0, min(a.npl, (group + 1) * a.gsz - e0)) : 0;
   double top = -INFINITY;
   for (int j = 0; j < n; ++j) top = fmax(top, (double)clean(to_f(row[e0 + j])));
@@ -137,6 +149,7 @@ __device__ __noinline__ void route_row_exact(const RouteArgs& a, long t, int lan
     }
     if (!(best > -INFINITY)) break;
     if (id >= e0 && id < e0 + n) taken |= 1u << (id - e0);
+    // the owner's score, from its logit
     const double w = score(id);
     total += w;
     if (lane == s) {
@@ -151,17 +164,87 @@ __device__ __noinline__ void route_row_exact(const RouteArgs& a, long t, int lan
   }
 }
 
-template <typename T, int NPL>
+// What the fast path cannot tell apart, in fp64. These read the row again, so that the fast
+// path's values never need an address.
+struct ExactRow {
+  double sum;  // softmax denominator
+  float top;
+  bool softmax;
+  template <typename T>
+  FUS_DEVICE ExactRow(const RouteArgs& a, const T* row, int e0, int n, float t)
+      : sum(1.0), top(t), softmax(a.softmax) {
+    if (!softmax) return;
+    sum = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const float l = clean(to_f(row[e0 + j]));
+      if (l > -INFINITY) sum += exp((double)l - (double)top);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+  }
+  FUS_DEVICE double score(float l) const {
+    return softmax ? exp((double)l - (double)top) / sum : 1.0 / (1.0 + exp(-(double)l));
+  }
+};
+
+// rank of this lane's group among the groups
+template <typename T>
+__device__ __noinline__ int group_rank_exact(const RouteArgs& a, const T* row, float top, int e0,
+                                             int n, int group) {
+  const ExactRow x(a, row, e0, n, top);
+  double a1 = -INFINITY, a2 = -INFINITY;
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    const float l = clean(to_f(row[e0 + j]));
+    if (!(l > -INFINITY)) continue;
+    const double v = x.score(l) + (a.bias ? (double)__ldg(a.bias + e0 + j) : 0.0);
+    a2 = fmax(a2, fmin(a1, v));
+    a1 = fmax(a1, v);
+  }
+  for (int o = 1; o < a.lpg; o <<= 1) {
+    const double b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
+    a2 = fmax(fmin(a1, b1), fmax(a2, b2));
+    a1 = fmax(a1, b1);
+  }
+  const double g = a2 > -INFINITY ? a1 + a2 : a1;
+  int better = 0;
+  for (int q = 0; q < a.n_group; ++q) {
+    const double og = __shfl_sync(kAll, g, q * a.lpg);
+    better += og > g || (og == g && q < group);
+  }
+  return better;
+}
+
+// rank of this lane's candidate among `count`
+template <typename T>
+__device__ __noinline__ int rank_exact(const RouteArgs& a, const T* row, float top, int e0, int n,
+                                       float logit, int id, int count, int lane) {
+  const ExactRow x(a, row, e0, n, top);
+  double c = -INFINITY;
+  if (lane < count) c = x.score(logit) + (a.bias ? (double)__ldg(a.bias + id) : 0.0);
+  int rank = 0;
+  for (int q = 0; q < count; ++q) {
+    const double oc = __shfl_sync(kAll, c, q);
+    const int oi = __shfl_sync(kAll, id, q);
+    rank += oc > c || (oc == c && oi < id);
+  }
+  return rank;
+}
+
+template <typename T, int NPL, bool SOFTMAX, bool GROUPED>
 __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs a) {
-  __shared__ float2 cand[kWarps][32];  // (choice, logit)
-  __shared__ int cand_id[kWarps][32];
+  __shared__ __align__(16) float row_c[kWarps][NPL * 32], row_l[kWarps][NPL * 32];  // lane-major
+  __shared__ float2 cand[kWarps][32];                                 // (choice, id)
+  __shared__ float sorted[kWarps][33];
+  __shared__ int place[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long t = (long)blockIdx.x * kWarps + warp;
   if (t >= a.T) return;
   const T* row = reinterpret_cast<const T*>(a.logits) + t * a.ld;
-  const int group = lane / a.lpg;
-  const int e0 = group * a.gsz + (lane % a.lpg) * a.npl;
-  const int n = group < a.n_group ? max(0, min(a.npl, (group + 1) * a.gsz - e0)) : 0;
+  const int group = GROUPED ? lane >> a.lpg_log2 : 0;
+  const int e0 = GROUPED ? group * a.gsz + (lane & (a.lpg - 1)) * NPL : lane * NPL;
+  const int n = group < a.n_group ? max(0, min(NPL, (group + 1) * a.gsz - e0)) : 0;
   float l[NPL];
   // whole aligned runs of 16 bytes where the row allows
   constexpr int V = 16 / sizeof(T);
@@ -177,41 +260,65 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
 #pragma unroll
     for (int j = 0; j < NPL; ++j) l[j] = j < n ? clean(to_f(row[e0 + j])) : -INFINITY;
   }
-  float top = -INFINITY, sum = 1.f;
-  if (a.softmax) {
+  float top = 0.f, inv = 1.f;
+  if (SOFTMAX) {
+    top = l[0];
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) top = fmaxf(top, l[j]);
+    for (int j = 1; j < NPL; ++j) top = fmaxf(top, l[j]);
     top = value_of(__reduce_max_sync(kAll, key_of(top)));
-    sum = 0.f;
+    float sum = 0.f;
+    if (top > -INFINITY) {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) sum += l[j] > -INFINITY ? __expf(l[j] - top) : 0.f;
-    sum = warp_sum(sum);
+      for (int j = 0; j < NPL; ++j) sum += ex2(kLog2e * (l[j] - top));
+    }
+    inv = 1.0f / warp_sum(sum);
   }
-  // choices; `tol` bounds the error of a difference of two of them (scores up to 1, fast
-  // exponential and division, one addition)
-  const bool plain = !a.bias && a.n_group == 1;  // the logits rank themselves
+  auto score = [&](float v) {
+    return SOFTMAX ? ex2(kLog2e * (v - top)) * inv : sigmoid_fast(v);
+  };
+  // choices; `tol` bounds the error of a difference of two of them
+  const bool plain = !a.bias && !GROUPED;  // the logits rank themselves
   float c[NPL];
   float tol = 0.f;
-  bool again = false;
   if (plain) {
 #pragma unroll
     for (int j = 0; j < NPL; ++j) c[j] = l[j];
   } else {
-    const float inv = __fdividef(1.0f, sum);
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      float s = a.softmax ? __expf(l[j] - top) * inv : sigmoid_fast(l[j]);
-      if (a.bias && j < n) s += __ldg(a.bias + e0 + j);
-      c[j] = l[j] > -INFINITY ? s : -INFINITY;
+    for (int j = 0; j < NPL; ++j) c[j] = score(l[j]);
+    if (a.bias) {
+      if (NPL % 4 == 0 && n == NPL && ((uintptr_t)(a.bias + e0) & 15) == 0) {
+#pragma unroll
+        for (int j = 0; j < NPL; j += 4) {
+          const float4 b = __ldg(reinterpret_cast<const float4*>(a.bias + e0 + j));
+          c[j] += b.x;
+          c[j + 1] += b.y;
+          c[j + 2] += b.z;
+          c[j + 3] += b.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j)
+          if (j < n) c[j] += __ldg(a.bias + e0 + j);
+      }
     }
-    // softmax: the sum of up to 1024 terms adds some 2^-19 of a score
-    tol = a.softmax ? 8e-6f : 4e-6f;
-  }
-  float best = -INFINITY;
-  if (a.n_group > 1) {
-    float a1 = -INFINITY, a2 = -INFINITY;
+    float low = l[0];
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) {
+    for (int j = 1; j < NPL; ++j) low = fminf(low, l[j]);
+    if (!(low > -INFINITY)) {  // masked experts, and places past the group
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) c[j] = l[j] > -INFINITY ? c[j] : -INFINITY;
+    }
+    // sigmoid: an exponential within 2 ulp and its argument's rounding (1.2e-7 of s (1 - s) |l|,
+    // below 1e-7), the sum 6e-8, a reciprocal within 1.2e-7; the addition 6e-8 of the choice;
+    // all twice. softmax: the sum of up to 1024 terms adds some 2^-19 of a score.
+    tol = SOFTMAX ? 8e-6f : 9e-7f;
+  }
+  float best;
+  if (GROUPED) {
+    float a1 = c[0], a2 = -INFINITY;
+#pragma unroll
+    for (int j = 1; j < NPL; ++j) {
       a2 = fmaxf(a2, fminf(a1, c[j]));
       a1 = fmaxf(a1, c[j]);
     }
@@ -222,87 +329,131 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
       a1 = fmaxf(a1, b1);
     }
     const float g = a2 > -INFINITY ? a1 + a2 : a1;
-    const float gt = 2.f * tol * (1.f + fabsf(g));
     int better = 0;
-    bool near = false;
+#pragma unroll 4
     for (int q = 0; q < a.n_group; ++q) {
       const float og = __shfl_sync(kAll, g, q * a.lpg);
       better += og > g || (og == g && q < group);
-      near |= q != group && fabsf(og - g) <= gt;
     }
-    again = group < a.n_group && near && (better == a.topk_group - 1 || better == a.topk_group);
+    if (a.topk_group < a.n_group) {
+      // the last group in and the first one out: too near to tell apart in fp32?
+      const bool real = group < a.n_group;
+      const int in = __ffs(__ballot_sync(kAll, real && better == a.topk_group - 1)) - 1;
+      const int out = __ffs(__ballot_sync(kAll, real && better == a.topk_group)) - 1;
+      const float gi = __shfl_sync(kAll, g, in), go = __shfl_sync(kAll, g, out);
+      if (gi - go <= 2.f * tol * (1.f + fabsf(gi)))
+        better = group_rank_exact<T>(a, row, top, e0, n, group);
+    }
     if (better >= a.topk_group) {
       best = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NPL; ++j) c[j] = -INFINITY;
     }
   } else {
+    best = c[0];
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) best = fmaxf(best, c[j]);
+    for (int j = 1; j < NPL; ++j) best = fmaxf(best, c[j]);
   }
   // k-th largest lane maximum (equal maxima leave together: the bound only gets lower)
   uint32_t mine = key_of(best), bound = 0;
+#pragma unroll 4
   for (int s = 0; s < a.topk; ++s) {
     bound = __reduce_max_sync(kAll, mine);
     if (mine == bound) mine = 0;
   }
-  float limit = value_of(bound);
-  again |= !(bound > key_of(-INFINITY));  // fewer than k lanes with a finite choice
-  limit -= tol * (1.f + fabsf(limit));
-  int count = 0;
+  const float kth = value_of(bound);
+  const bool few = !(bound > key_of(-INFINITY));  // fewer than k lanes with a finite choice
+  const float limit = kth - tol * (1.f + fabsf(kth));
+  uint32_t left = 0;  // this lane's candidates
 #pragma unroll
-  for (int j = 0; j < NPL; ++j) {
-    const bool is = c[j] >= limit;
-    const unsigned m = __ballot_sync(kAll, is);
-    if (is) {
-      const int at = count + __popc(m & ((1u << lane) - 1));
-      if (at < 32) {
-        cand[warp][at] = make_float2(c[j], l[j]);
-        cand_id[warp][at] = e0 + j;
+  for (int j = 0; j < NPL; ++j) left |= c[j] >= limit ? 1u << j : 0u;
+  if (left) {
+    float* pc = &row_c[warp][lane * NPL];
+    float* pl = &row_l[warp][lane * NPL];
+    if (NPL % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j + 3 < NPL; j += 4) {
+        *reinterpret_cast<float4*>(pc + j) = make_float4(c[j], c[j + 1], c[j + 2], c[j + 3]);
+        *reinterpret_cast<float4*>(pl + j) = make_float4(l[j], l[j + 1], l[j + 2], l[j + 3]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) {
+        pc[j] = c[j];
+        pl[j] = l[j];
+      }
+    }
+  }
+  int count = 0;
+  for (unsigned m = __ballot_sync(kAll, left != 0); m; m = __ballot_sync(kAll, left != 0)) {
+    // the lanes of m put down one candidate each
+    if (left) {
+      const int slot = count + __popc(m & ((1u << lane) - 1));
+      if (slot < 32) place[warp][slot] = lane * NPL + __ffs(left) - 1;
+      left &= left - 1;
     }
     count += __popc(m);
   }
   __syncwarp();
-  if (__any_sync(kAll, again) || count > 32) {
+  if (few || count > 32) {
     route_row_exact<T>(a, t, lane);
     return;
   }
-  const float2 my = lane < count ? cand[warp][lane] : make_float2(-INFINITY, 0.f);
-  const int id = lane < count ? cand_id[warp][lane] : 0x7fffffff;
+  float choice = -INFINITY, logit = 0.f;
+  int id = 0x7fffffff;
+  if (lane < count) {
+    const int at = place[warp][lane];
+    choice = row_c[warp][at];
+    logit = row_l[warp][at];
+    const int from = at / NPL;
+    id = (GROUPED ? (from >> a.lpg_log2) * a.gsz + (from & (a.lpg - 1)) * NPL : from * NPL) + at % NPL;
+    cand[warp][lane] = make_float2(choice, __int_as_float(id));
+  }
+  __syncwarp();
   int rank = 0;
-  bool near = false;
-  const float my_tol = tol * (1.f + fabsf(my.x));
+#pragma unroll 4
   for (int q = 0; q < count; ++q) {
-    const float oc = cand[warp][q].x;
-    const int oi = cand_id[warp][q];
-    rank += oc > my.x || (oc == my.x && oi < id);
-    near |= oi != id && fabsf(oc - my.x) <= my_tol;
+    const float2 o = cand[warp][q];
+    rank += o.x > choice || (o.x == choice && __float_as_int(o.y) < id);
+  }
+  if (!plain) {
+    // neighbours in the order, the first one out among them, too near to tell apart?
+    if (lane < count) sorted[warp][rank] = choice;
+    if (lane == 0) sorted[warp][count] = -INFINITY;
+    __syncwarp();
+    const bool near = lane < count && rank < a.topk &&
+                      choice - sorted[warp][rank + 1] <= tol * (1.f + fabsf(choice));
+    if (__any_sync(kAll, near)) rank = rank_exact<T>(a, row, top, e0, n, logit, id, count, lane);
   }
   const bool chosen = lane < count && rank < a.topk;
-  if (__any_sync(kAll, chosen && near && !plain)) {
-    route_row_exact<T>(a, t, lane);
-    return;
-  }
-  float w = 0.f;
-  if (chosen)
-    w = a.softmax ? expf(my.y - top) / sum : 1.0f / (1.0f + expf(-my.y));
-  if (a.renorm) w = w / fmaxf(warp_sum(w), 1e-20f);
+  float w = chosen ? score(logit) : 0.f;
+  if (a.renorm) w = __fdividef(w, fmaxf(warp_sum(w), 1e-20f));
   if (chosen) {
     a.topw[t * a.topk + rank] = w * a.scale;
     a.topi[t * a.topk + rank] = id;
   }
 }
 
+template <typename T, int NPL>
+void launch_npl(const RouteArgs& a, cudaStream_t st) {
+  const int grid = (a.T + kWarps - 1) / kWarps;
+  auto fn = a.softmax ? (a.n_group > 1 ? route_topk_kernel<T, NPL, true, true>
+                                       : route_topk_kernel<T, NPL, true, false>)
+                      : (a.n_group > 1 ? route_topk_kernel<T, NPL, false, true>
+                                       : route_topk_kernel<T, NPL, false, false>);
+  fn<<<grid, kWarps * 32, 0, st>>>(a);
+}
+
 template <typename T>
 int launch_route(const RouteArgs& a, cudaStream_t st) {
-  const int grid = (a.T + kWarps - 1) / kWarps;
-  if (a.npl <= 1) route_topk_kernel<T, 1><<<grid, kWarps * 32, 0, st>>>(a);
-  else if (a.npl <= 2) route_topk_kernel<T, 2><<<grid, kWarps * 32, 0, st>>>(a);
-  else if (a.npl <= 4) route_topk_kernel<T, 4><<<grid, kWarps * 32, 0, st>>>(a);
-  else if (a.npl <= 8) route_topk_kernel<T, 8><<<grid, kWarps * 32, 0, st>>>(a);
-  else if (a.npl <= 16) route_topk_kernel<T, 16><<<grid, kWarps * 32, 0, st>>>(a);
-  else route_topk_kernel<T, 32><<<grid, kWarps * 32, 0, st>>>(a);
+  switch (a.npl) {
+    case 1: launch_npl<T, 1>(a, st); break;
+    case 2: launch_npl<T, 2>(a, st); break;
+    case 4: launch_npl<T, 4>(a, st); break;
+    case 8: launch_npl<T, 8>(a, st); break;
+    case 16: launch_npl<T, 16>(a, st); break;
+    default: launch_npl<T, 32>(a, st); break;
+  }
   return check_launch("route_topk");
 }
 
@@ -330,7 +481,11 @@ extern "C" int fus_route_topk(const void* logits, int dtype, long ld, const floa
   RouteArgs a{};
   a.gsz = E / n_group;
   a.lpg = 32;
-  while (a.lpg * n_group > 32) a.lpg >>= 1;
+  a.lpg_log2 = 5;
+  while (a.lpg * n_group > 32) {
+    a.lpg >>= 1;
+    --a.lpg_log2;
+  }
   a.npl = (a.gsz + a.lpg - 1) / a.lpg;
   if (a.npl > 32) return set_error(FUS_E_UNSUPPORTED, "route_topk: E=%d too many experts", E);
   // 16-byte loads want whole runs: a power of two of experts for a lane
