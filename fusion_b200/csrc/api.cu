@@ -88,7 +88,7 @@ int make_tmap_bf16_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
 }
 
 int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
-                    uint32_t box_inner, uint32_t box_rows) {
+                    uint32_t box_inner, uint32_t box_rows, bool swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(FUS_E_LAUNCH, "cuTensorMapEncodeTiled unavailable");
   if (!aligned16(base) || ld % 16)
@@ -98,7 +98,7 @@ int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t r
   cuuint32_t box[2] = {box_inner, box_rows};
   cuuint32_t es[2] = {1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                  es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(FUS_E_INVALID, "cuTensorMapEncodeTiled failed (%d): inner=%llu rows=%llu",

@@ -90,9 +90,9 @@ struct Cfg {
 // type (1 = e2m1), 17-22 N >> 3, 23 scale type (1 = e8m0, 0 = e4m3), 24-28 M >> 4, 29-30 A
 // scale id (which bytes of the 32-bit scale cell this MMA reads: 0 or 2 for scale_vec::2X)
 template <int FMT>
-FUS_DEVICE uint32_t fp4_idesc(int n, int id) {
+FUS_DEVICE uint32_t fp4_idesc(int m, int n, int id) {
   return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
-         ((FMT == FUS_FP4_MX ? 1u : 0u) << 23) | ((uint32_t)(128 >> 4) << 24) |
+         ((FMT == FUS_FP4_MX ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24) |
          ((uint32_t)id << 4) | ((uint32_t)id << 29);
 }
 
@@ -115,14 +115,57 @@ FUS_DEVICE void tc_mma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, u
         : "memory");
 }
 
-// one 512-byte scale atom, shared -> tensor memory (4 columns, repeated over the 4 lane
-// quarters)
+// one 512-byte scale atom in shared memory: no swizzle, 8-row core matrices of 128 bytes
+// following one another
+FUS_DEVICE uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)8 << 16) | ((uint64_t)8 << 32) |
+         ((uint64_t)1 << 46);
+}
+// ... into tensor memory (4 columns, repeated over the 4 lane quarters)
 FUS_DEVICE void tc_cp_scales(uint32_t taddr, uint32_t saddr) {
-  // no swizzle, 8-row core matrices of 128 bytes following one another
-  const uint64_t desc = (uint64_t)((saddr >> 4) & 0x3fff) | ((uint64_t)8 << 16) |
-                        ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr),
+               "l"(scale_desc(saddr))
                : "memory");
+}
+
+// The group's staged chunk, token-major [CHUNK][128] fp32, to its output rows: nj live tokens,
+// rows[] their output rows (-1: none), weight tile mt; 16 bytes for a thread and row.
+template <bool SWIGLU, int CHUNK>
+FUS_DEVICE void store_chunk(const Fp4Args& a, const float* S, const int* rows, int nj, int mt,
+                            int et) {
+  constexpr int PER = SWIGLU ? 8 : 16;  // threads of a token row, 8 features each
+  const int f = (et % PER) * 8;
+  const int col = mt * (SWIGLU ? 64 : 128) + f;
+#pragma unroll
+  for (int j0 = 0; j0 < CHUNK; j0 += kGroupThreads / PER) {
+    const int j = j0 + et / PER;
+    if (j >= nj || col >= a.out_cols) continue;
+    const int row = rows[j];
+    if (row < 0) continue;
+    float o[8];
+    *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(S + j * 128 + f);
+    *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<const float4*>(S + j * 128 + f + 4);
+    if (SWIGLU) {
+      float w[8];
+      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(S + j * 128 + 64 + f);
+      *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(S + j * 128 + 68 + f);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) o[t] = silu_mul(o[t], w[t]);
+    }
+    if (a.row_scale) {
+      const float rs = __ldg(a.row_scale + row);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) o[t] *= rs;
+    }
+    if (a.out_f32) {
+      float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + (long)row * a.ldo + col);
+      d[0] = make_float4(o[0], o[1], o[2], o[3]);
+      d[1] = make_float4(o[4], o[5], o[6], o[7]);
+    } else {
+      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (long)row * a.ldo + col) =
+          pack8(o);
+    }
+  }
 }
 
 template <int BN, int FMT, bool SWIGLU>
@@ -281,7 +324,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
               const int cell = FMT == FUS_FP4_MX ? j / 2 : j;
               const int id = FMT == FUS_FP4_MX ? (j % 2) * 2 : 0;
               tc_mma_fp4<FMT>(acc, sw128_desc(sA + s * C::A_BYTES + 32 * j),
-                              sw128_desc(sB + s * C::B_BYTES + 32 * j), fp4_idesc<FMT>(nm, id),
+                              sw128_desc(sB + s * C::B_BYTES + 32 * j), fp4_idesc<FMT>(128, nm, id),
                               sf + 4 * cell, sf + C::SFB_OFF + 4 * C::ATOMS * cell, (k | j) != 0);
             }
           }
@@ -358,42 +401,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
 #pragma unroll
         for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[j]) * alpha;
         named_bar_sync(1 + grp, kGroupThreads);
-        constexpr int PER = SWIGLU ? 8 : 16;  // threads of a token row, 8 features each
-        const int nj = min(C::CHUNK, live - c0);
-        const int f = (et % PER) * 8;
-        const int col = mt * (SWIGLU ? 64 : 128) + f;
-#pragma unroll
-        for (int j0 = 0; j0 < C::CHUNK; j0 += kGroupThreads / PER) {
-          const int j = j0 + et / PER;
-          if (j >= nj || col >= a.out_cols) continue;
-          const int row = s_row[c0 + j];
-          if (row < 0) continue;
-          float o[8];
-          *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(S + j * 128 + f);
-          *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<const float4*>(S + j * 128 + f + 4);
-          if (SWIGLU) {
-            float w[8];
-            *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(S + j * 128 + 64 + f);
-            *reinterpret_cast<float4*>(w + 4) =
-                *reinterpret_cast<const float4*>(S + j * 128 + 68 + f);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) o[t] = silu_mul(o[t], w[t]);
-          }
-          if (a.row_scale) {
-            const float rs = __ldg(a.row_scale + row);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) o[t] *= rs;
-          }
-          if (a.out_f32) {
-            float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) +
-                                                  (long)row * a.ldo + col);
-            d[0] = make_float4(o[0], o[1], o[2], o[3]);
-            d[1] = make_float4(o[4], o[5], o[6], o[7]);
-          } else {
-            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) +
-                                      (long)row * a.ldo + col) = pack8(o);
-          }
-        }
+        store_chunk<SWIGLU, C::CHUNK>(a, S, s_row + c0, min(C::CHUNK, live - c0), mt, et);
         named_bar_sync(1 + grp, kGroupThreads);
       }
       tc_fence_before();
@@ -402,10 +410,10 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       ++n;
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
-    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, C::TMEM_COLS);
   }
@@ -434,15 +442,21 @@ int launch(const CUtensorMap& tw, const CUtensorMap& tx, const Fp4Args& a, long 
   return check_launch("fp4_grouped_gemm");
 }
 
+}  // namespace
+
+#include "fp4_gemm_pair.cuh"
+
+namespace {
+
 template <int FMT, bool SWIGLU>
-int launch_bn(int bn, const CUtensorMap& tw, const CUtensorMap& tx, const Fp4Args& a, long units,
-              cudaStream_t st) {
+int launch_bn(int bn, const CUtensorMap& tw, const CUtensorMap& tx, const fus_fp4_gemm_desc* d,
+              const Fp4Args& a, long units, cudaStream_t st) {
   switch (bn) {
     case 16: return launch<16, FMT, SWIGLU>(tw, tx, a, units, st);
     case 32: return launch<32, FMT, SWIGLU>(tw, tx, a, units, st);
     case 64: return launch<64, FMT, SWIGLU>(tw, tx, a, units, st);
     case 128: return launch<128, FMT, SWIGLU>(tw, tx, a, units, st);
-    default: return launch<256, FMT, SWIGLU>(tw, tx, a, units, st);
+    default: return launch_pair<FMT, SWIGLU>(tw, d, a, (int)(units / a.m_tiles), st);
   }
 }
 
@@ -525,10 +539,10 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   if (rc) return rc;
   cudaStream_t st = as_stream(stream);
   if (d->fmt == FUS_FP4_MX)
-    return sw ? launch_bn<FUS_FP4_MX, true>(d->block_n, tw, tx, a, units, st)
-              : launch_bn<FUS_FP4_MX, false>(d->block_n, tw, tx, a, units, st);
-  return sw ? launch_bn<FUS_FP4_NV, true>(d->block_n, tw, tx, a, units, st)
-            : launch_bn<FUS_FP4_NV, false>(d->block_n, tw, tx, a, units, st);
+    return sw ? launch_bn<FUS_FP4_MX, true>(d->block_n, tw, tx, d, a, units, st)
+              : launch_bn<FUS_FP4_MX, false>(d->block_n, tw, tx, d, a, units, st);
+  return sw ? launch_bn<FUS_FP4_NV, true>(d->block_n, tw, tx, d, a, units, st)
+            : launch_bn<FUS_FP4_NV, false>(d->block_n, tw, tx, d, a, units, st);
 }
 
 }  // namespace

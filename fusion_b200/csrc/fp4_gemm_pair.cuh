@@ -1,0 +1,378 @@
+// SM-pair form of the four-bit product for 256-token blocks (tcgen05 cta_group::2). Included by
+// fp4_gemm.cu.
+//
+// At 256 tokens for an expert the product is bound by what a stage brings into shared memory
+// and the MMAs read back from it, not by the tensor pipe: a 128 x 256 tile of one CTA moves
+// 54 KB for 512 cycles of MMA. A cluster of two CTAs computes 256 weight rows x 256 tokens with
+// M = 256 MMAs of the leader (rank 0): CTA r stages weight tile 2 mt + r with its scales, half
+// of the token rows, and the scales of all of them (each SM's tensor core scales its own rows
+// against all tokens). 38 KB for 512 cycles.
+//
+// Both CTAs' copies complete on the leader's full barrier (tensor copies of .cta_group::2, the
+// scales too; no multicast). The leader's warp 2 copies both CTAs' scales into their tensor
+// memory (tcgen05.cp.cta_group::2), its warp 1 issues the MMAs; commits free the stage and
+// hand over the accumulators on both CTAs. The accumulators fill 256 columns and are not
+// double-buffered: the epilogue reads them into registers at once (128 columns for a
+// thread) and frees them before it converts and stores.
+#pragma once
+
+namespace {
+
+template <int FMT>
+struct PairCfg {
+  static constexpr int BN = 256;
+  static constexpr int CELLS = fp4_cells(FMT);
+  static constexpr int A_BYTES = 128 * 128;
+  static constexpr int B_BYTES = 128 * 128;  // half of the tokens
+  static constexpr int SFA_BYTES = CELLS * 512;
+  static constexpr int SFB_BYTES = CELLS * 1024;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
+  static constexpr int BOX = 32;  // token rows of a TMA box
+  static constexpr int GROUPS = 2;
+  static constexpr int COLS_THREAD = BN / GROUPS;  // accumulator columns of a thread
+  static constexpr int CHUNK = 32;
+  static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
+  static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);
+  static constexpr int STAGES = (226 * 1024 - EPI_BYTES - 1280) / STAGE_BYTES;
+  static constexpr int SFB_OFF = CELLS * 4;
+  static constexpr int SF_COLS = SFB_OFF + CELLS * 8;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
+  static_assert(BN + 2 * SF_COLS <= TMEM_COLS && STAGES >= 4, "resources");
+};
+
+template <int FMT>
+FUS_DEVICE void tc_mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                uint32_t sfb, uint32_t accumulate) {
+  if (FMT == FUS_FP4_MX)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, "
+        "[%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// one scale atom of each CTA of the pair into its own tensor memory
+FUS_DEVICE void tc_cp_scales_pair(uint32_t taddr, uint32_t saddr) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr),
+               "l"(scale_desc(saddr))
+               : "memory");
+}
+// arrive on this CTA's `bar` once the thread's earlier copies and MMAs of the pair are done
+FUS_DEVICE void tc_commit_pair_local(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+
+template <int FMT, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREADS, 1)
+    fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tw,
+                         const __grid_constant__ CUtensorMap tx,
+                         const __grid_constant__ CUtensorMap twsf,
+                         const __grid_constant__ CUtensorMap txsf,
+                         const __grid_constant__ Fp4Args a) {
+  using C = PairCfg<FMT>;
+  constexpr int STAGES = C::STAGES, BN = C::BN;
+  extern __shared__ uint8_t smem_raw[];
+  // the same offsets in both CTAs: the dynamic window starts at the same address in each
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  const uint32_t sA = smem_u32(smem);
+  const uint32_t sB = sA + STAGES * C::A_BYTES;
+  const uint32_t sSA = sB + STAGES * C::B_BYTES;
+  const uint32_t sSB = sSA + STAGES * C::SFA_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + C::EPI_BYTES);
+  const uint32_t bar_full = smem_u32(bars);          // leader's used
+  const uint32_t bar_empty = bar_full + 8 * STAGES;  // both
+  const uint32_t bar_acc = bar_empty + 8 * STAGES;   // both
+  const uint32_t bar_free = bar_acc + 8;             // leader's used
+  const uint32_t bar_sf = bar_free + 8;              // [2] leader's
+  const uint32_t bar_sf_free = bar_sf + 16;          // [2] leader's
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const bool leader = rank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+    }
+    mbar_init(bar_acc, 1);
+    mbar_init(bar_free, 2 * 4 * C::GROUPS);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar_sf + 8 * b, 1);
+      mbar_init(bar_sf_free + 8 * b, 1);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tw);
+    tma_prefetch_desc(&tx);
+    tma_prefetch_desc(&twsf);
+    tma_prefetch_desc(&txsf);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  // barriers initialised and TMEM allocated in both CTAs before either touches the other
+  tc_fence_before();
+  cluster_barrier();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int rows_used = a.ntp ? min(__ldg(a.ntp), a.x_rows) : a.x_rows;
+  const int m_pairs = (a.m_tiles + 1) / 2;
+  const int units = (rows_used + BN - 1) / BN * m_pairs;
+  const int first = (int)cluster_id_x(), stride = (int)cluster_count_x();
+  auto expert_of = [&](int blk) {
+    const int e = a.expert_ids ? __ldg(a.expert_ids + blk) : 0;
+    if (e >= 0 && e < a.n_experts) return e;
+    raise_status(a.status, FUS_ERR_BAD_EXPERT);
+    return -1;
+  };
+  auto live_of = [&](int blk) {
+    int live = 0;
+    for (int j = lane; j < BN; j += 32) {
+      const int pos = blk * BN + j;
+      live += pos < rows_used && (!a.live_ids || __ldg(a.live_ids + pos) < a.live_limit);
+    }
+    return __reduce_add_sync(0xffffffffu, live);
+  };
+  auto width_of = [](int live) { return max(16, (live + 15) & ~15); };
+
+  if (warp == 0) {
+    // ---- producer (both CTAs) ----
+    const uint64_t pol_w = a.stream_w ? policy_evict_first() : policy_evict_normal();
+    const uint64_t pol_x = policy_evict_last();
+    int it = 0;
+    bool waited = a.pdl == 0;
+    int ok = 1;
+    for (int u = first; u < units && ok; u += stride) {
+      const int blk = u / m_pairs, mt = (u - blk * m_pairs) * 2 + rank;
+      const int e = expert_of(blk);
+      if (e < 0) continue;
+      const int half = width_of(live_of(blk)) / 2;  // this CTA's token rows
+      const int boxes = (half + C::BOX - 1) / C::BOX;
+      if (lane == 0) {
+        const uint32_t bytes =
+            2 * (C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + boxes * C::BOX * 128);
+        // scale atoms as rows of 128 bytes; a tile past the expert's last gives no output, and
+        // past the last expert's reads zeros
+        const int wsf_row = (e * a.m_tiles + mt) * a.nst * (C::SFA_BYTES / 128);
+        const int xsf_row = blk * a.nst * (C::SFB_BYTES / 128);
+        auto load_w = [&](int s, int k) {
+          const uint32_t full = cluster_map(bar_full + 8 * s, 0);
+          if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
+          if (SWIGLU) {
+            const int r = e * a.w_rows + mt * 64;
+            tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, r, pol_w);
+            tma_load_2d_pair(sA + s * C::A_BYTES + 64 * 128, &tw, full, k * 128,
+                             r + a.w_rows / 2, pol_w);
+          } else {
+            tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128,
+                             pol_w);
+          }
+          tma_load_2d_pair(sSA + s * C::SFA_BYTES, &twsf, full, 0,
+                           wsf_row + k * (C::SFA_BYTES / 128), pol_w);
+        };
+        auto load_x = [&](int s, int k) {
+          const uint32_t full = cluster_map(bar_full + 8 * s, 0);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d_pair(sB + s * C::B_BYTES + b * C::BOX * 128, &tx, full, k * 128,
+                             blk * BN + rank * half + b * C::BOX, pol_x);
+          tma_load_2d_pair(sSB + s * C::SFB_BYTES, &txsf, full, 0,
+                           xsf_row + k * (C::SFB_BYTES / 128), pol_x);
+        };
+        int k0 = 0;
+        if (!waited) {
+          // programmatic dependent of the quantiser: weights first, rows after it
+          k0 = min(a.nst, STAGES);
+          for (int k = 0; k < k0; ++k) load_w(k, k);
+          pdl_wait();
+          for (int k = 0; k < k0; ++k) load_x(k, k);
+          it = k0;
+          waited = true;
+        }
+        for (int k = k0; k < a.nst; ++k, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
+            ok = 0;
+            break;
+          }
+          load_w(s, k);
+          load_x(s, k);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (lane == 0 && !waited) pdl_wait();
+  } else if (warp == 1 && leader) {
+    // ---- MMAs ----
+    int it = 0, n = 0;
+    int ok = 1;
+    for (int u = first; u < units && ok; u += stride) {
+      const int blk = u / m_pairs;
+      if (expert_of(blk) < 0) continue;
+      const int nm = width_of(live_of(blk));
+      if (lane == 0) {
+        ok = mbar_wait_bounded(bar_free, (n & 1) ^ 1, abort_flag, a.status);
+        tc_fence_after();
+        for (int k = 0; k < a.nst && ok; ++k, ++it) {
+          const int s = it % STAGES, b = it & 1;
+          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
+               mbar_wait_bounded(bar_sf + 8 * b, (it >> 1) & 1, abort_flag, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sf = tmem + BN + b * C::SF_COLS;
+          const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j < steps) {
+              const int cell = FMT == FUS_FP4_MX ? j / 2 : j;
+              const int id = FMT == FUS_FP4_MX ? (j % 2) * 2 : 0;
+              tc_mma_fp4_pair<FMT>(tmem, sw128_desc(sA + s * C::A_BYTES + 32 * j),
+                                   sw128_desc(sB + s * C::B_BYTES + 32 * j),
+                                   fp4_idesc<FMT>(256, nm, id), sf + 4 * cell,
+                                   sf + C::SFB_OFF + 8 * cell, (k | j) != 0);
+            }
+          }
+          tc_commit_pair(bar_empty + 8 * s);
+          tc_commit_pair_local(bar_sf_free + 8 * b);
+        }
+        if (ok) tc_commit_pair(bar_acc);
+      }
+      ++n;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+  } else if (warp == 2 && leader) {
+    // ---- scales into both CTAs' tensor memory ----
+    int it = 0;
+    int ok = 1;
+    for (int u = first; u < units && ok; u += stride) {
+      const int blk = u / m_pairs;
+      if (expert_of(blk) < 0) continue;
+      const int atoms = live_of(blk) <= 128 ? 1 : 2;
+      if (lane == 0) {
+        for (int k = 0; k < a.nst; ++k, ++it) {
+          const int s = it % STAGES, b = it & 1;
+          ok = mbar_wait_bounded(bar_sf_free + 8 * b, ((it >> 1) & 1) ^ 1, abort_flag, a.status) &&
+               mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sf = tmem + BN + b * C::SF_COLS;
+#pragma unroll
+          for (int c = 0; c < C::CELLS; ++c) {
+            tc_cp_scales_pair(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (t < atoms)
+                tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * 2 + t),
+                                  sSB + s * C::SFB_BYTES + 512 * (c * 2 + t));
+          }
+          tc_commit_pair_local(bar_sf + 8 * b);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue (both CTAs): group g has columns [128 g, 128 g + 128) ----
+    const int q4 = warp & 3;
+    const int grp = (warp - 4) >> 2;
+    const int m = q4 * 32 + lane;
+    const int et = threadIdx.x - 128 - grp * kGroupThreads;
+    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
+    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
+                                        C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
+    const float gx = a.xg ? __ldg(a.xg) : 1.0f;
+    const uint32_t free_leader = cluster_map(bar_free, 0);
+    int n = 0;
+    for (int u = first; u < units; u += stride) {
+      const int blk = u / m_pairs, mt = (u - blk * m_pairs) * 2 + rank;
+      const int e = expert_of(blk);
+      if (e < 0) continue;
+      const int live = live_of(blk) - grp * C::COLS_THREAD;  // of this group's columns
+      for (int j = et; j < min(live, C::COLS_THREAD); j += kGroupThreads) {
+        const int pos = blk * BN + grp * C::COLS_THREAD + j;
+        const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
+        s_row[j] = row < a.out_rows ? row : -1;
+      }
+      const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
+      if (!mbar_wait_bounded(bar_acc, n & 1, abort_flag, a.status)) break;
+      tc_fence_after();
+      uint32_t v[C::COLS_THREAD];
+      const uint32_t acc = tmem + grp * C::COLS_THREAD + ((uint32_t)(q4 * 32) << 16);
+#pragma unroll
+      for (int c = 0; c < C::COLS_THREAD; c += 16)
+        if (c < live) tmem_ld16_issue(acc + c, v + c);
+#pragma unroll
+      for (int c = 0; c < C::COLS_THREAD; c += 16)
+        if (c < live) tmem_ld_wait(v + c);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(free_leader);
+      ++n;
+#pragma unroll
+      for (int c0 = 0; c0 < C::COLS_THREAD; c0 += C::CHUNK) {
+        if (c0 >= live) break;
+#pragma unroll
+        for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[c0 + j]) * alpha;
+        named_bar_sync(1 + grp, kGroupThreads);
+        store_chunk<SWIGLU, C::CHUNK>(a, S, s_row + c0, min(C::CHUNK, live - c0), mt, et);
+        named_bar_sync(1 + grp, kGroupThreads);
+      }
+    }
+  }
+  // neither CTA leaves (or frees the pair's TMEM) while the other may still signal its
+  // barriers or read its shared memory
+  __syncwarp();
+  tc_fence_before();
+  cluster_barrier();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, C::TMEM_COLS);
+}
+
+template <int FMT, bool SWIGLU>
+int launch_pair(const CUtensorMap& tw, const fus_fp4_gemm_desc* d, const Fp4Args& a, int blocks,
+                cudaStream_t st) {
+  using C = PairCfg<FMT>;
+  auto fn = fp4_gemm_pair_kernel<FMT, SWIGLU>;
+  if (int rc = ensure_smem_attr((const void*)fn, C::SMEM_BYTES, "fp4_grouped_gemm")) return rc;
+  CUtensorMap tx, twsf, txsf;
+  const uint64_t wsf_rows = (uint64_t)a.n_experts * a.m_tiles * a.nst * (C::SFA_BYTES / 128);
+  const uint64_t xsf_rows = (uint64_t)blocks * a.nst * (C::SFB_BYTES / 128);
+  if (wsf_rows > 0x7fffffffu || xsf_rows > 0x7fffffffu)
+    return set_error(FUS_E_UNSUPPORTED, "fp4_gemm: too many scales");
+  int rc = make_tmap_u8_2d(&tx, d->xq, (uint64_t)d->K / 2, (uint64_t)d->x_rows,
+                           (uint64_t)d->ldxq, 128, C::BOX);
+  if (!rc) rc = make_tmap_u8_2d(&twsf, d->wsf, 128, wsf_rows, 128, 128, C::SFA_BYTES / 128, false);
+  if (!rc) rc = make_tmap_u8_2d(&txsf, d->xsf, 128, xsf_rows, 128, 128, C::SFB_BYTES / 128, false);
+  if (rc) return rc;
+  const long units = (long)blocks * ((a.m_tiles + 1) / 2);
+  const long pairs = num_sms() / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (units < pairs ? units : pairs)));
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tw, tx, twsf, txsf, a);
+  if (e != cudaSuccess)
+    return set_error(FUS_E_LAUNCH, "fp4_grouped_gemm: %s", cudaGetErrorString(e));
+  return check_launch("fp4_grouped_gemm");
+}
+
+}  // namespace

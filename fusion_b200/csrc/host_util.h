@@ -19,9 +19,10 @@ int check_launch(const char* what);
 // row, `rows` rows, row pitch `ld` elements, box = box_inner x box_rows.
 int make_tmap_bf16_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
                       uint32_t box_inner, uint32_t box_rows);
-// Same for rows of bytes (packed 4-bit operands): `inner` bytes, row pitch `ld` bytes
+// Same for rows of bytes (packed 4-bit operands and, without swizzle, their scales): `inner`
+// bytes, row pitch `ld` bytes
 int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
-                    uint32_t box_inner, uint32_t box_rows);
+                    uint32_t box_inner, uint32_t box_rows, bool swizzle = true);
 // row-major output tile map for TMA stores (no swizzle: the staging tile is row-major)
 int make_tmap_store_2d(CUtensorMap* m, const void* base, bool f32, uint64_t inner, uint64_t rows,
                        uint64_t ld, uint32_t box_inner, uint32_t box_rows);
