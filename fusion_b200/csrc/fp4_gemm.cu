@@ -16,7 +16,7 @@
 //             the 64-row boxes that hold live rows), one bulk copy each of their scale atoms
 //   warp 1  : TMEM owner; one lane issues a stage's four K = 64 MMAs
 //   warp 2  : one lane copies a stage's scales into tensor memory (tcgen05.cp) ahead of the
-//             MMAs, into one of two buffers. Issued by the MMA thread they would run in order
+//             MMAs, into columns of that stage. Issued by the MMA thread they would run in order
 //             with the MMAs, about 55 cycles each: 12 of them for 512 cycles of MMA (dense
 //             8192 x 4096 x 6144 NV: 290 -> 230 us with 128-token blocks)
 //   warps 4-11 (4-7 up to 64 token columns): epilogue, two groups that take chunks of 32 columns
@@ -78,9 +78,9 @@ struct Cfg {
   static constexpr int STAGES = RING_TARGET / STAGE_BYTES > 8 ? 8 : RING_TARGET / STAGE_BYTES;
   static constexpr int ACCS = BN <= 128 ? 2 : 1;
   static constexpr int SFB_OFF = CELLS * 4;                      // token scales, after the weights'
-  static constexpr int SF_COLS = SFB_OFF + CELLS * ATOMS * 4;    // one of two scale buffers
+  static constexpr int SF_COLS = SFB_OFF + CELLS * ATOMS * 4;    // a stage's scales
   static constexpr int SF_COL = ACCS * BN;
-  static constexpr int COLS = SF_COL + 2 * SF_COLS;
+  static constexpr int COLS = SF_COL + STAGES * SF_COLS;
   static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
   static_assert(STAGES >= 3 && CTAS * TMEM_COLS <= 512 && COLS <= 512, "resources");
@@ -186,9 +186,8 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
   const uint32_t bar_empty = bar_full + 8 * STAGES;
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // accumulator finished
   const uint32_t bar_free = bar_acc + 8 * C::ACCS;   // accumulator drained
-  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // scales are in tensor memory
-  const uint32_t bar_sf_free = bar_sf + 16;          // their MMAs are done
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * C::ACCS + 4);
+  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // a stage's scales are in tensor memory
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -196,14 +195,11 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
+      mbar_init(bar_sf + 8 * s, 1);
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(bar_acc + 8 * b, 1);
       mbar_init(bar_free + 8 * b, 4 * C::GROUPS);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar_sf + 8 * b, 1);
-      mbar_init(bar_sf_free + 8 * b, 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -311,12 +307,12 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
         tc_fence_after();
         const uint32_t acc = tmem + buf * BN;
         for (int k = 0; k < a.nst && ok; ++k, ++it) {
-          const int s = it % STAGES, b = it & 1;
+          const int s = it % STAGES;
           ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_sf + 8 * b, (it >> 1) & 1, abort_flag, a.status);
+               mbar_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sf = tmem + C::SF_COL + b * C::SF_COLS;
+          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -329,7 +325,6 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
             }
           }
           tc_commit(bar_empty + 8 * s);
-          tc_commit(bar_sf_free + 8 * b);
         }
         if (ok) tc_commit(bar_acc + 8 * buf);
       }
@@ -346,12 +341,12 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
       if (lane == 0) {
         for (int k = 0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES, b = it & 1;
-          ok = mbar_wait_bounded(bar_sf_free + 8 * b, ((it >> 1) & 1) ^ 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+          const int s = it % STAGES;
+          // a full stage: the MMAs that read its scale columns before are done
+          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sf = tmem + C::SF_COL + b * C::SF_COLS;
+          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
             tc_cp_scales(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
@@ -361,7 +356,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
                 tc_cp_scales(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
                              sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
           }
-          tc_commit(bar_sf + 8 * b);
+          tc_commit(bar_sf + 8 * s);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -521,7 +516,10 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   a.scatter = d->scatter;
   a.out_f32 = d->out_dtype == FUS_DT_F32;
   const int blocks = ceil_div(d->x_rows, d->block_n);
-  a.stream_w = blocks <= 2L * d->n_experts;
+  // weights that one block of each expert reads leave L2 first; with more blocks the second
+  // one finds them there
+  a.stream_w = (d->live_ids ? (long)d->live_limit : (long)d->x_rows) <=
+               (long)d->n_experts * d->block_n / 2;
   a.row_scale = d->row_scale;
   a.out = d->out;
   a.ldo = d->ldo;

@@ -38,7 +38,7 @@ struct PairCfg {
   static constexpr int SF_COLS = SFB_OFF + CELLS * 8;
   static constexpr int TMEM_COLS = 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
-  static_assert(BN + 2 * SF_COLS <= TMEM_COLS && STAGES >= 4, "resources");
+  static_assert(BN + STAGES * SF_COLS <= TMEM_COLS && STAGES >= 4, "resources");
 };
 
 template <int FMT>
@@ -94,9 +94,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
   const uint32_t bar_empty = bar_full + 8 * STAGES;  // both
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // both
   const uint32_t bar_free = bar_acc + 8;             // leader's used
-  const uint32_t bar_sf = bar_free + 8;              // [2] leader's
-  const uint32_t bar_sf_free = bar_sf + 16;          // [2] leader's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  const uint32_t bar_sf = bar_free + 8;              // leader's used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -106,13 +105,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
+      mbar_init(bar_sf + 8 * s, 1);
     }
     mbar_init(bar_acc, 1);
     mbar_init(bar_free, 2 * 4 * C::GROUPS);
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar_sf + 8 * b, 1);
-      mbar_init(bar_sf_free + 8 * b, 1);
-    }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tw);
@@ -228,12 +224,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         ok = mbar_wait_bounded(bar_free, (n & 1) ^ 1, abort_flag, a.status);
         tc_fence_after();
         for (int k = 0; k < a.nst && ok; ++k, ++it) {
-          const int s = it % STAGES, b = it & 1;
+          const int s = it % STAGES;
           ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_sf + 8 * b, (it >> 1) & 1, abort_flag, a.status);
+               mbar_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sf = tmem + BN + b * C::SF_COLS;
+          const uint32_t sf = tmem + BN + s * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -247,7 +243,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
             }
           }
           tc_commit_pair(bar_empty + 8 * s);
-          tc_commit_pair_local(bar_sf_free + 8 * b);
         }
         if (ok) tc_commit_pair(bar_acc);
       }
@@ -264,12 +259,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       const int atoms = live_of(blk) <= 128 ? 1 : 2;
       if (lane == 0) {
         for (int k = 0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES, b = it & 1;
-          ok = mbar_wait_bounded(bar_sf_free + 8 * b, ((it >> 1) & 1) ^ 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+          const int s = it % STAGES;
+          // a full stage: the MMAs that read its scale columns before are done
+          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sf = tmem + BN + b * C::SF_COLS;
+          const uint32_t sf = tmem + BN + s * C::SF_COLS;
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
             tc_cp_scales_pair(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
@@ -279,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
                 tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * 2 + t),
                                   sSB + s * C::SFB_BYTES + 512 * (c * 2 + t));
           }
-          tc_commit_pair_local(bar_sf + 8 * b);
+          tc_commit_pair_local(bar_sf + 8 * s);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
