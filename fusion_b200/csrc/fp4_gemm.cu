@@ -12,8 +12,8 @@
 //
 // A CTA loops over (block, weight tile) units with one continuous ring of stages (256 K
 // elements = 128 bytes of a row):
-//   warp 0  : producer, one lane: TMA boxes of weights and token rows (128-byte swizzle; only
-//             the 64-row boxes that hold live rows), one bulk copy each of their scale atoms
+//   warp 0  : producer, one lane: a TMA box of weights and one of token rows (128-byte swizzle),
+//             one bulk copy each of their scale atoms
 //   warp 1  : TMEM owner; one lane issues a stage's four K = 64 MMAs
 //   warp 2  : one lane copies a stage's scales into tensor memory (tcgen05.cp) ahead of the
 //             MMAs, into columns of that stage. Issued by the MMA thread they would run in order
@@ -56,6 +56,14 @@ struct Fp4Args {
   int* status;
 };
 
+// The rows of a token block in one box: the smallest of these maps that holds the live ones
+// (32, 64, 96 or 128 rows; blocks up to 64 rows use the first, with a box of the block). A
+// copy costs about 75 cycles beside its bytes, so one is issued, not four of 32 rows (copies
+// alone, 8192 x 4096 x 6144 by pairs: 92 -> 72 us).
+struct TokenMaps {
+  CUtensorMap m[4];
+};
+
 constexpr int kGroupThreads = 128;  // an epilogue group: the four lane quarters of TMEM
 
 template <int BN, int FMT>
@@ -71,7 +79,6 @@ struct Cfg {
   static constexpr int GROUPS = BN > 64 ? 2 : 1;
   static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
   static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);  // staging, row numbers
-  static constexpr int BOX = BN < 64 ? BN : 64;  // token rows of a TMA box
   // two CTAs for an SM up to 64 token columns (TMEM 256 columns each), else one
   static constexpr int CTAS = BN <= 64 ? 2 : 1;
   static constexpr int RING_TARGET = (CTAS == 2 ? 112 : 226) * 1024 - EPI_BYTES - 1280;
@@ -170,7 +177,7 @@ FUS_DEVICE void store_chunk(const Fp4Args& a, const float* S, const int* rows, i
 
 template <int BN, int FMT, bool SWIGLU>
 __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ TokenMaps tx,
                     const __grid_constant__ Fp4Args a) {
   using C = Cfg<BN, FMT>;
   constexpr int STAGES = C::STAGES;
@@ -204,7 +211,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tw);
-    tma_prefetch_desc(&tx);
+    tma_prefetch_desc(&tx.m[0]);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -244,20 +251,17 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
       const int e = expert_of(blk);
       if (e < 0) continue;
-      const int boxes = BN > 64 ? max(1, (live_of(blk) + 63) / 64) : 1;
+      const int box = BN > 64 ? max(0, (live_of(blk) - 1) / 32) : 0;
       if (lane == 0) {
         const uint8_t* wsf = a.wsf + ((long)e * a.m_tiles + mt) * a.nst * C::SFA_BYTES;
         const uint8_t* xsf = a.xsf + (long)blk * a.nst * C::SFB_BYTES;
-        const uint32_t bytes =
-            C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + boxes * C::BOX * 128;
+        const uint32_t bytes = C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES +
+                               (BN > 64 ? 32 * (box + 1) : BN) * 128;
         auto load_w = [&](int s, int k) {
           const uint32_t full = bar_full + 8 * s;
           mbar_arrive_expect_tx(full, bytes);
-          if (SWIGLU) {
-            const int r = e * a.w_rows + mt * 64;
-            tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, r, pol_w);
-            tma_load_2d(sA + s * C::A_BYTES + 64 * 128, &tw, full, k * 128, r + a.w_rows / 2,
-                        pol_w);
+          if (SWIGLU) {  // 64 gate rows, their 64 up rows
+            tma_load_3d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0, pol_w);
           } else {
             tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
           }
@@ -265,9 +269,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
         };
         auto load_x = [&](int s, int k) {
           const uint32_t full = bar_full + 8 * s;
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(sB + s * C::B_BYTES + b * C::BOX * 128, &tx, full, k * 128,
-                        blk * BN + b * C::BOX, pol_x);
+          tma_load_2d(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN, pol_x);
           bulk_load(sSB + s * C::SFB_BYTES, xsf + (long)k * C::SFB_BYTES, C::SFB_BYTES, full, pol_x);
         };
         int k0 = 0;
@@ -415,7 +417,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
 }
 
 template <int BN, int FMT, bool SWIGLU>
-int launch(const CUtensorMap& tw, const CUtensorMap& tx, const Fp4Args& a, long units,
+int launch(const CUtensorMap& tw, const TokenMaps& tx, const Fp4Args& a, long units,
            cudaStream_t st) {
   using C = Cfg<BN, FMT>;
   auto fn = fp4_gemm_kernel<BN, FMT, SWIGLU>;
@@ -444,14 +446,14 @@ int launch(const CUtensorMap& tw, const CUtensorMap& tx, const Fp4Args& a, long 
 namespace {
 
 template <int FMT, bool SWIGLU>
-int launch_bn(int bn, const CUtensorMap& tw, const CUtensorMap& tx, const fus_fp4_gemm_desc* d,
+int launch_bn(int bn, const CUtensorMap& tw, const TokenMaps& tx, const fus_fp4_gemm_desc* d,
               const Fp4Args& a, long units, cudaStream_t st) {
   switch (bn) {
     case 16: return launch<16, FMT, SWIGLU>(tw, tx, a, units, st);
     case 32: return launch<32, FMT, SWIGLU>(tw, tx, a, units, st);
     case 64: return launch<64, FMT, SWIGLU>(tw, tx, a, units, st);
     case 128: return launch<128, FMT, SWIGLU>(tw, tx, a, units, st);
-    default: return launch_pair<FMT, SWIGLU>(tw, d, a, (int)(units / a.m_tiles), st);
+    default: return launch_pair<FMT, SWIGLU>(tw, tx, d, a, (int)(units / a.m_tiles), st);
   }
 }
 
@@ -528,12 +530,16 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   a.status = status;
   const long units = (long)blocks * a.m_tiles;
   if (units > 0x7fffffffL) return set_error(FUS_E_UNSUPPORTED, "fp4_gemm: too many tiles");
-  CUtensorMap tw, tx;
-  int rc = make_tmap_u8_2d(&tw, d->wq, (uint64_t)d->K / 2, (uint64_t)d->n_experts * d->w_rows,
-                           (uint64_t)d->K / 2, 128, sw ? 64 : 128);
-  if (!rc)
-    rc = make_tmap_u8_2d(&tx, d->xq, (uint64_t)d->K / 2, (uint64_t)d->x_rows, (uint64_t)d->ldxq,
-                         128, d->block_n < 64 ? d->block_n : 64);
+  CUtensorMap tw;
+  TokenMaps tx;
+  const uint64_t row = (uint64_t)d->K / 2, rows = (uint64_t)d->n_experts * d->w_rows;
+  const uint64_t half = (uint64_t)d->w_rows / 2;
+  // SwiGLU: two planes, the gate rows and the up rows of the stack
+  int rc = sw ? make_tmap_u8_3d(&tw, d->wq, row, rows - half, row, 2, half * row, 128, 64, 2)
+              : make_tmap_u8_2d(&tw, d->wq, row, rows, row, 128, 128);
+  for (int i = 0; i < 4 && !rc; ++i)
+    rc = make_tmap_u8_2d(&tx.m[i], d->xq, row, (uint64_t)d->x_rows, (uint64_t)d->ldxq, 128,
+                         d->block_n <= 64 ? d->block_n : 32 * (i + 1));
   if (rc) return rc;
   cudaStream_t st = as_stream(stream);
   if (d->fmt == FUS_FP4_MX)

@@ -27,7 +27,6 @@ struct PairCfg {
   static constexpr int SFA_BYTES = CELLS * 512;
   static constexpr int SFB_BYTES = CELLS * 1024;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-  static constexpr int BOX = 32;  // token rows of a TMA box
   static constexpr int GROUPS = 2;
   static constexpr int COLS_THREAD = BN / GROUPS;  // accumulator columns of a thread
   static constexpr int CHUNK = 32;
@@ -75,7 +74,7 @@ FUS_DEVICE void tc_commit_pair_local(uint32_t bar) {
 template <int FMT, bool SWIGLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREADS, 1)
     fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tw,
-                         const __grid_constant__ CUtensorMap tx,
+                         const __grid_constant__ TokenMaps tx,
                          const __grid_constant__ CUtensorMap twsf,
                          const __grid_constant__ CUtensorMap txsf,
                          const __grid_constant__ Fp4Args a) {
@@ -112,7 +111,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tw);
-    tma_prefetch_desc(&tx);
+    tma_prefetch_desc(&tx.m[0]);
     tma_prefetch_desc(&twsf);
     tma_prefetch_desc(&txsf);
   }
@@ -158,10 +157,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int half = width_of(live_of(blk)) / 2;  // this CTA's token rows
-      const int boxes = (half + C::BOX - 1) / C::BOX;
+      const int box = (half - 1) / 32;
       if (lane == 0) {
         const uint32_t bytes =
-            2 * (C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + boxes * C::BOX * 128);
+            2 * (C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + 32 * (box + 1) * 128);
         // scale atoms as rows of 128 bytes; a tile past the expert's last gives no output, and
         // past the last expert's reads zeros
         const int wsf_row = (e * a.m_tiles + mt) * a.nst * (C::SFA_BYTES / 128);
@@ -170,10 +169,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
           const uint32_t full = cluster_map(bar_full + 8 * s, 0);
           if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
           if (SWIGLU) {
-            const int r = e * a.w_rows + mt * 64;
-            tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, r, pol_w);
-            tma_load_2d_pair(sA + s * C::A_BYTES + 64 * 128, &tw, full, k * 128,
-                             r + a.w_rows / 2, pol_w);
+            tma_load_3d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0,
+                             pol_w);
           } else {
             tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128,
                              pol_w);
@@ -183,9 +180,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         };
         auto load_x = [&](int s, int k) {
           const uint32_t full = cluster_map(bar_full + 8 * s, 0);
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d_pair(sB + s * C::B_BYTES + b * C::BOX * 128, &tx, full, k * 128,
-                             blk * BN + rank * half + b * C::BOX, pol_x);
+          tma_load_2d_pair(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN + rank * half,
+                           pol_x);
           tma_load_2d_pair(sSB + s * C::SFB_BYTES, &txsf, full, 0,
                            xsf_row + k * (C::SFB_BYTES / 128), pol_x);
         };
@@ -337,19 +333,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
 }
 
 template <int FMT, bool SWIGLU>
-int launch_pair(const CUtensorMap& tw, const fus_fp4_gemm_desc* d, const Fp4Args& a, int blocks,
-                cudaStream_t st) {
+int launch_pair(const CUtensorMap& tw, const TokenMaps& tx, const fus_fp4_gemm_desc* d,
+                const Fp4Args& a, int blocks, cudaStream_t st) {
   using C = PairCfg<FMT>;
   auto fn = fp4_gemm_pair_kernel<FMT, SWIGLU>;
   if (int rc = ensure_smem_attr((const void*)fn, C::SMEM_BYTES, "fp4_grouped_gemm")) return rc;
-  CUtensorMap tx, twsf, txsf;
+  CUtensorMap twsf, txsf;
   const uint64_t wsf_rows = (uint64_t)a.n_experts * a.m_tiles * a.nst * (C::SFA_BYTES / 128);
   const uint64_t xsf_rows = (uint64_t)blocks * a.nst * (C::SFB_BYTES / 128);
   if (wsf_rows > 0x7fffffffu || xsf_rows > 0x7fffffffu)
     return set_error(FUS_E_UNSUPPORTED, "fp4_gemm: too many scales");
-  int rc = make_tmap_u8_2d(&tx, d->xq, (uint64_t)d->K / 2, (uint64_t)d->x_rows,
-                           (uint64_t)d->ldxq, 128, C::BOX);
-  if (!rc) rc = make_tmap_u8_2d(&twsf, d->wsf, 128, wsf_rows, 128, 128, C::SFA_BYTES / 128, false);
+  int rc = make_tmap_u8_2d(&twsf, d->wsf, 128, wsf_rows, 128, 128, C::SFA_BYTES / 128, false);
   if (!rc) rc = make_tmap_u8_2d(&txsf, d->xsf, 128, xsf_rows, 128, 128, C::SFB_BYTES / 128, false);
   if (rc) return rc;
   const long units = (long)blocks * ((a.m_tiles + 1) / 2);

@@ -23,6 +23,10 @@ int make_tmap_bf16_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
 // bytes, row pitch `ld` bytes
 int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
                     uint32_t box_inner, uint32_t box_rows, bool swizzle = true);
+// ... of `planes` (> 1) such matrices, plane_ld bytes apart, in a box of box_planes
+int make_tmap_u8_3d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
+                    uint64_t planes, uint64_t plane_ld, uint32_t box_inner, uint32_t box_rows,
+                    uint32_t box_planes, bool swizzle = true);
 // row-major output tile map for TMA stores (no swizzle: the staging tile is row-major)
 int make_tmap_store_2d(CUtensorMap* m, const void* base, bool f32, uint64_t inner, uint64_t rows,
                        uint64_t ld, uint32_t box_inner, uint32_t box_rows);
