@@ -159,6 +159,23 @@ FUS_DEVICE bool mbar_wait_bounded(uint32_t bar, uint32_t parity, volatile int* a
   }
 }
 
+// One lane of a converged warp, the same one each time. Copies and tensor-core instructions take
+// their addresses from the warp's uniform registers: a loop that the whole warp runs in step,
+// with the issue behind elect_one(), keeps them there; behind `lane == 0` every issue moves
+// them over again.
+FUS_DEVICE bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// mbar_wait_bounded by a whole warp; one answer for all lanes
+FUS_DEVICE bool warp_wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort,
+                                  int* status) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, status));
+}
+
 // ------------------------------------------------------------------------------------
 // TMA (tiled tensor copies global -> shared, completion counted on an mbarrier)
 // ------------------------------------------------------------------------------------

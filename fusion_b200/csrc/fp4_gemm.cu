@@ -196,6 +196,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
   const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // a stage's scales are in tensor memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [GROUPS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -246,74 +247,75 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     const uint64_t pol_x = policy_evict_last();
     int it = 0;  // stages issued
     bool waited = a.pdl == 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int box = BN > 64 ? max(0, (live_of(blk) - 1) / 32) : 0;
-      if (lane == 0) {
-        const uint8_t* wsf = a.wsf + ((long)e * a.m_tiles + mt) * a.nst * C::SFA_BYTES;
-        const uint8_t* xsf = a.xsf + (long)blk * a.nst * C::SFB_BYTES;
-        const uint32_t bytes = C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES +
-                               (BN > 64 ? 32 * (box + 1) : BN) * 128;
-        auto load_w = [&](int s, int k) {
-          const uint32_t full = bar_full + 8 * s;
-          mbar_arrive_expect_tx(full, bytes);
-          if (SWIGLU) {  // 64 gate rows, their 64 up rows
-            tma_load_3d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0, pol_w);
-          } else {
-            tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
-          }
-          bulk_load(sSA + s * C::SFA_BYTES, wsf + (long)k * C::SFA_BYTES, C::SFA_BYTES, full, pol_w);
-        };
-        auto load_x = [&](int s, int k) {
-          const uint32_t full = bar_full + 8 * s;
-          tma_load_2d(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN, pol_x);
-          bulk_load(sSB + s * C::SFB_BYTES, xsf + (long)k * C::SFB_BYTES, C::SFB_BYTES, full, pol_x);
-        };
-        int k0 = 0;
-        if (!waited) {
-          // programmatic dependent of the quantiser: the first ring's weights are requested
-          // while it runs, its rows after it
-          k0 = min(a.nst, STAGES);
-          for (int k = 0; k < k0; ++k) load_w(k, k);
-          pdl_wait();
-          for (int k = 0; k < k0; ++k) load_x(k, k);
-          it = k0;
-          waited = true;
+      const uint8_t* wsf = a.wsf + ((long)e * a.m_tiles + mt) * a.nst * C::SFA_BYTES;
+      const uint8_t* xsf = a.xsf + (long)blk * a.nst * C::SFB_BYTES;
+      const uint32_t bytes = C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES +
+                             (BN > 64 ? 32 * (box + 1) : BN) * 128;
+      auto load_w = [&](int s, int k) {
+        const uint32_t full = bar_full + 8 * s;
+        mbar_arrive_expect_tx(full, bytes);
+        if (SWIGLU) {  // 64 gate rows, their 64 up rows
+          tma_load_3d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0, pol_w);
+        } else {
+          tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
         }
-        for (int k = k0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
-            ok = 0;
-            break;
-          }
+        bulk_load(sSA + s * C::SFA_BYTES, wsf + (long)k * C::SFA_BYTES, C::SFA_BYTES, full, pol_w);
+      };
+      auto load_x = [&](int s, int k) {
+        const uint32_t full = bar_full + 8 * s;
+        tma_load_2d(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN, pol_x);
+        bulk_load(sSB + s * C::SFB_BYTES, xsf + (long)k * C::SFB_BYTES, C::SFB_BYTES, full, pol_x);
+      };
+      int k0 = 0;
+      if (!waited) {
+        // programmatic dependent of the quantiser: the first ring's weights are requested
+        // while it runs, its rows after it
+        k0 = min(a.nst, STAGES);
+        if (elect_one())
+          for (int k = 0; k < k0; ++k) load_w(k, k);
+        pdl_wait();
+        if (elect_one())
+          for (int k = 0; k < k0; ++k) load_x(k, k);
+        __syncwarp();
+        it = k0;
+        waited = true;
+      }
+      for (int k = k0; k < a.nst; ++k, ++it) {
+        const int s = it % STAGES;
+        ok = warp_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status);
+        if (!ok) break;
+        if (elect_one()) {
           load_w(s, k);
           load_x(s, k);
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
-    if (lane == 0 && !waited) pdl_wait();
+    if (!waited) pdl_wait();
   } else if (warp == 1) {
     int it = 0, n = 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const int blk = u / a.m_tiles;
       if (expert_of(blk) < 0) continue;
       const int nm = max(16, (live_of(blk) + 15) & ~15);
-      if (lane == 0) {
-        const int buf = n % C::ACCS;
-        ok = mbar_wait_bounded(bar_free + 8 * buf, ((n / C::ACCS) & 1) ^ 1, abort_flag, a.status);
+      const int buf = n % C::ACCS;
+      ok = warp_wait_bounded(bar_free + 8 * buf, ((n / C::ACCS) & 1) ^ 1, abort_flag, a.status);
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * BN;
+      for (int k = 0; k < a.nst && ok; ++k, ++it) {
+        const int s = it % STAGES;
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
+             warp_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t acc = tmem + buf * BN;
-        for (int k = 0; k < a.nst && ok; ++k, ++it) {
-          const int s = it % STAGES;
-          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-          if (!ok) break;
-          tc_fence_after();
+        if (elect_one()) {
           const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
@@ -327,27 +329,27 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
             }
           }
           tc_commit(bar_empty + 8 * s);
+          if (k == a.nst - 1) tc_commit(bar_acc + 8 * buf);
         }
-        if (ok) tc_commit(bar_acc + 8 * buf);
+        __syncwarp();
       }
       ++n;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
   } else if (warp == 2) {
     int it = 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const int blk = u / a.m_tiles;
       if (expert_of(blk) < 0) continue;
       // atoms of token scales that hold live rows
       const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
-      if (lane == 0) {
-        for (int k = 0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES;
-          // a full stage: the MMAs that read its scale columns before are done
-          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-          if (!ok) break;
-          tc_fence_after();
+      for (int k = 0; k < a.nst; ++k, ++it) {
+        const int s = it % STAGES;
+        // a full stage: the MMAs that read its scale columns before are done
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
@@ -360,8 +362,8 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
           }
           tc_commit(bar_sf + 8 * s);
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
   } else if (warp >= 4) {
     const int q4 = warp & 3;  // the TMEM lanes this warp may read
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
     int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
                                         C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
+    volatile int* my_ok = group_ok + grp;
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
     int n = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -386,7 +389,11 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       }
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
       const int buf = n % C::ACCS;
-      if (!mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status)) break;
+      // one thread of the group waits, the others rest at the barrier: 256 spinning threads
+      // slow the issuing warps down
+      if (et == 0) *my_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
+      named_bar_sync(1 + grp, kGroupThreads);
+      if (!*my_ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q4 * 32) << 16);
       for (int c0 = grp * C::CHUNK; c0 < live; c0 += C::GROUPS * C::CHUNK) {

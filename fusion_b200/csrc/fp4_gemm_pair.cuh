@@ -96,6 +96,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
   const uint32_t bar_sf = bar_free + 8;              // leader's used
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [GROUPS]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
@@ -151,80 +152,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
     const uint64_t pol_x = policy_evict_last();
     int it = 0;
     bool waited = a.pdl == 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = first; u < units && ok; u += stride) {
       const int blk = u / m_pairs, mt = (u - blk * m_pairs) * 2 + rank;
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int half = width_of(live_of(blk)) / 2;  // this CTA's token rows
       const int box = (half - 1) / 32;
-      if (lane == 0) {
-        const uint32_t bytes =
-            2 * (C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + 32 * (box + 1) * 128);
-        // scale atoms as rows of 128 bytes; a tile past the expert's last gives no output, and
-        // past the last expert's reads zeros
-        const int wsf_row = (e * a.m_tiles + mt) * a.nst * (C::SFA_BYTES / 128);
-        const int xsf_row = blk * a.nst * (C::SFB_BYTES / 128);
-        auto load_w = [&](int s, int k) {
-          const uint32_t full = cluster_map(bar_full + 8 * s, 0);
-          if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
-          if (SWIGLU) {
-            tma_load_3d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0,
-                             pol_w);
-          } else {
-            tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128,
-                             pol_w);
-          }
-          tma_load_2d_pair(sSA + s * C::SFA_BYTES, &twsf, full, 0,
-                           wsf_row + k * (C::SFA_BYTES / 128), pol_w);
-        };
-        auto load_x = [&](int s, int k) {
-          const uint32_t full = cluster_map(bar_full + 8 * s, 0);
-          tma_load_2d_pair(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN + rank * half,
-                           pol_x);
-          tma_load_2d_pair(sSB + s * C::SFB_BYTES, &txsf, full, 0,
-                           xsf_row + k * (C::SFB_BYTES / 128), pol_x);
-        };
-        int k0 = 0;
-        if (!waited) {
-          // programmatic dependent of the quantiser: weights first, rows after it
-          k0 = min(a.nst, STAGES);
-          for (int k = 0; k < k0; ++k) load_w(k, k);
-          pdl_wait();
-          for (int k = 0; k < k0; ++k) load_x(k, k);
-          it = k0;
-          waited = true;
+      const uint32_t bytes =
+          2 * (C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES + 32 * (box + 1) * 128);
+      // scale atoms as rows of 128 bytes; a tile past the expert's last gives no output, and
+      // past the last expert's reads zeros
+      const int wsf_row = (e * a.m_tiles + mt) * a.nst * (C::SFA_BYTES / 128);
+      const int xsf_row = blk * a.nst * (C::SFB_BYTES / 128);
+      auto load_w = [&](int s, int k) {
+        const uint32_t full = cluster_map(bar_full + 8 * s, 0);
+        if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
+        if (SWIGLU) {
+          tma_load_3d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0,
+                           pol_w);
+        } else {
+          tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
         }
-        for (int k = k0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status)) {
-            ok = 0;
-            break;
-          }
+        tma_load_2d_pair(sSA + s * C::SFA_BYTES, &twsf, full, 0,
+                         wsf_row + k * (C::SFA_BYTES / 128), pol_w);
+      };
+      auto load_x = [&](int s, int k) {
+        const uint32_t full = cluster_map(bar_full + 8 * s, 0);
+        tma_load_2d_pair(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN + rank * half,
+                         pol_x);
+        tma_load_2d_pair(sSB + s * C::SFB_BYTES, &txsf, full, 0,
+                         xsf_row + k * (C::SFB_BYTES / 128), pol_x);
+      };
+      int k0 = 0;
+      if (!waited) {
+        // programmatic dependent of the quantiser: weights first, rows after it
+        k0 = min(a.nst, STAGES);
+        if (elect_one())
+          for (int k = 0; k < k0; ++k) load_w(k, k);
+        pdl_wait();
+        if (elect_one())
+          for (int k = 0; k < k0; ++k) load_x(k, k);
+        __syncwarp();
+        it = k0;
+        waited = true;
+      }
+      for (int k = k0; k < a.nst; ++k, ++it) {
+        const int s = it % STAGES;
+        ok = warp_wait_bounded(bar_empty + 8 * s, ((it / STAGES) & 1) ^ 1, abort_flag, a.status);
+        if (!ok) break;
+        if (elect_one()) {
           load_w(s, k);
           load_x(s, k);
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
-    if (lane == 0 && !waited) pdl_wait();
+    if (!waited) pdl_wait();
   } else if (warp == 1 && leader) {
     // ---- MMAs ----
     int it = 0, n = 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = first; u < units && ok; u += stride) {
       const int blk = u / m_pairs;
       if (expert_of(blk) < 0) continue;
       const int nm = width_of(live_of(blk));
-      if (lane == 0) {
-        ok = mbar_wait_bounded(bar_free, (n & 1) ^ 1, abort_flag, a.status);
+      ok = warp_wait_bounded(bar_free, (n & 1) ^ 1, abort_flag, a.status);
+      tc_fence_after();
+      for (int k = 0; k < a.nst && ok; ++k, ++it) {
+        const int s = it % STAGES;
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
+             warp_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        if (!ok) break;
         tc_fence_after();
-        for (int k = 0; k < a.nst && ok; ++k, ++it) {
-          const int s = it % STAGES;
-          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-               mbar_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-          if (!ok) break;
-          tc_fence_after();
+        if (elect_one()) {
           const uint32_t sf = tmem + BN + s * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
@@ -239,27 +240,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
             }
           }
           tc_commit_pair(bar_empty + 8 * s);
+          if (k == a.nst - 1) tc_commit_pair(bar_acc);
         }
-        if (ok) tc_commit_pair(bar_acc);
+        __syncwarp();
       }
       ++n;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
   } else if (warp == 2 && leader) {
     // ---- scales into both CTAs' tensor memory ----
     int it = 0;
-    int ok = 1;
+    bool ok = true;
     for (int u = first; u < units && ok; u += stride) {
       const int blk = u / m_pairs;
       if (expert_of(blk) < 0) continue;
       const int atoms = live_of(blk) <= 128 ? 1 : 2;
-      if (lane == 0) {
-        for (int k = 0; k < a.nst; ++k, ++it) {
-          const int s = it % STAGES;
-          // a full stage: the MMAs that read its scale columns before are done
-          ok = mbar_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-          if (!ok) break;
-          tc_fence_after();
+      for (int k = 0; k < a.nst; ++k, ++it) {
+        const int s = it % STAGES;
+        // a full stage: the MMAs that read its scale columns before are done
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t sf = tmem + BN + s * C::SF_COLS;
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
@@ -272,8 +273,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
           }
           tc_commit_pair_local(bar_sf + 8 * s);
         }
+        __syncwarp();
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
   } else if (warp >= 4) {
     // ---- epilogue (both CTAs): group g has columns [128 g, 128 g + 128) ----
@@ -284,6 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
     float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
     int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
                                         C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
+    volatile int* my_ok = group_ok + grp;
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
     const uint32_t free_leader = cluster_map(bar_free, 0);
     int n = 0;
@@ -298,7 +300,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         s_row[j] = row < a.out_rows ? row : -1;
       }
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
-      if (!mbar_wait_bounded(bar_acc, n & 1, abort_flag, a.status)) break;
+      // one thread of the group waits, the others rest at the barrier: 256 spinning threads
+      // slow the issuing warps down
+      if (et == 0) *my_ok = mbar_wait_bounded(bar_acc, n & 1, abort_flag, a.status);
+      named_bar_sync(1 + grp, kGroupThreads);
+      if (!*my_ok) break;
       tc_fence_after();
       uint32_t v[C::COLS_THREAD];
       const uint32_t acc = tmem + grp * C::COLS_THREAD + ((uint32_t)(q4 * 32) << 16);
