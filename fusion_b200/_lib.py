@@ -222,7 +222,7 @@ SIGNATURES: dict[str, tuple] = {
     "fus_fp4_weight_scale_bytes": (sz, [i32, i32, i32, i32, i32]),
     "fus_fp4_pack_scales": (i32, [vp, i32, i32, i32, i32, i32, vp, vp]),
     "fus_fp4_grouped_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, vp]),
-    "fus_fp4_expert_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, i32, i64, i32, i32, vp, vp]),
+    "fus_fp4_expert_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, i32, i64, i32, i32, vp, vp, vp]),
     "fus_fold_weight": (i32, [vp, vp, vp, i64, i32, i32, i64, vp, vp]),
     "fus_scale_sum_planes": (i32, [vp, i32, i64, i32, i32, vp, vp, i64, vp, vp]),
     "fus_ep_p2p_decode_forward": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp, vp]),

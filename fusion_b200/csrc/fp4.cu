@@ -158,21 +158,36 @@ FUS_DEVICE uint64_t resolve16(uint64_t lo, uint64_t hi, const uint32_t* r, float
   return lo;
 }
 
+// place of every (token, slot) pair in the dispatch order: pos[id] = p where ids[p] = id. Pairs
+// that are not placed keep junk; the reader checks ids[pos[id]] = id.
+__global__ void fp4_invert_kernel(const int* __restrict__ ids, const int* __restrict__ ntp, int cap,
+                                  int limit, int* __restrict__ pos) {
+  const int used = ntp ? min(__ldg(ntp), cap) : cap;
+  const int p = blockIdx.x * blockDim.x + threadIdx.x;
+  if (p >= used) return;
+  const int id = __ldg(ids + p);
+  if (id >= 0 && id < limit) pos[id] = p;
+}
+
 // One thread quantises 16 elements of `iters` rows; blockDim (UX, 256 / UX), UX a power of two
 // >= 16 that divides the row's padded K / 16, so a row's 256 elements are 16 neighbouring lanes
 // and the scale bytes of a cell, in four (NV) or eight (MX) of them, leave as one 4-byte store.
 // Bound: HBM (2.56 bytes an element from bf16) and, close behind, instruction issue: what
 // does not depend on the row is computed once for several rows.
-template <typename T, int FMT>
+// SPREAD: the rows are tokens, each written to the places of its id_div (token, slot) pairs in
+// the dispatch order, pos[] (checked against ids[]).
+template <typename T, int FMT, bool SPREAD>
 __global__ void __launch_bounds__(256)
     fp4_quantize_kernel(const T* __restrict__ x, int ldx, int x_rows, int rows, int iters,
                         const int* __restrict__ ntp, const int* __restrict__ ids, int id_div,
-                        int id_limit, int K, const float* __restrict__ gscale, int rows_per_g,
+                        int id_limit, const int* __restrict__ pos, int K,
+                        const float* __restrict__ gscale, int rows_per_g,
                         int tile_log2, uint8_t* __restrict__ q, int ldq,
                         uint8_t* __restrict__ sf, int vec, int* status) {
   pdl_allow_dependents();
   const int k = (blockIdx.y * blockDim.x + threadIdx.x) * 16;
-  const int used = ntp ? min(__ldg(ntp), rows) : rows;
+  const int used = !SPREAD && ntp ? min(__ldg(ntp), rows) : rows;
+  const int placed = SPREAD && ntp ? __ldg(ntp) : 0x7fffffff;
   const int j0 = k / fp4_block(FMT);  // this thread's scale
   const int tile = 1 << tile_log2;
   const long per_tile = (long)gridDim.y * blockDim.x / 16 * fp4_stage_scale_bytes(FMT, tile);
@@ -194,7 +209,7 @@ __global__ void __launch_bounds__(256)
   auto fetch = [&](int p) {
     next_live = p < used;
     int src = p;
-    if (next_live && ids) {
+    if (!SPREAD && next_live && ids) {
       const int id = __ldg(ids + p);
       next_live = id >= 0 && id < id_limit;  // dispatch pads keep what their rows held
       src = id_div > 1 ? id / id_div : id;
@@ -259,19 +274,28 @@ __global__ void __launch_bounds__(256)
       byte = FMT == FUS_FP4_MX ? 255 : 127;
       c = make_uint2(0, 0);
     }
-    if (data) *reinterpret_cast<uint2*>(q + (long)p * ldq) = c;
     // scales: NV one byte of each lane, MX one of each lane pair; zeros past K
     if (!data) byte = 0;
     uint32_t word = byte << shift;
 #pragma unroll
     for (int o = kLanes / 4; o < kLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
     if (!live) continue;
-    if (tile_log2 == 0) {
-      if (k < K && (FMT == FUS_FP4_NV || (threadIdx.x & 1) == 0))
-        sf[(long)p * (K / fp4_block(FMT)) + j0] = (uint8_t)byte;
-    } else if ((threadIdx.x & (kLanes - 1)) == 0) {
-      *reinterpret_cast<uint32_t*>(cells + (p >> tile_log2) * per_tile +
-                                   fp4_row_offset(p & (tile - 1))) = word;
+    for (int slot = 0; slot < (SPREAD ? id_div : 1); ++slot) {
+      int d = p;
+      if (SPREAD) {
+        const int id = p * id_div + slot;
+        if (id >= id_limit) break;
+        d = __ldg(pos + id);
+        if (d < 0 || d >= x_rows || d >= placed || __ldg(ids + d) != id) continue;
+      }
+      if (data) *reinterpret_cast<uint2*>(q + (long)d * ldq) = c;
+      if (tile_log2 == 0) {
+        if (k < K && (FMT == FUS_FP4_NV || (threadIdx.x & 1) == 0))
+          sf[(long)d * (K / fp4_block(FMT)) + j0] = (uint8_t)byte;
+      } else if ((threadIdx.x & (kLanes - 1)) == 0) {
+        *reinterpret_cast<uint32_t*>(cells + (d >> tile_log2) * per_tile +
+                                     fp4_row_offset(d & (tile - 1))) = word;
+      }
     }
   }
 }
@@ -395,15 +419,18 @@ int shape_of(long rows, int K, dim3& grid, dim3& block) {
 
 template <typename T>
 int quantize_launch(const void* x, long ldx, int x_rows, long rows, const int* ntp, const int* ids,
-                    int id_div, int id_limit, int K, int fmt, const float* gscale,
+                    int id_div, int id_limit, const int* pos, int K, int fmt, const float* gscale,
                     long rows_per_g, int tile, void* q, long ldq, void* sf, cudaStream_t st,
                     int* status) {
   dim3 grid, block;
   const int iters = shape_of(rows, K, grid, block);
   const int vec = (reinterpret_cast<uintptr_t>(x) % 32) == 0 && (ldx * (long)sizeof(T)) % 32 == 0;
-  auto fn = fmt == FUS_FP4_MX ? fp4_quantize_kernel<T, FUS_FP4_MX> : fp4_quantize_kernel<T, FUS_FP4_NV>;
+  auto fn = pos ? (fmt == FUS_FP4_MX ? fp4_quantize_kernel<T, FUS_FP4_MX, true>
+                                     : fp4_quantize_kernel<T, FUS_FP4_NV, true>)
+                : (fmt == FUS_FP4_MX ? fp4_quantize_kernel<T, FUS_FP4_MX, false>
+                                     : fp4_quantize_kernel<T, FUS_FP4_NV, false>);
   fn<<<grid, block, 0, st>>>(reinterpret_cast<const T*>(x), (int)ldx, x_rows, (int)rows, iters, ntp,
-                             ids, id_div, id_limit, K, gscale, (int)rows_per_g, log2_of(tile),
+                             ids, id_div, id_limit, pos, K, gscale, (int)rows_per_g, log2_of(tile),
                              reinterpret_cast<uint8_t*>(q), (int)ldq,
                              reinterpret_cast<uint8_t*>(sf), vec, status);
   return check_launch("fp4_quantize");
@@ -436,6 +463,22 @@ int check_common(const char* what, int fmt, int dtype, long rows, int K, int til
 }
 
 }  // namespace
+
+int fp4_quantize_spread(const void* x, int dtype, long ldx, int T, int K, int fmt, const float* g,
+                        const int* ids, int per_token, int limit, const int* ntp, int cap, int tile,
+                        int* pos, void* q, long ldq, void* sf, void* stream, int* status) {
+  cudaStream_t st = as_stream(stream);
+  fp4_invert_kernel<<<(cap + 255) / 256, 256, 0, st>>>(ids, ntp, cap, limit, pos);
+  if (int rc = check_launch("fp4_quantize")) return rc;
+#define FUS_Q(E)                                                                                 \
+  quantize_launch<E>(x, ldx, cap, T, ntp, ids, per_token, limit, pos, K, fmt, g, 0, tile, q, ldq, \
+                     sf, st, status)
+  if (dtype == FUS_DT_BF16) return FUS_Q(__nv_bfloat16);
+  if (dtype == FUS_DT_F16) return FUS_Q(__half);
+  return FUS_Q(float);
+#undef FUS_Q
+}
+
 }  // namespace fus
 
 using namespace fus;
@@ -468,7 +511,7 @@ extern "C" int fus_fp4_quantize(const void* x, int dtype, long ldx, int x_rows, 
     return set_error(FUS_E_INVALID, "fp4_quantize: FUS_FP4_MX takes no factor");
   cudaStream_t st = as_stream(stream);
 #define FUS_Q(T)                                                                               \
-  quantize_launch<T>(x, ldx, x_rows, rows, ntp, ids, id_div, id_limit, K, fmt, gscale,          \
+  quantize_launch<T>(x, ldx, x_rows, rows, ntp, ids, id_div, id_limit, nullptr, K, fmt, gscale,          \
                      rows_per_g, tile, q, ldq, sf, st, status)
   if (dtype == FUS_DT_BF16) return FUS_Q(__nv_bfloat16);
   if (dtype == FUS_DT_F16) return FUS_Q(__half);

@@ -19,10 +19,10 @@
 //             MMAs, into columns of that stage. Issued by the MMA thread they would run in order
 //             with the MMAs, about 55 cycles each: 12 of them for 512 cycles of MMA (dense
 //             8192 x 4096 x 6144 NV: 290 -> 230 us with 128-token blocks)
-//   warps 4-11 (4-7 up to 64 token columns): epilogue, two groups that take chunks of 32 columns
-//             in turn, TMEM -> registers -> shared (token-major) -> 16-byte stores
-// Up to 128 token columns the accumulator is double-buffered: the next unit's MMAs run while
-// the epilogue drains.
+//   warps 4-7: epilogue, TMEM -> registers -> shared (token-major) -> 16-byte stores
+// The accumulator is double-buffered: the next unit's MMAs run while the epilogue drains.
+// Blocks up to 64 tokens run here, two CTAs on an SM (bound by HBM: the weights); wider ones on
+// SM pairs, fp4_gemm_pair.cuh.
 #include "fp4.cuh"
 #include "host_util.h"
 
@@ -64,33 +64,32 @@ struct TokenMaps {
   CUtensorMap m[4];
 };
 
+constexpr long kSpreadElements = 1 << 22;  // see fus_fp4_expert_gemm
+
 constexpr int kGroupThreads = 128;  // an epilogue group: the four lane quarters of TMEM
 
 template <int BN, int FMT>
 struct Cfg {
   static constexpr int CELLS = fp4_cells(FMT);
-  static constexpr int ATOMS = fp4_atoms(BN);
   static constexpr int A_BYTES = 128 * 128;
   static constexpr int B_BYTES = BN * 128;
   static constexpr int SFA_BYTES = CELLS * 512;
-  static constexpr int SFB_BYTES = CELLS * ATOMS * 512;
+  static constexpr int SFB_BYTES = CELLS * 512;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int CHUNK = BN < 32 ? BN : 32;  // token columns of an epilogue step
-  static constexpr int GROUPS = BN > 64 ? 2 : 1;
-  static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
-  static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);  // staging, row numbers
-  // two CTAs for an SM up to 64 token columns (TMEM 256 columns each), else one
-  static constexpr int CTAS = BN <= 64 ? 2 : 1;
-  static constexpr int RING_TARGET = (CTAS == 2 ? 112 : 226) * 1024 - EPI_BYTES - 1280;
+  static constexpr int THREADS = 128 + kGroupThreads;
+  static constexpr int EPI_BYTES = CHUNK * 128 * 4 + BN * 4;  // staging, row numbers
+  static constexpr int CTAS = 2;                              // for an SM (TMEM 256 columns each)
+  static constexpr int RING_TARGET = 112 * 1024 - EPI_BYTES - 1280;
   static constexpr int STAGES = RING_TARGET / STAGE_BYTES > 8 ? 8 : RING_TARGET / STAGE_BYTES;
-  static constexpr int ACCS = BN <= 128 ? 2 : 1;
+  static constexpr int ACCS = 2;
   static constexpr int SFB_OFF = CELLS * 4;                      // token scales, after the weights'
-  static constexpr int SF_COLS = SFB_OFF + CELLS * ATOMS * 4;    // a stage's scales
+  static constexpr int SF_COLS = SFB_OFF + CELLS * 4;            // a stage's scales
   static constexpr int SF_COL = ACCS * BN;
   static constexpr int COLS = SF_COL + STAGES * SF_COLS;
-  static constexpr int TMEM_COLS = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static constexpr int TMEM_COLS = COLS <= 128 ? 128 : 256;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
-  static_assert(STAGES >= 3 && CTAS * TMEM_COLS <= 512 && COLS <= 512, "resources");
+  static_assert(STAGES >= 3 && CTAS * TMEM_COLS <= 512 && COLS <= TMEM_COLS, "resources");
 };
 
 // Instruction descriptor of the block-scaled kinds: bits 4-5 B scale id, 7-9 / 10-11 A / B
@@ -177,7 +176,7 @@ FUS_DEVICE void store_chunk(const Fp4Args& a, const float* S, const int* rows, i
 
 template <int BN, int FMT, bool SWIGLU>
 __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
-    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ TokenMaps tx,
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
                     const __grid_constant__ Fp4Args a) {
   using C = Cfg<BN, FMT>;
   constexpr int STAGES = C::STAGES;
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
   const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // a stage's scales are in tensor memory
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [GROUPS]
+  volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -207,12 +206,12 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(bar_acc + 8 * b, 1);
-      mbar_init(bar_free + 8 * b, 4 * C::GROUPS);
+      mbar_init(bar_free + 8 * b, 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tw);
-    tma_prefetch_desc(&tx.m[0]);
+    tma_prefetch_desc(&tx);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
@@ -252,14 +251,11 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
       const int e = expert_of(blk);
       if (e < 0) continue;
-      const int box = BN > 64 ? max(0, (live_of(blk) - 1) / 32) : 0;
       const uint8_t* wsf = a.wsf + ((long)e * a.m_tiles + mt) * a.nst * C::SFA_BYTES;
       const uint8_t* xsf = a.xsf + (long)blk * a.nst * C::SFB_BYTES;
-      const uint32_t bytes = C::A_BYTES + C::SFA_BYTES + C::SFB_BYTES +
-                             (BN > 64 ? 32 * (box + 1) : BN) * 128;
       auto load_w = [&](int s, int k) {
         const uint32_t full = bar_full + 8 * s;
-        mbar_arrive_expect_tx(full, bytes);
+        mbar_arrive_expect_tx(full, C::STAGE_BYTES);
         if (SWIGLU) {  // 64 gate rows, their 64 up rows
           tma_load_3d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0, pol_w);
         } else {
@@ -269,7 +265,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       };
       auto load_x = [&](int s, int k) {
         const uint32_t full = bar_full + 8 * s;
-        tma_load_2d(sB + s * C::B_BYTES, &tx.m[box], full, k * 128, blk * BN, pol_x);
+        tma_load_2d(sB + s * C::B_BYTES, &tx, full, k * 128, blk * BN, pol_x);
         bulk_load(sSB + s * C::SFB_BYTES, xsf + (long)k * C::SFB_BYTES, C::SFB_BYTES, full, pol_x);
       };
       int k0 = 0;
@@ -325,7 +321,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
               const int id = FMT == FUS_FP4_MX ? (j % 2) * 2 : 0;
               tc_mma_fp4<FMT>(acc, sw128_desc(sA + s * C::A_BYTES + 32 * j),
                               sw128_desc(sB + s * C::B_BYTES + 32 * j), fp4_idesc<FMT>(128, nm, id),
-                              sf + 4 * cell, sf + C::SFB_OFF + 4 * C::ATOMS * cell, (k | j) != 0);
+                              sf + 4 * cell, sf + C::SFB_OFF + 4 * cell, (k | j) != 0);
             }
           }
           tc_commit(bar_empty + 8 * s);
@@ -341,8 +337,6 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       const int blk = u / a.m_tiles;
       if (expert_of(blk) < 0) continue;
-      // atoms of token scales that hold live rows
-      const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
       for (int k = 0; k < a.nst; ++k, ++it) {
         const int s = it % STAGES;
         // a full stage: the MMAs that read its scale columns before are done
@@ -354,11 +348,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
             tc_cp_scales(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
-#pragma unroll
-            for (int t = 0; t < C::ATOMS; ++t)
-              if (t < atoms)
-                tc_cp_scales(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
-                             sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
+            tc_cp_scales(sf + C::SFB_OFF + 4 * c, sSB + s * C::SFB_BYTES + 512 * c);
           }
           tc_commit(bar_sf + 8 * s);
         }
@@ -367,13 +357,10 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     }
   } else if (warp >= 4) {
     const int q4 = warp & 3;  // the TMEM lanes this warp may read
-    const int grp = (warp - 4) >> 2;
     const int m = q4 * 32 + lane;
-    const int et = threadIdx.x - 128 - grp * kGroupThreads;
-    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
-    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
-                                        C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
-    volatile int* my_ok = group_ok + grp;
+    const int et = threadIdx.x - 128;
+    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES);
+    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES + C::CHUNK * 128 * 4);
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
     int n = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
@@ -381,7 +368,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int live = live_of(blk);
-      // output rows, out of range: -1 (read by this group only, after its barrier below)
+      // output rows, out of range: -1 (read after the barrier below)
       for (int j = et; j < live; j += kGroupThreads) {
         const int pos = blk * BN + j;
         const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
@@ -391,12 +378,12 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const int buf = n % C::ACCS;
       // one thread of the group waits, the others rest at the barrier: 256 spinning threads
       // slow the issuing warps down
-      if (et == 0) *my_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
-      named_bar_sync(1 + grp, kGroupThreads);
-      if (!*my_ok) break;
+      if (et == 0) *group_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
+      named_bar_sync(1, kGroupThreads);
+      if (!*group_ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q4 * 32) << 16);
-      for (int c0 = grp * C::CHUNK; c0 < live; c0 += C::GROUPS * C::CHUNK) {
+      for (int c0 = 0; c0 < live; c0 += C::CHUNK) {
         uint32_t v[C::CHUNK];
 #pragma unroll
         for (int c = 0; c < C::CHUNK; c += 16) tmem_ld16_issue(acc + c0 + c, v + c);
@@ -404,9 +391,9 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
         for (int c = 0; c < C::CHUNK; c += 16) tmem_ld_wait(v + c);
 #pragma unroll
         for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[j]) * alpha;
-        named_bar_sync(1 + grp, kGroupThreads);
+        named_bar_sync(1, kGroupThreads);
         store_chunk<SWIGLU, C::CHUNK>(a, S, s_row + c0, min(C::CHUNK, live - c0), mt, et);
-        named_bar_sync(1 + grp, kGroupThreads);
+        named_bar_sync(1, kGroupThreads);
       }
       tc_fence_before();
       __syncwarp();
@@ -440,7 +427,7 @@ int launch(const CUtensorMap& tw, const TokenMaps& tx, const Fp4Args& a, long un
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = a.pdl ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tw, tx, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tw, tx.m[0], a);
   if (e != cudaSuccess)
     return set_error(FUS_E_LAUNCH, "fp4_grouped_gemm: %s", cudaGetErrorString(e));
   return check_launch("fp4_grouped_gemm");
@@ -459,8 +446,8 @@ int launch_bn(int bn, const CUtensorMap& tw, const TokenMaps& tx, const fus_fp4_
     case 16: return launch<16, FMT, SWIGLU>(tw, tx, a, units, st);
     case 32: return launch<32, FMT, SWIGLU>(tw, tx, a, units, st);
     case 64: return launch<64, FMT, SWIGLU>(tw, tx, a, units, st);
-    case 128: return launch<128, FMT, SWIGLU>(tw, tx, a, units, st);
-    default: return launch_pair<FMT, SWIGLU>(tw, tx, d, a, (int)(units / a.m_tiles), st);
+    case 128: return launch_pair<128, FMT, SWIGLU>(tw, tx, d, a, (int)(units / a.m_tiles), st);
+    default: return launch_pair<256, FMT, SWIGLU>(tw, tx, d, a, (int)(units / a.m_tiles), st);
   }
 }
 
@@ -566,18 +553,40 @@ extern "C" int fus_fp4_grouped_gemm(const fus_fp4_gemm_desc* d, void* stream, in
 }
 
 extern "C" int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, int x_dtype,
-                                   long ldx, int src_rows, int gather_div, void* stream,
-                                   int* status) {
+                                   long ldx, int src_rows, int gather_div, int* pair_ws,
+                                   void* stream, int* status) {
   if (int rc = check_gemm(d)) return rc;
   if (d->x_rows == 0 || d->out_rows == 0) return FUS_OK;
   if (gather_div < 0 || (gather_div > 0 && !d->live_ids))
     return set_error(FUS_E_INVALID, "fp4_expert_gemm: gathered rows need live_ids");
+  if (gather_div > 0 && (long)src_rows * gather_div < d->live_limit)
+    return set_error(FUS_E_INVALID, "fp4_expert_gemm: %d rows for %d pairs", src_rows, d->live_limit);
+  // Large batches: a token is quantised once and written to its pairs' rows (two launches: the
+  // places, then the rows). One pass over the dispatch order, which quantises a token for each
+  // of its pairs, has a launch less (2.2 us) and more to compute (1.4 to 2.2 million elements a
+  // us). NV, spread / one pass: 8192 pairs of 1024 tokens, K 6144 121 / 144 us with the product,
+  // 1024 of 128, K 6144 91.8 / 95.8, 1024 of 128, K 2048 19.1 / 16.9.
+  const bool spread = pair_ws && gather_div > 1 &&
+                      ((long)d->live_limit - src_rows) * d->K >= kSpreadElements;
   // rows in dispatch order: pads are skipped by their id, gathered or not
-  if (int rc = fus_fp4_quantize(x, x_dtype, ldx, src_rows, d->K, d->fmt, d->xg, 0,
-                                gather_div ? d->live_ids : nullptr, gather_div ? gather_div : 1,
-                                d->live_limit, d->ntp, d->x_rows, d->block_n,
-                                const_cast<void*>(d->xq), d->ldxq, const_cast<void*>(d->xsf),
-                                stream, status))
+  if (spread) {
+    // the checks of fus_fp4_quantize, on no rows
+    if (int rc = fus_fp4_quantize(x, x_dtype, ldx, src_rows, d->K, d->fmt, d->xg, 0, nullptr, 1, 0,
+                                  nullptr, 0, d->block_n, nullptr, 0, nullptr, stream, status))
+      return rc;
+    if (!x || ldx < d->K || ldx > 0x7fffffffL || d->ldxq > 0x7fffffffL)
+      return set_error(FUS_E_INVALID, "fp4_expert_gemm: bad source rows");
+    if (int rc = fp4_quantize_spread(x, x_dtype, ldx, src_rows, d->K, d->fmt, d->xg, d->live_ids,
+                                     gather_div, d->live_limit, d->ntp, d->x_rows, d->block_n,
+                                     pair_ws, const_cast<void*>(d->xq), d->ldxq,
+                                     const_cast<void*>(d->xsf), stream, status))
+      return rc;
+  } else if (int rc = fus_fp4_quantize(x, x_dtype, ldx, src_rows, d->K, d->fmt, d->xg, 0,
+                                       gather_div ? d->live_ids : nullptr,
+                                       gather_div ? gather_div : 1, d->live_limit, d->ntp,
+                                       d->x_rows, d->block_n, const_cast<void*>(d->xq), d->ldxq,
+                                       const_cast<void*>(d->xsf), stream, status)) {
     return rc;
+  }
   return gemm_launch(d, 1, stream, status);
 }

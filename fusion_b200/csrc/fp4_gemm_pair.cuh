@@ -1,5 +1,5 @@
-// SM-pair form of the four-bit product for 256-token blocks (tcgen05 cta_group::2). Included by
-// fp4_gemm.cu.
+// SM-pair form of the four-bit product for blocks of 128 and 256 tokens (tcgen05 cta_group::2).
+// Included by fp4_gemm.cu.
 //
 // At 256 tokens for an expert the product is bound by what a stage brings into shared memory
 // and the MMAs read back from it, not by the tensor pipe: a 128 x 256 tile of one CTA moves
@@ -11,33 +11,36 @@
 // Both CTAs' copies complete on the leader's full barrier (tensor copies of .cta_group::2, the
 // scales too; no multicast). The leader's warp 2 copies both CTAs' scales into their tensor
 // memory (tcgen05.cp.cta_group::2), its warp 1 issues the MMAs; commits free the stage and
-// hand over the accumulators on both CTAs. The accumulators fill 256 columns and are not
-// double-buffered: the epilogue reads them into registers at once (128 columns for a
-// thread) and frees them before it converts and stores.
+// hand over the accumulators on both CTAs. 256 columns hold them, two buffers of 128-token
+// blocks or one of 256: the epilogue reads its half into registers at once and frees the
+// buffer before it converts and stores.
 #pragma once
 
 namespace {
 
-template <int FMT>
+template <int BN, int FMT>
 struct PairCfg {
-  static constexpr int BN = 256;
   static constexpr int CELLS = fp4_cells(FMT);
   static constexpr int A_BYTES = 128 * 128;
-  static constexpr int B_BYTES = 128 * 128;  // half of the tokens
+  static constexpr int ATOMS = fp4_atoms(BN);
+  static constexpr int B_BYTES = BN / 2 * 128;  // half of the tokens
   static constexpr int SFA_BYTES = CELLS * 512;
-  static constexpr int SFB_BYTES = CELLS * 1024;
+  static constexpr int SFB_BYTES = CELLS * ATOMS * 512;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int GROUPS = 2;
   static constexpr int COLS_THREAD = BN / GROUPS;  // accumulator columns of a thread
   static constexpr int CHUNK = 32;
   static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
   static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);
-  static constexpr int STAGES = (226 * 1024 - EPI_BYTES - 1280) / STAGE_BYTES;
+  static constexpr int FIT = (226 * 1024 - EPI_BYTES - 1280) / STAGE_BYTES;
+  static constexpr int STAGES = FIT > 7 ? 7 : FIT;
+  static constexpr int ACCS = 256 / BN;  // accumulators
   static constexpr int SFB_OFF = CELLS * 4;
-  static constexpr int SF_COLS = SFB_OFF + CELLS * 8;
+  static constexpr int SF_COLS = SFB_OFF + CELLS * ATOMS * 4;  // a stage's scales
+  static constexpr int SF_COL = ACCS * BN;
   static constexpr int TMEM_COLS = 512;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + 256 + 1024;
-  static_assert(BN + STAGES * SF_COLS <= TMEM_COLS && STAGES >= 4, "resources");
+  static_assert(SF_COL + STAGES * SF_COLS <= TMEM_COLS && STAGES >= 4, "resources");
 };
 
 template <int FMT>
@@ -71,15 +74,15 @@ FUS_DEVICE void tc_commit_pair_local(uint32_t bar) {
       : "memory");
 }
 
-template <int FMT, bool SWIGLU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREADS, 1)
+template <int BN, int FMT, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::THREADS), 1)
     fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tw,
                          const __grid_constant__ TokenMaps tx,
                          const __grid_constant__ CUtensorMap twsf,
                          const __grid_constant__ CUtensorMap txsf,
                          const __grid_constant__ Fp4Args a) {
-  using C = PairCfg<FMT>;
-  constexpr int STAGES = C::STAGES, BN = C::BN;
+  using C = PairCfg<BN, FMT>;
+  constexpr int STAGES = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   // the same offsets in both CTAs: the dynamic window starts at the same address in each
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -92,9 +95,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
   const uint32_t bar_full = smem_u32(bars);          // leader's used
   const uint32_t bar_empty = bar_full + 8 * STAGES;  // both
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // both
-  const uint32_t bar_free = bar_acc + 8;             // leader's used
-  const uint32_t bar_sf = bar_free + 8;              // leader's used
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2);
+  const uint32_t bar_free = bar_acc + 8 * C::ACCS;   // leader's used
+  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // leader's used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [GROUPS]
 
@@ -107,8 +110,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       mbar_init(bar_empty + 8 * s, 1);
       mbar_init(bar_sf + 8 * s, 1);
     }
-    mbar_init(bar_acc, 1);
-    mbar_init(bar_free, 2 * 4 * C::GROUPS);
+    for (int b = 0; b < C::ACCS; ++b) {
+      mbar_init(bar_acc + 8 * b, 1);
+      mbar_init(bar_free + 8 * b, 2 * 4 * C::GROUPS);
+    }
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tw);
@@ -217,7 +222,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       const int blk = u / m_pairs;
       if (expert_of(blk) < 0) continue;
       const int nm = width_of(live_of(blk));
-      ok = warp_wait_bounded(bar_free, (n & 1) ^ 1, abort_flag, a.status);
+      const int buf = n % C::ACCS;
+      ok = warp_wait_bounded(bar_free + 8 * buf, ((n / C::ACCS) & 1) ^ 1, abort_flag, a.status);
       tc_fence_after();
       for (int k = 0; k < a.nst && ok; ++k, ++it) {
         const int s = it % STAGES;
@@ -226,21 +232,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t sf = tmem + BN + s * C::SF_COLS;
+          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j < steps) {
               const int cell = FMT == FUS_FP4_MX ? j / 2 : j;
               const int id = FMT == FUS_FP4_MX ? (j % 2) * 2 : 0;
-              tc_mma_fp4_pair<FMT>(tmem, sw128_desc(sA + s * C::A_BYTES + 32 * j),
+              tc_mma_fp4_pair<FMT>(tmem + buf * BN, sw128_desc(sA + s * C::A_BYTES + 32 * j),
                                    sw128_desc(sB + s * C::B_BYTES + 32 * j),
                                    fp4_idesc<FMT>(256, nm, id), sf + 4 * cell,
-                                   sf + C::SFB_OFF + 8 * cell, (k | j) != 0);
+                                   sf + C::SFB_OFF + 4 * C::ATOMS * cell, (k | j) != 0);
             }
           }
           tc_commit_pair(bar_empty + 8 * s);
-          if (k == a.nst - 1) tc_commit_pair(bar_acc);
+          if (k == a.nst - 1) tc_commit_pair(bar_acc + 8 * buf);
         }
         __syncwarp();
       }
@@ -253,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
     for (int u = first; u < units && ok; u += stride) {
       const int blk = u / m_pairs;
       if (expert_of(blk) < 0) continue;
-      const int atoms = live_of(blk) <= 128 ? 1 : 2;
+      const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
       for (int k = 0; k < a.nst; ++k, ++it) {
         const int s = it % STAGES;
         // a full stage: the MMAs that read its scale columns before are done
@@ -261,15 +267,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t sf = tmem + BN + s * C::SF_COLS;
+          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
 #pragma unroll
           for (int c = 0; c < C::CELLS; ++c) {
             tc_cp_scales_pair(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < C::ATOMS; ++t)
               if (t < atoms)
-                tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * 2 + t),
-                                  sSB + s * C::SFB_BYTES + 512 * (c * 2 + t));
+                tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
+                                  sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
           }
           tc_commit_pair_local(bar_sf + 8 * s);
         }
@@ -277,7 +283,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       }
     }
   } else if (warp >= 4) {
-    // ---- epilogue (both CTAs): group g has columns [128 g, 128 g + 128) ----
+    // ---- epilogue (both CTAs): each group has half of the columns ----
     const int q4 = warp & 3;
     const int grp = (warp - 4) >> 2;
     const int m = q4 * 32 + lane;
@@ -287,13 +293,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
                                         C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
     volatile int* my_ok = group_ok + grp;
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
-    const uint32_t free_leader = cluster_map(bar_free, 0);
     int n = 0;
     for (int u = first; u < units; u += stride) {
       const int blk = u / m_pairs, mt = (u - blk * m_pairs) * 2 + rank;
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int live = live_of(blk) - grp * C::COLS_THREAD;  // of this group's columns
+      const int buf = n % C::ACCS;
       for (int j = et; j < min(live, C::COLS_THREAD); j += kGroupThreads) {
         const int pos = blk * BN + grp * C::COLS_THREAD + j;
         const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
@@ -302,12 +308,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
       // one thread of the group waits, the others rest at the barrier: 256 spinning threads
       // slow the issuing warps down
-      if (et == 0) *my_ok = mbar_wait_bounded(bar_acc, n & 1, abort_flag, a.status);
+      if (et == 0) *my_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
       named_bar_sync(1 + grp, kGroupThreads);
       if (!*my_ok) break;
       tc_fence_after();
       uint32_t v[C::COLS_THREAD];
-      const uint32_t acc = tmem + grp * C::COLS_THREAD + ((uint32_t)(q4 * 32) << 16);
+      const uint32_t acc = tmem + buf * BN + grp * C::COLS_THREAD + ((uint32_t)(q4 * 32) << 16);
 #pragma unroll
       for (int c = 0; c < C::COLS_THREAD; c += 16)
         if (c < live) tmem_ld16_issue(acc + c, v + c);
@@ -316,7 +322,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
         if (c < live) tmem_ld_wait(v + c);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(free_leader);
+      if (lane == 0) mbar_arrive_remote(cluster_map(bar_free + 8 * buf, 0));
       ++n;
 #pragma unroll
       for (int c0 = 0; c0 < C::COLS_THREAD; c0 += C::CHUNK) {
@@ -338,11 +344,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg<FMT>::THREAD
   if (warp == 1) tmem_dealloc_pair(tmem, C::TMEM_COLS);
 }
 
-template <int FMT, bool SWIGLU>
+template <int BN, int FMT, bool SWIGLU>
 int launch_pair(const CUtensorMap& tw, const TokenMaps& tx, const fus_fp4_gemm_desc* d,
                 const Fp4Args& a, int blocks, cudaStream_t st) {
-  using C = PairCfg<FMT>;
-  auto fn = fp4_gemm_pair_kernel<FMT, SWIGLU>;
+  using C = PairCfg<BN, FMT>;
+  auto fn = fp4_gemm_pair_kernel<BN, FMT, SWIGLU>;
   if (int rc = ensure_smem_attr((const void*)fn, C::SMEM_BYTES, "fp4_grouped_gemm")) return rc;
   CUtensorMap twsf, txsf;
   const uint64_t wsf_rows = (uint64_t)a.n_experts * a.m_tiles * a.nst * (C::SFA_BYTES / 128);

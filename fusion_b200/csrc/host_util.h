@@ -76,6 +76,12 @@ int route_small_launch(const void* h, const void* r, const void* gamma, float ep
 int route_small_check(int T, int H, int E, int topk, int n_group, int topk_group, int block_m,
                       int nplanes);
 
+// fus_fp4_quantize of T tokens whose rows go to the places of their `per_token` pairs in a dispatch
+// order of `cap` rows (arguments checked by the caller); pos: `limit` ints of workspace
+int fp4_quantize_spread(const void* x, int dtype, long ldx, int T, int K, int fmt, const float* g,
+                        const int* ids, int per_token, int limit, const int* ntp, int cap, int tile,
+                        int* pos, void* q, long ldq, void* sf, void* stream, int* status);
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }

@@ -100,8 +100,8 @@ class ExpertGemmFP4:
         d = L.Fp4GemmDesc.from_buffer_copy(self._desc)
         # the packed rows: fresh for each call, so calls on other streams and captured graphs
         # never share them
-        rows = torch.empty(cap * d.ldxq + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n),
-                           dtype=torch.uint8, device=self.device)
+        size = cap * d.ldxq + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n)
+        rows = torch.empty(size + 4 * pairs, dtype=torch.uint8, device=self.device)
         d.xq = ops._p(rows)
         d.xsf = d.xq + cap * d.ldxq
         d.x_rows, d.block_n = cap, block_n
@@ -111,5 +111,5 @@ class ExpertGemmFP4:
         d.out, d.ldo = ops._p(out), ops._rows2d(out, "out")
         d.out_rows, d.out_dtype = out.shape[0], ops.DT[out.dtype]
         ops._call_on(self._dev, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
-                     x.shape[0], topk if gather else 0)
+                     x.shape[0], topk if gather else 0, d.xq + size)
         return out

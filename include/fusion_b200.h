@@ -419,8 +419,9 @@ int fus_fp4_pack_scales(const void* scales, int fmt, int n_experts, int w_rows, 
  * 32, 64, 128, 256}, 16-byte aligned rows. Rows of out outside [0, out_rows) are dropped.
  * fus_fp4_expert_gemm quantises the rows first, into the descriptor's xq and xsf (then
  * workspaces, not inputs): dispatch row p is x[live_ids[p] / gather_div], or x[p] with
- * gather_div 0. The two kernels overlap (the weights are requested while rows are
- * quantised). */
+ * gather_div 0. The quantisation and the product overlap (the weights are requested while
+ * rows are quantised). pair_ws: live_limit ints of workspace or NULL; with it the tokens of
+ * large batches are quantised once each instead of once for each of their pairs. */
 typedef struct fus_fp4_gemm_desc {
   const void* wq;         /* [n_experts, w_rows, K / 2] packed weights                      */
   const void* wsf;        /* their scale tiles (fus_fp4_pack_scales)                        */
@@ -446,7 +447,7 @@ typedef struct fus_fp4_gemm_desc {
 } fus_fp4_gemm_desc;
 int fus_fp4_grouped_gemm(const fus_fp4_gemm_desc* d, void* stream, int* status);
 int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, int x_dtype, long ldx,
-                        int src_rows, int gather_div, void* stream, int* status);
+                        int src_rows, int gather_div, int* pair_ws, void* stream, int* status);
 
 /* ---------------------------------------------------------------------------------
  * Element-wise / merge kernels

@@ -101,8 +101,8 @@ def test_gemm_refusals():
                      ({"ldxq": 16}, "aligned"), ({"x_rows": -1}, "row counts")):
         _refused(call(**kw), text)
     d = desc(live_ids=None, scatter=0)
-    _refused(L.lib().fus_fp4_expert_gemm(ctypes.byref(d), P, 0, 64, 4, 8, None, None), "live_ids")
-    _refused(L.lib().fus_fp4_expert_gemm(None, P, 0, 64, 4, 8, None, None), "null descriptor")
+    _refused(L.lib().fus_fp4_expert_gemm(ctypes.byref(d), P, 0, 64, 4, 8, None, None, None), "live_ids")
+    _refused(L.lib().fus_fp4_expert_gemm(None, P, 0, 64, 4, 8, None, None, None), "null descriptor")
 
 
 def test_python_refusals():
