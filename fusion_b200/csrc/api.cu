@@ -87,30 +87,39 @@ int make_tmap_bf16_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t
   return FUS_OK;
 }
 
-int make_tmap_u8_3d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
-                    uint64_t planes, uint64_t plane_ld, uint32_t box_inner, uint32_t box_rows,
-                    uint32_t box_planes, bool swizzle) {
+int make_tmap_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box, bool swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return set_error(FUS_E_LAUNCH, "cuTensorMapEncodeTiled unavailable");
-  if (!aligned16(base) || ld % 16 || plane_ld % 16)
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], es[5];
+  bool aligned = aligned16(base);
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+    es[i] = 1;
+    if (i) {
+      st[i - 1] = strides[i - 1];
+      aligned = aligned && strides[i - 1] % 16 == 0;
+    }
+  }
+  if (!aligned)
     return set_error(FUS_E_INVALID, "tensor map: base and row pitch must be 16-byte aligned");
-  cuuint64_t dims[3] = {inner, rows, planes};
-  cuuint64_t strides[2] = {ld, plane_ld};
-  cuuint32_t box[3] = {box_inner, box_rows, box_planes};
-  cuuint32_t es[3] = {1, 1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes > 1 ? 3 : 2, const_cast<void*>(base),
-                  dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), d, st, b, es,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(FUS_E_INVALID, "cuTensorMapEncodeTiled failed (%d): inner=%llu rows=%llu",
-                     (int)r, (unsigned long long)inner, (unsigned long long)rows);
+                     (int)r, (unsigned long long)dims[0], (unsigned long long)dims[1]);
   return FUS_OK;
 }
 
 int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
                     uint32_t box_inner, uint32_t box_rows, bool swizzle) {
-  return make_tmap_u8_3d(m, base, inner, rows, ld, 1, 0, box_inner, box_rows, 1, swizzle);
+  const uint64_t dims[2] = {inner, rows};
+  const uint32_t box[2] = {box_inner, box_rows};
+  return make_tmap_u8(m, base, 2, dims, &ld, box, swizzle);
 }
 
 int make_tmap_store_2d(CUtensorMap* m, const void* base, bool f32, uint64_t inner, uint64_t rows,

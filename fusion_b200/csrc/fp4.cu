@@ -364,7 +364,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // row-major scales [n_experts * w_rows, K / n] -> weight scale tiles of 128 rows for each
-// expert; gate_up: tile t holds gate rows [64t, 64t + 64) and their up rows
+// expert; gate_up: tile t holds gate rows [64t, 64t + 64) and their up rows, 8 and 8 in turn
 __global__ void fp4_pack_kernel(const uint8_t* __restrict__ src, int n_experts, int w_rows,
                                 int tiles, int n_scales, int fmt, int gate_up, long per_tile,
                                 uint8_t* __restrict__ dst, long words) {
@@ -378,8 +378,8 @@ __global__ void fp4_pack_kernel(const uint8_t* __restrict__ src, int n_experts, 
   const int e = (int)(t / tiles), tl = (int)(t % tiles);
   int row;
   if (gate_up) {
-    const int f = tl * 64 + (r & 63);
-    row = f < w_rows / 2 ? f + (r >= 64 ? w_rows / 2 : 0) : w_rows;
+    const int f = tl * 64 + r / 16 * 8 + r % 8;
+    row = f < w_rows / 2 ? f + (r % 16 >= 8 ? w_rows / 2 : 0) : w_rows;
   } else {
     row = tl * 128 + r;
   }

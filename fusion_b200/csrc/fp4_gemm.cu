@@ -78,7 +78,8 @@ struct Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int CHUNK = BN < 32 ? BN : 32;  // token columns of an epilogue step
   static constexpr int THREADS = 128 + kGroupThreads;
-  static constexpr int EPI_BYTES = CHUNK * 128 * 4 + BN * 4;  // staging, row numbers
+  static constexpr int STAGE_OUT = CHUNK * 256;  // staged bf16 rows, two buffers
+  static constexpr int EPI_BYTES = 2 * STAGE_OUT + BN * 8;  // ..., row numbers and scales
   static constexpr int CTAS = 2;                              // for an SM (TMEM 256 columns each)
   static constexpr int RING_TARGET = 112 * 1024 - EPI_BYTES - 1280;
   static constexpr int STAGES = RING_TARGET / STAGE_BYTES > 8 ? 8 : RING_TARGET / STAGE_BYTES;
@@ -134,43 +135,162 @@ FUS_DEVICE void tc_cp_scales(uint32_t taddr, uint32_t saddr) {
                : "memory");
 }
 
-// The group's staged chunk, token-major [CHUNK][128] fp32, to its output rows: nj live tokens,
-// rows[] their output rows (-1: none), weight tile mt; 16 bytes for a thread and row.
-template <bool SWIGLU, int CHUNK>
-FUS_DEVICE void store_chunk(const Fp4Args& a, const float* S, const int* rows, int nj, int mt,
-                            int et) {
-  constexpr int PER = SWIGLU ? 8 : 16;  // threads of a token row, 8 features each
-  const int f = (et % PER) * 8;
-  const int col = mt * (SWIGLU ? 64 : 128) + f;
+// ---- epilogue: TMEM -> registers -> shared -> global ----
+// A warp reads its 32 lanes (weight rows) as two 16-lane fragments v[2][4 NI] of NI x 8 token
+// columns: a thread has rows t / 4 and t / 4 + 8 of each half, two neighbouring tokens. With
+// SwiGLU those two rows are a feature's gate and up (rows come 8 gate, 8 up), so the product
+// never leaves the thread. Results go to bf16 rows of tokens by transposing 8 x 8 matrix
+// stores, 16-byte pieces swizzled by the token so that neither side meets a bank twice, and
+// leave as 16 bytes for a thread. (Staging fp32 by feature took 4 times the shared-memory
+// passes: 8192 x 6144 x 2048 over 32 experts FIGS us against FIGS.) fp32 output is written
+// straight from the fragments, 32 bytes of a row by eight lanes.
+template <int NI>
+FUS_DEVICE void read_chunk(uint32_t taddr, uint32_t* v) {
+  if (NI == 4) {
+    tmem_ld_16x32_issue(taddr, v);
+    tmem_ld_16x32_issue(taddr + (16u << 16), v + 16);
+  } else {
+    tmem_ld_16x16_issue(taddr, v);
+    tmem_ld_16x16_issue(taddr + (16u << 16), v + 8);
+  }
+}
+template <int NI>
+FUS_DEVICE void wait_chunk(uint32_t* v) {
+  tmem_ld_wait(v);
+  if (NI == 4) tmem_ld_wait(v + 16);
+}
+
+// the chunk's finished values of one thread, in place: alpha, SwiGLU, the rows' scales rs[]
+// (null: none). SwiGLU leaves them in the gate's places.
+template <bool SWIGLU, int NI>
+FUS_DEVICE void finish_chunk(uint32_t* v, float alpha, const float* rs, int lane) {
 #pragma unroll
-  for (int j0 = 0; j0 < CHUNK; j0 += kGroupThreads / PER) {
+  for (int i = 0; i < NI; ++i) {
+    const float2 sc = rs ? *reinterpret_cast<const float2*>(rs + 8 * i + 2 * (lane & 3))
+                         : make_float2(1.f, 1.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t* r = v + h * 4 * NI + 4 * i;
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(r[j]) * alpha;
+      if (SWIGLU) {
+        x[0] = silu_mul(x[0], x[2]);
+        x[1] = silu_mul(x[1], x[3]);
+      }
+      if (rs) {
+        x[0] *= sc.x;
+        x[1] *= sc.y;
+        x[2] *= sc.x;
+        x[3] *= sc.y;
+      }
+#pragma unroll
+      for (int j = 0; j < (SWIGLU ? 2 : 4); ++j) r[j] = __float_as_uint(x[j]);
+    }
+  }
+}
+
+FUS_DEVICE uint32_t pack_bf(uint32_t lo, uint32_t hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+template <bool SWIGLU, int NI>
+FUS_DEVICE void stage_chunk(const uint32_t* v, uint32_t stage, int q4, int lane) {
+  const int j = lane & 7, mi = lane >> 3;
+  if (SWIGLU) {  // rows of 64 features: matrices (half 0, half 1) of two token blocks
+#pragma unroll
+    for (int i = 0; i < NI; i += 2) {
+      uint32_t m[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t* r = v + (q & 1) * 4 * NI + 4 * (i + (q >> 1));
+        m[q] = pack_bf(r[0], r[1]);
+      }
+      stmatrix_x4_trans(stage + (8 * (i + (mi >> 1)) + j) * 128 + ((q4 * 2 + (mi & 1)) ^ j) * 16, m);
+    }
+  } else {  // rows of 128 features: four matrices of a token block
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      uint32_t m[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t* r = v + (q >> 1) * 4 * NI + 4 * i + 2 * (q & 1);
+        m[q] = pack_bf(r[0], r[1]);
+      }
+      stmatrix_x4_trans(stage + (8 * i + j) * 256 + ((q4 * 4 + mi) ^ j) * 16, m);
+    }
+  }
+}
+
+// staged rows -> output rows (rows[]: -1 none), by the group's 128 threads
+template <bool SWIGLU, int NI>
+FUS_DEVICE void store_chunk(const Fp4Args& a, const uint8_t* stage, const int* rows, int nj, int mt,
+                            int et) {
+  constexpr int PER = SWIGLU ? 8 : 16;  // 16-byte pieces of a row
+  const int q = et % PER;
+  const int col = mt * PER * 8 + q * 8;
+  if (col >= a.out_cols) return;
+#pragma unroll
+  for (int j0 = 0; j0 < 8 * NI; j0 += kGroupThreads / PER) {
     const int j = j0 + et / PER;
-    if (j >= nj || col >= a.out_cols) continue;
+    if (j >= nj) continue;
     const int row = rows[j];
     if (row < 0) continue;
-    float o[8];
-    *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(S + j * 128 + f);
-    *reinterpret_cast<float4*>(o + 4) = *reinterpret_cast<const float4*>(S + j * 128 + f + 4);
-    if (SWIGLU) {
-      float w[8];
-      *reinterpret_cast<float4*>(w) = *reinterpret_cast<const float4*>(S + j * 128 + 64 + f);
-      *reinterpret_cast<float4*>(w + 4) = *reinterpret_cast<const float4*>(S + j * 128 + 68 + f);
+    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (long)row * a.ldo + col) =
+        *reinterpret_cast<const uint4*>(stage + j * PER * 16 + (q ^ (j & 7)) * 16);
+  }
+}
+
+template <bool SWIGLU, int NI>
+FUS_DEVICE void store_chunk_f32(const Fp4Args& a, const uint32_t* v, const int* rows, int nj, int mt,
+                                int q4, int lane) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) o[t] = silu_mul(o[t], w[t]);
-    }
-    if (a.row_scale) {
-      const float rs = __ldg(a.row_scale + row);
+  for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int t = 0; t < 8; ++t) o[t] *= rs;
+    for (int e = 0; e < 2; ++e) {
+      const int j = 8 * i + 2 * (lane & 3) + e;
+      const int row = j < nj ? rows[j] : -1;
+      if (row < 0) continue;
+      float* d = reinterpret_cast<float*>(a.out) + (long)row * a.ldo;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int sub = 0; sub < (SWIGLU ? 1 : 2); ++sub) {
+          const int col = SWIGLU ? mt * 64 + q4 * 16 + h * 8 + (lane >> 2)
+                                 : mt * 128 + q4 * 32 + h * 16 + sub * 8 + (lane >> 2);
+          if (col < a.out_cols) d[col] = __uint_as_float(v[h * 4 * NI + 4 * i + 2 * sub + e]);
+        }
     }
-    if (a.out_f32) {
-      float4* d = reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + (long)row * a.ldo + col);
-      d[0] = make_float4(o[0], o[1], o[2], o[3]);
-      d[1] = make_float4(o[4], o[5], o[6], o[7]);
-    } else {
-      *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (long)row * a.ldo + col) =
-          pack8(o);
-    }
+}
+
+// One chunk of 8 NI token columns whose fragments v are read: `nj` of them are live, with output
+// rows rows[] and scales rs[]. `turn` alternates the two staging buffers, so one barrier of the
+// group is enough: a buffer is written again only after the barrier of the chunk between.
+template <bool SWIGLU, int NI>
+FUS_DEVICE void write_chunk(const Fp4Args& a, uint32_t* v, float alpha, uint8_t* stage, int& turn,
+                            const int* rows, const float* rs, int nj, int mt, int q4, int lane,
+                            int et, int barrier) {
+  finish_chunk<SWIGLU, NI>(v, alpha, a.row_scale ? rs : nullptr, lane);
+  if (a.out_f32) {
+    store_chunk_f32<SWIGLU, NI>(a, v, rows, nj, mt, q4, lane);
+    return;
+  }
+  stage += turn * (8 * NI * 256);
+  turn ^= 1;
+  stage_chunk<SWIGLU, NI>(v, smem_u32(stage), q4, lane);
+  named_bar_sync(barrier, kGroupThreads);
+  store_chunk<SWIGLU, NI>(a, stage, rows, nj, mt, et);
+}
+
+// Row numbers (out of range: -1) and scales of `n` columns from dispatch position `pos0`. The caller's
+// next barrier of the group makes them visible.
+FUS_DEVICE void load_rows(const Fp4Args& a, int pos0, int n, int* rows, float* rs, int et) {
+  for (int j = et; j < n; j += kGroupThreads) {
+    int row = a.scatter ? __ldg(a.live_ids + pos0 + j) : pos0 + j;
+    if (row >= a.out_rows) row = -1;
+    rows[j] = row;
+    if (a.row_scale) rs[j] = row >= 0 ? __ldg(a.row_scale + row) : 0.f;
   }
 }
 
@@ -256,8 +376,9 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       auto load_w = [&](int s, int k) {
         const uint32_t full = bar_full + 8 * s;
         mbar_arrive_expect_tx(full, C::STAGE_BYTES);
-        if (SWIGLU) {  // 64 gate rows, their 64 up rows
-          tma_load_3d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0, pol_w);
+        if (SWIGLU) {  // 8 groups of 8 gate rows and their up rows
+          tma_load_4d(sA + s * C::A_BYTES, &tw, full, k * 128, 0, 0, (e * a.w_rows + mt * 64) / 8,
+                      pol_w);
         } else {
           tma_load_2d(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
         }
@@ -357,43 +478,35 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     }
   } else if (warp >= 4) {
     const int q4 = warp & 3;  // the TMEM lanes this warp may read
-    const int m = q4 * 32 + lane;
     const int et = threadIdx.x - 128;
-    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES);
-    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES + C::CHUNK * 128 * 4);
+    constexpr int NI = C::CHUNK / 8;
+    uint8_t* stage = smem + STAGES * C::STAGE_BYTES;
+    int* s_row = reinterpret_cast<int*>(stage + 2 * C::STAGE_OUT);
+    float* s_rs = reinterpret_cast<float*>(s_row + BN);
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
-    int n = 0;
+    int n = 0, turn = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const int blk = u / a.m_tiles, mt = u - blk * a.m_tiles;
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int live = live_of(blk);
-      // output rows, out of range: -1 (read after the barrier below)
-      for (int j = et; j < live; j += kGroupThreads) {
-        const int pos = blk * BN + j;
-        const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
-        s_row[j] = row < a.out_rows ? row : -1;
-      }
+      // every thread is done with the rows of the unit before
+      named_bar_sync(1, kGroupThreads);
+      load_rows(a, blk * BN, live, s_row, s_rs, et);
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
       const int buf = n % C::ACCS;
-      // one thread of the group waits, the others rest at the barrier: 256 spinning threads
-      // slow the issuing warps down
+      // one thread waits, the others rest at the barrier
       if (et == 0) *group_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
       named_bar_sync(1, kGroupThreads);
       if (!*group_ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(q4 * 32) << 16);
       for (int c0 = 0; c0 < live; c0 += C::CHUNK) {
-        uint32_t v[C::CHUNK];
-#pragma unroll
-        for (int c = 0; c < C::CHUNK; c += 16) tmem_ld16_issue(acc + c0 + c, v + c);
-#pragma unroll
-        for (int c = 0; c < C::CHUNK; c += 16) tmem_ld_wait(v + c);
-#pragma unroll
-        for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[j]) * alpha;
-        named_bar_sync(1, kGroupThreads);
-        store_chunk<SWIGLU, C::CHUNK>(a, S, s_row + c0, min(C::CHUNK, live - c0), mt, et);
-        named_bar_sync(1, kGroupThreads);
+        uint32_t v[8 * NI];
+        read_chunk<NI>(acc + c0, v);
+        wait_chunk<NI>(v);
+        write_chunk<SWIGLU, NI>(a, v, alpha, stage, turn, s_row + c0, s_rs + c0, live - c0, mt, q4,
+                                lane, et, 1);
       }
       tc_fence_before();
       __syncwarp();
@@ -527,10 +640,17 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   CUtensorMap tw;
   TokenMaps tx;
   const uint64_t row = (uint64_t)d->K / 2, rows = (uint64_t)d->n_experts * d->w_rows;
-  const uint64_t half = (uint64_t)d->w_rows / 2;
-  // SwiGLU: two planes, the gate rows and the up rows of the stack
-  int rc = sw ? make_tmap_u8_3d(&tw, d->wq, row, rows - half, row, 2, half * row, 128, 64, 2)
-              : make_tmap_u8_2d(&tw, d->wq, row, rows, row, 128, 128);
+  int rc;
+  if (sw) {
+    // tiles of 8 gate rows, their 8 up rows, the next 8, ...: (bytes, row of 8, half, group)
+    const uint64_t half = (uint64_t)d->w_rows / 2;
+    const uint64_t dims[4] = {row, 8, 2, (rows - half) / 8};
+    const uint64_t strides[3] = {row, half * row, 8 * row};
+    const uint32_t box[4] = {128, 8, 2, 8};
+    rc = make_tmap_u8(&tw, d->wq, 4, dims, strides, box);
+  } else {
+    rc = make_tmap_u8_2d(&tw, d->wq, row, rows, row, 128, 128);
+  }
   for (int i = 0; i < 4 && !rc; ++i)
     rc = make_tmap_u8_2d(&tx.m[i], d->xq, row, (uint64_t)d->x_rows, (uint64_t)d->ldxq, 128,
                          d->block_n <= 64 ? d->block_n : 32 * (i + 1));

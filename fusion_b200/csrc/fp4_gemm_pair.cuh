@@ -31,7 +31,8 @@ struct PairCfg {
   static constexpr int COLS_THREAD = BN / GROUPS;  // accumulator columns of a thread
   static constexpr int CHUNK = 32;
   static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
-  static constexpr int EPI_BYTES = GROUPS * (CHUNK * 128 * 4 + BN * 4);
+  static constexpr int STAGE_OUT = CHUNK * 256;  // staged bf16 rows of a group, two buffers
+  static constexpr int EPI_BYTES = GROUPS * (2 * STAGE_OUT + COLS_THREAD * 8);
   static constexpr int FIT = (226 * 1024 - EPI_BYTES - 1280) / STAGE_BYTES;
   static constexpr int STAGES = FIT > 7 ? 7 : FIT;
   static constexpr int ACCS = 256 / BN;  // accumulators
@@ -174,8 +175,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
         const uint32_t full = cluster_map(bar_full + 8 * s, 0);
         if (leader) mbar_arrive_expect_tx(bar_full + 8 * s, bytes);
         if (SWIGLU) {
-          tma_load_3d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 64, 0,
-                           pol_w);
+          tma_load_4d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, 0, 0,
+                           (e * a.w_rows + mt * 64) / 8, pol_w);
         } else {
           tma_load_2d_pair(sA + s * C::A_BYTES, &tw, full, k * 128, e * a.w_rows + mt * 128, pol_w);
         }
@@ -286,53 +287,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
     // ---- epilogue (both CTAs): each group has half of the columns ----
     const int q4 = warp & 3;
     const int grp = (warp - 4) >> 2;
-    const int m = q4 * 32 + lane;
     const int et = threadIdx.x - 128 - grp * kGroupThreads;
-    float* S = reinterpret_cast<float*>(smem + STAGES * C::STAGE_BYTES) + grp * C::CHUNK * 128;
-    int* s_row = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES +
-                                        C::GROUPS * C::CHUNK * 128 * 4) + grp * BN;
+    constexpr int NI = C::CHUNK / 8, NCH = C::COLS_THREAD / C::CHUNK;
+    uint8_t* stage = smem + STAGES * C::STAGE_BYTES + grp * (2 * C::STAGE_OUT + C::COLS_THREAD * 8);
+    int* s_row = reinterpret_cast<int*>(stage + 2 * C::STAGE_OUT);
+    float* s_rs = reinterpret_cast<float*>(s_row + C::COLS_THREAD);
     volatile int* my_ok = group_ok + grp;
     const float gx = a.xg ? __ldg(a.xg) : 1.0f;
-    int n = 0;
+    int n = 0, turn = 0;
     for (int u = first; u < units; u += stride) {
       const int blk = u / m_pairs, mt = (u - blk * m_pairs) * 2 + rank;
       const int e = expert_of(blk);
       if (e < 0) continue;
       const int live = live_of(blk) - grp * C::COLS_THREAD;  // of this group's columns
       const int buf = n % C::ACCS;
-      for (int j = et; j < min(live, C::COLS_THREAD); j += kGroupThreads) {
-        const int pos = blk * BN + grp * C::COLS_THREAD + j;
-        const int row = a.scatter ? __ldg(a.live_ids + pos) : pos;
-        s_row[j] = row < a.out_rows ? row : -1;
-      }
+      // every thread is done with the rows of the unit before
+      named_bar_sync(1 + grp, kGroupThreads);
+      load_rows(a, blk * BN + grp * C::COLS_THREAD, min(live, C::COLS_THREAD), s_row, s_rs, et);
       const float alpha = (a.wg ? __ldg(a.wg + e) : 1.0f) * gx;
-      // one thread of the group waits, the others rest at the barrier: 256 spinning threads
-      // slow the issuing warps down
+      // one thread of the group waits, the others rest at the barrier
       if (et == 0) *my_ok = mbar_wait_bounded(bar_acc + 8 * buf, (n / C::ACCS) & 1, abort_flag, a.status);
       named_bar_sync(1 + grp, kGroupThreads);
       if (!*my_ok) break;
       tc_fence_after();
-      uint32_t v[C::COLS_THREAD];
+      uint32_t v[NCH][8 * NI];
       const uint32_t acc = tmem + buf * BN + grp * C::COLS_THREAD + ((uint32_t)(q4 * 32) << 16);
 #pragma unroll
-      for (int c = 0; c < C::COLS_THREAD; c += 16)
-        if (c < live) tmem_ld16_issue(acc + c, v + c);
+      for (int c = 0; c < NCH; ++c)
+        if (c * C::CHUNK < live) read_chunk<NI>(acc + c * C::CHUNK, v[c]);
 #pragma unroll
-      for (int c = 0; c < C::COLS_THREAD; c += 16)
-        if (c < live) tmem_ld_wait(v + c);
+      for (int c = 0; c < NCH; ++c)
+        if (c * C::CHUNK < live) wait_chunk<NI>(v[c]);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(cluster_map(bar_free + 8 * buf, 0));
       ++n;
 #pragma unroll
-      for (int c0 = 0; c0 < C::COLS_THREAD; c0 += C::CHUNK) {
-        if (c0 >= live) break;
-#pragma unroll
-        for (int j = 0; j < C::CHUNK; ++j) S[j * 128 + m] = __uint_as_float(v[c0 + j]) * alpha;
-        named_bar_sync(1 + grp, kGroupThreads);
-        store_chunk<SWIGLU, C::CHUNK>(a, S, s_row + c0, min(C::CHUNK, live - c0), mt, et);
-        named_bar_sync(1 + grp, kGroupThreads);
-      }
+      for (int c = 0; c < NCH; ++c)
+        if (c * C::CHUNK < live)
+          write_chunk<SWIGLU, NI>(a, v[c], alpha, stage, turn, s_row + c * C::CHUNK,
+                                  s_rs + c * C::CHUNK, live - c * C::CHUNK, mt, q4, lane, et,
+                                  1 + grp);
     }
   }
   // neither CTA leaves (or frees the pair's TMEM) while the other may still signal its

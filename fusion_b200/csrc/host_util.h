@@ -19,14 +19,13 @@ int check_launch(const char* what);
 // row, `rows` rows, row pitch `ld` elements, box = box_inner x box_rows.
 int make_tmap_bf16_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
                       uint32_t box_inner, uint32_t box_rows);
-// Same for rows of bytes (packed 4-bit operands and, without swizzle, their scales): `inner`
-// bytes, row pitch `ld` bytes
+// Same for bytes (packed 4-bit operands and, without swizzle, their scales), of any rank: dims from
+// the contiguous one, strides in bytes from the second
+int make_tmap_u8(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
+                 const uint64_t* strides, const uint32_t* box, bool swizzle = true);
+// rows of `inner` bytes, row pitch `ld` bytes
 int make_tmap_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
                     uint32_t box_inner, uint32_t box_rows, bool swizzle = true);
-// ... of `planes` (> 1) such matrices, plane_ld bytes apart, in a box of box_planes
-int make_tmap_u8_3d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t ld,
-                    uint64_t planes, uint64_t plane_ld, uint32_t box_inner, uint32_t box_rows,
-                    uint32_t box_planes, bool swizzle = true);
 // row-major output tile map for TMA stores (no swizzle: the staging tile is row-major)
 int make_tmap_store_2d(CUtensorMap* m, const void* base, bool f32, uint64_t inner, uint64_t rows,
                        uint64_t ld, uint32_t box_inner, uint32_t box_rows);
