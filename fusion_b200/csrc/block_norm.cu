@@ -23,7 +23,14 @@ struct NormArgs {
 
 FUS_DEVICE float gate_act(float g, int act) {
   if (act == FUS_GATE_SIGMOID) return __fdividef(1.0f, 1.0f + __expf(-g));
-  if (act == FUS_GATE_TANH) return tanhf(g);
+  if (act == FUS_GATE_TANH) {
+    // 1 - 2 / (1 + e^2g), and near zero, where that cancels, the series (its next term is below
+    // 4e-7 of the value at 1/4)
+    const float e = 1.0f - __fdividef(2.0f, 1.0f + __expf(2.0f * g));
+    const float q = g * g;
+    const float near = g + g * q * (-1.0f / 3 + q * (2.0f / 15 + q * (-17.0f / 315)));
+    return fabsf(g) < 0.25f ? near : e;
+  }
   return g;
 }
 
@@ -63,6 +70,26 @@ FUS_DEVICE void load_v(const T* p, int i0, int N, bool whole, float* f) {
     for (int j = 0; j < V; ++j) f[j] = i0 + j >= 0 && i0 + j < N ? to_f(p[i0 + j]) : 0.f;
   }
 }
+// V elements that start `skip` elements (1 .. V - 1) into the line a, and go on in the line b
+template <typename T, int V>
+FUS_DEVICE uint4 shift_lines(const uint4& a, const uint4& b, int skip) {
+  uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int bytes = skip * (int)sizeof(T);
+  if (bytes & 8) {
+#pragma unroll
+    for (int j = 0; j < 6; ++j) r[j] = r[j + 2];
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) r[j] = r[j + 1];
+  }
+  if (bytes & 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __funnelshift_r(r[j], r[j + 1], 16);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // The same for the weights, which every row reads (kept in L1). They start on 16 bytes but
 // the row does not: element i0 is `off` short of a 16-byte line, so two lines are read and
 // shifted together.
@@ -72,22 +99,7 @@ FUS_DEVICE void load_w(const T* p, int i0, int N, bool whole, int off, float* f)
     unpack_v<T, V>(__ldg(reinterpret_cast<const uint4*>(p + i0)), f);
   } else if (whole && i0 + off + V <= N) {
     const uint4* line = reinterpret_cast<const uint4*>(p + i0 + off - V);
-    const uint4 a = __ldg(line), b = __ldg(line + 1);
-    uint32_t r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    const int bytes = (V - off) * (int)sizeof(T);  // 2 .. 14, a multiple of sizeof(T)
-    if (bytes & 8) {
-#pragma unroll
-      for (int j = 0; j < 6; ++j) r[j] = r[j + 2];
-    }
-    if (bytes & 4) {
-#pragma unroll
-      for (int j = 0; j < 5; ++j) r[j] = r[j + 1];
-    }
-    if (bytes & 2) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = __funnelshift_r(r[j], r[j + 1], 16);
-    }
-    unpack_v<T, V>(make_uint4(r[0], r[1], r[2], r[3]), f);
+    unpack_v<T, V>(shift_lines<T, V>(__ldg(line), __ldg(line + 1), V - off), f);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = i0 + j >= 0 && i0 + j < N ? to_f(p[i0 + j]) : 0.f;
@@ -105,7 +117,7 @@ FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, const float* f) {
 }
 
 // One CTA for a row, VPT 16-byte vectors for a thread. MODE 0: every row of every tensor starts
-// on 16 bytes. 1: rows start anywhere, but alike in all row tensors (odd widths): vectors
+// on 16 bytes, the weights too. 1: the weights do, rows start anywhere, but alike in all row tensors (odd widths): vectors
 // follow the 16-byte lines of memory, the ones at the ends go by element. 2: by element.
 template <typename T, int VPT, int MODE>
 __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs a) {
@@ -186,37 +198,61 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
 }
 
 // Many rows: persistent CTAs, each with a ring of rows that bulk copies fill ahead of the
-// arithmetic, so that loads never wait for a row's two sums and barriers. The weights (and a
-// channel gate) stay in registers over all rows.
+// arithmetic, so that loads never wait for a row's two sums and barriers. Aligned rows keep the
+// weights (and a channel gate) in registers over all rows. SHIFT: rows start anywhere, but alike
+// in all row tensors (odd widths); the 16-byte lines that hold a row are copied, its vectors
+// are those lines, and the weights wait in shared memory, two lines shifted together for a vector.
+// What lines hold beside the row is its neighbours', never used; the first row's first line
+// and the last row's last are not copied where they reach past the tensor: those few elements
+// are loaded one by one.
 constexpr int kRingThreads = 256;
+constexpr int kRingRows = 4 * 148;
 
-template <typename T, int VPT, bool FULL>
+template <typename T, int VPT, bool FULL, bool SHIFT>
 __global__ void __launch_bounds__(kRingThreads, 2)
     norm_gate_residual_ring_kernel(const NormArgs a, int rows, int stages, int* status) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float red[2][32];
   __shared__ uint64_t bars[8];
   __shared__ volatile int abort_flag;
-  extern __shared__ uint8_t ring[];  // stages x (y row | res row | gate row)
-  const int N = a.N, nv = N / V;
-  const uint32_t row_bytes = (uint32_t)N * sizeof(T);
+  extern __shared__ __align__(16) uint8_t ring[];  // SHIFT: weights; stages x (y | res | gate)
+  const int N = a.N;
+  const int lines = (N + V - 1) / V + (SHIFT ? 1 : 0);  // at most, of a row
+  const uint32_t row_bytes = (uint32_t)lines * 16;
   const uint32_t stage_bytes = row_bytes * (FULL ? 3 : 2);
   const uint32_t bar = smem_u32(bars);
+  // SHIFT: post | pre | channel gate, each a line of zeros, the weights, two lines of zeros
+  const int w_lines = lines + 2;
+  uint4* s_w = reinterpret_cast<uint4*>(ring);
+  uint8_t* stage0 = ring + (SHIFT ? 3 * w_lines * 16 : 0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) mbar_init(bar + 8 * s, 1);
     abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
+  // elements of a row's first line before the row
+  auto offset_of = [&](long t) {
+    return SHIFT ? (int)((reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(a.y) + t * a.ldy) & 15) /
+                         sizeof(T))
+                 : 0;
+  };
   auto load_row = [&](long t, int s) {
     const uint64_t pol = policy_evict_first();
-    const uint32_t dst = smem_u32(ring) + s * stage_bytes;
-    mbar_arrive_expect_tx(bar + 8 * s, stage_bytes);
-    bulk_load(dst, reinterpret_cast<const T*>(a.y) + t * a.ldy, row_bytes, bar + 8 * s, pol);
-    bulk_load(dst + row_bytes, reinterpret_cast<const T*>(a.res) + t * a.ldr, row_bytes,
+    const int off = offset_of(t);
+    int l0 = 0, l1 = (N + off + V - 1) / V;  // lines copied
+    if (SHIFT && t == 0 && off > 0) l0 = 1;
+    if (SHIFT && t == rows - 1) l1 = (N + off) / V;
+    const uint32_t bytes = l1 > l0 ? (uint32_t)(l1 - l0) * 16 : 0;
+    const uint32_t dst = smem_u32(stage0) + s * stage_bytes + l0 * 16;
+    const int from = l0 * V - off;
+    mbar_arrive_expect_tx(bar + 8 * s, bytes * (FULL ? 3 : 2));
+    if (bytes == 0) return;
+    bulk_load(dst, reinterpret_cast<const T*>(a.y) + t * a.ldy + from, bytes, bar + 8 * s, pol);
+    bulk_load(dst + row_bytes, reinterpret_cast<const T*>(a.res) + t * a.ldr + from, bytes,
               bar + 8 * s, pol);
     if (FULL)
-      bulk_load(dst + 2 * row_bytes, reinterpret_cast<const T*>(a.gate) + t * a.ldg, row_bytes,
+      bulk_load(dst + 2 * row_bytes, reinterpret_cast<const T*>(a.gate) + t * a.ldg + from, bytes,
                 bar + 8 * s, pol);
   };
   if (threadIdx.x == 0)
@@ -224,39 +260,89 @@ __global__ void __launch_bounds__(kRingThreads, 2)
       const long t = blockIdx.x + (long)s * gridDim.x;
       if (t < rows) load_row(t, s);
     }
-  uint4 post[VPT], pre[VPT], gch[VPT];
+  uint4 keep[SHIFT ? 1 : 3][VPT];  // post, pre, channel gate
+  const T* src[3] = {reinterpret_cast<const T*>(a.post_w), reinterpret_cast<const T*>(a.pre_w),
+                     a.gate_kind == 2 ? reinterpret_cast<const T*>(a.gate) : nullptr};
+  if (SHIFT) {
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    const int i = threadIdx.x + v * kRingThreads;
-    post[v] = pre[v] = gch[v] = make_uint4(0, 0, 0, 0);
-    if (i < nv) {
-      if (a.post_w) post[v] = __ldg(reinterpret_cast<const uint4*>(a.post_w) + i);
-      if (a.pre_w) pre[v] = __ldg(reinterpret_cast<const uint4*>(a.pre_w) + i);
-      if (a.gate_kind == 2) gch[v] = __ldg(reinterpret_cast<const uint4*>(a.gate) + i);
+    for (int w = 0; w < 3; ++w) {
+      if (!src[w]) continue;
+      uint4* d = s_w + w * w_lines;
+      for (int i = threadIdx.x; i < w_lines; i += kRingThreads) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        const int i0 = (i - 1) * V;  // weights of the line
+        if (i0 >= 0 && i0 + V <= N) {
+          u = __ldg(reinterpret_cast<const uint4*>(src[w] + i0));
+        } else if (i0 >= 0) {
+          T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+          for (int j = 0; j < V; ++j) e[j] = i0 + j < N ? src[w][i0 + j] : from_f<T>(0.f);
+        }
+        d[i] = u;
+      }
     }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int i = threadIdx.x + v * kRingThreads;
+        keep[SHIFT ? 0 : w][v] = src[w] && i < lines ? __ldg(reinterpret_cast<const uint4*>(src[w]) + i)
+                                                     : make_uint4(0, 0, 0, 0);
+      }
   }
   int n = 0;
   for (long t = blockIdx.x; t < rows; t += gridDim.x, ++n) {
     const int s = n % stages;
+    const int off = offset_of(t);
     float scale = a.alpha;
     if (a.gate_kind == 1)
       scale *= gate_act(to_f(reinterpret_cast<const T*>(a.gate)[t * a.ldg]), a.act);
     if (!mbar_wait_bounded(bar + 8 * s, (n / stages) & 1, &abort_flag, status)) break;
-    const uint4* sy = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
-    const uint4* sr = sy + nv;
-    const uint4* sg = sr + nv;
+    const uint4* sy = reinterpret_cast<const uint4*>(stage0 + s * stage_bytes);
+    const uint4* sr = sy + lines;
+    const uint4* sg = sr + lines;
+    auto whole = [&](int i) { return !SHIFT || (i >= 0 && i + V <= N); };  // elements i .. i + V
+    // weights of the vector of line i
+    auto weight = [&](int w, int v, int i, float* f) {
+      if (!SHIFT) {
+        unpack_v<T, V>(keep[SHIFT ? 0 : w][v], f);
+      } else {
+        const uint4* p = s_w + w * w_lines + i;  // lines start one of zeros earlier
+        unpack_v<T, V>(off ? shift_lines<T, V>(p[0], p[1], V - off) : p[1], f);
+      }
+    };
     float f[VPT][V];
     uint4 r[VPT], g[VPT];
     float ss = 0.f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = threadIdx.x + v * kRingThreads;
+      const int i0 = i * V - off;
       uint4 u = make_uint4(0, 0, 0, 0);
       r[v] = g[v] = u;
-      if (i < nv) {
+      if (i0 < N) {
         u = sy[i];
         r[v] = sr[i];
         if (FULL) g[v] = sg[i];
+        if (SHIFT && !whole(i0)) {
+          // an end of the row: zeros outside it, and what was not copied (see above)
+          const bool load = (i0 < 0 && t == 0) || (i0 + V > N && t == rows - 1);
+          T* e = reinterpret_cast<T*>(&u);
+          T* er = reinterpret_cast<T*>(&r[v]);
+          T* eg = reinterpret_cast<T*>(&g[v]);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            if (i0 + j < 0 || i0 + j >= N) {
+              e[j] = er[j] = eg[j] = from_f<T>(0.f);
+            } else if (load) {
+              e[j] = (reinterpret_cast<const T*>(a.y) + t * a.ldy)[i0 + j];
+              er[j] = (reinterpret_cast<const T*>(a.res) + t * a.ldr)[i0 + j];
+              if (FULL) eg[j] = (reinterpret_cast<const T*>(a.gate) + t * a.ldg)[i0 + j];
+            }
+          }
+        }
       }
       unpack_v<T, V>(u, f[v]);
 #pragma unroll
@@ -273,14 +359,19 @@ __global__ void __launch_bounds__(kRingThreads, 2)
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = threadIdx.x + v * kRingThreads;
+      const int i0 = i * V - off;
+      if (i0 >= N) continue;
       float w[V];
       if (a.post_w) {
-        unpack_v<T, V>(post[v], w);
+        weight(0, v, i, w);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[v][j] *= w[j];
       }
       if (FULL || a.gate_kind == 2) {
-        unpack_v<T, V>(FULL ? g[v] : gch[v], w);
+        if (FULL)
+          unpack_v<T, V>(g[v], w);
+        else
+          weight(2, v, i, w);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[v][j] *= gate_act(w[j], a.act);
       }
@@ -290,7 +381,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         f[v][j] = w[j] + scale * f[v][j];
         sh += f[v][j] * f[v][j];
       }
-      if (i < nv) reinterpret_cast<uint4*>(h)[i] = pack_v<T, V>(f[v]);
+      store_v<T, V>(h, i0, N, whole(i0), f[v]);
     }
     if (!a.x) continue;
     sh = cta_sum(sh, red[1]);
@@ -299,24 +390,35 @@ __global__ void __launch_bounds__(kRingThreads, 2)
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       const int i = threadIdx.x + v * kRingThreads;
+      const int i0 = i * V - off;
+      if (i0 >= N) continue;
       float w[V];
-      unpack_v<T, V>(pre[v], w);
+      weight(1, v, i, w);
 #pragma unroll
       for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
-      if (i < nv) reinterpret_cast<uint4*>(x)[i] = pack_v<T, V>(w);
+      store_v<T, V>(x, i0, N, whole(i0), w);
     }
   }
 }
 
-template <typename T, int VPT, bool FULL>
-int launch_ring(const NormArgs& a, int rows, int stages, cudaStream_t st, int* status) {
-  auto fn = norm_gate_residual_ring_kernel<T, VPT, FULL>;
-  const int bytes = stages * (FULL ? 3 : 2) * a.N * (int)sizeof(T);
+template <typename T, int VPT, bool FULL, bool SHIFT>
+int launch_ring(const NormArgs& a, int rows, int stages, int bytes, cudaStream_t st, int* status) {
+  auto fn = norm_gate_residual_ring_kernel<T, VPT, FULL, SHIFT>;
   // the limit is set once, to what two CTAs of an SM may have
   if (int rc = ensure_smem_attr((const void*)fn, 110 * 1024, "norm_gate_residual")) return rc;
   const int grid = 2 * num_sms();
   fn<<<grid < rows ? grid : rows, kRingThreads, bytes, st>>>(a, rows, stages, status);
   return check_launch("norm_gate_residual");
+}
+
+template <typename T, int VPT>
+int launch_ring_of(const NormArgs& a, int rows, int stages, int bytes, bool shift, cudaStream_t st,
+                   int* status) {
+  if (a.gate_kind == 3)
+    return shift ? launch_ring<T, VPT, true, true>(a, rows, stages, bytes, st, status)
+                 : launch_ring<T, VPT, true, false>(a, rows, stages, bytes, st, status);
+  return shift ? launch_ring<T, VPT, false, true>(a, rows, stages, bytes, st, status)
+               : launch_ring<T, VPT, false, false>(a, rows, stages, bytes, st, status);
 }
 
 template <typename T, int VPT>
@@ -332,7 +434,7 @@ void launch_mode(const NormArgs& a, int T_, int threads, int mode, cudaStream_t 
 template <typename T>
 int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
   constexpr int V = 16 / sizeof(T);
-  // alignment of the row tensors: mode 0 wants all on 16 bytes (weights too), mode 1 alike
+  // alignment of the row tensors: mode 0 wants all on 16 bytes, mode 1 alike (the weights always)
   const void* rowp[5] = {a.y, a.res, a.h, a.x, a.gate_kind == 3 ? a.gate : nullptr};
   const long rowl[5] = {a.ldy, a.ldr, a.ldh, a.ldx, a.ldg};
   bool on16 = true, alike = true;
@@ -343,26 +445,28 @@ int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
             (rowl[i] - a.ldy) % V == 0;
   }
   const void* wp[3] = {a.post_w, a.pre_w, a.gate_kind == 2 ? a.gate : nullptr};
-  for (const void* p : wp) on16 = on16 && (!p || aligned16(p));
-  const int mode = on16 ? 0 : alike ? 1 : 2;
+  bool w16 = true;
+  for (const void* p : wp) w16 = w16 && (!p || aligned16(p));
+  const int mode = !w16 ? 2 : on16 ? 0 : alike ? 1 : 2;
   const int nv = (a.N + V - 1) / V + (mode == 1 ? 1 : 0);
-  const bool full = a.gate_kind == 3;
-  // the ring wants whole aligned rows, some rows for each CTA and two stages at least
-  if (mode == 0 && a.N % V == 0 && rows >= 4 * 148 && nv > kRingThreads / 2 &&
-      nv <= 3 * kRingThreads) {
-    int stages = 108 * 1024 / ((full ? 3 : 2) * a.N * (int)sizeof(T));
+  // the ring: some rows for each CTA, most of its threads busy, two stages at least
+  const bool shift = mode != 0 || a.N % V != 0;
+  const int lines = (a.N + V - 1) / V + (shift ? 1 : 0);
+  if (mode < 2 && rows >= kRingRows && lines > kRingThreads / 2 && lines <= 3 * kRingThreads) {
+    const int fixed = shift ? 3 * (lines + 2) * 16 : 0;
+    const int stage = lines * 16 * (a.gate_kind == 3 ? 3 : 2);
+    int stages = (108 * 1024 - fixed) / stage;
     if (stages > 8) stages = 8;
     if (stages >= 2) {
-      const int vpt = (nv + kRingThreads - 1) / kRingThreads;
-#define FUS_RING(P) \
-  (full ? launch_ring<T, P, true>(a, rows, stages, st, status) \
-        : launch_ring<T, P, false>(a, rows, stages, st, status))
-      return vpt == 1 ? FUS_RING(1) : vpt == 2 ? FUS_RING(2) : FUS_RING(3);
-#undef FUS_RING
+      const int bytes = fixed + stages * stage;
+      const int vpt = (lines + kRingThreads - 1) / kRingThreads;
+      return vpt == 1   ? launch_ring_of<T, 1>(a, rows, stages, bytes, shift, st, status)
+             : vpt == 2 ? launch_ring_of<T, 2>(a, rows, stages, bytes, shift, st, status)
+                        : launch_ring_of<T, 3>(a, rows, stages, bytes, shift, st, status);
     }
   }
-  // few rows: as many threads as there are vectors (latency); many: four vectors for each
-  int vpt = rows <= 2 * 148 ? 1 : 4;
+  // few rows: as many threads as there are vectors (latency); many: two vectors for each
+  int vpt = rows <= 2 * 148 ? 1 : 2;
   while (vpt > 1 && nv < 32 * vpt) vpt >>= 1;
   while ((nv + vpt - 1) / vpt > 1024) vpt <<= 1;
   const int threads = ((nv + vpt - 1) / vpt + 31) / 32 * 32;

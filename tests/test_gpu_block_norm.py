@@ -58,6 +58,50 @@ def test_matches_formula(dtype, kind, act, T, N):
            np.sqrt((wh * wh).mean(1, keepdims=True) + 1e-5), dt, N)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("kind,act", [("none", "none"), ("token", "tanh"), ("channel", "tanh"),
+                                      ("full", "sigmoid")])
+@pytest.mark.parametrize("T,N", [(600, 6144), (593, 1536), (1200, 2048), (601, 5003), (900, 2049), (592, 1035),
+                                 (700, 3071)])
+def test_many_rows(dtype, kind, act, T, N):
+    """Batches that go through the ring of rows, whole 16-byte lines and odd widths."""
+    dt = DTYPES[dtype]
+    y, res, post_w, pre_w, gate = _make(T, N, dt, kind)
+    h, x = torch.empty_like(y), torch.empty_like(y)
+    ops.norm_gate_residual(y, res, h, x, post_w=post_w, pre_w=pre_w, gate=gate, gate_act=act, alpha=0.37, eps=1e-5)
+    h1 = torch.empty_like(y)
+    ops.norm_gate_residual(y, res, h1, gate=gate, gate_act=act, alpha=0.37)
+    r2, y2 = res.clone(), y.clone()  # in place
+    ops.norm_gate_residual(y2, r2, r2, y2, post_w=post_w, pre_w=pre_w, gate=gate, gate_act=act, alpha=0.37, eps=1e-5)
+    finish()
+    wh, wx, mag = _oracle(y, res, post_w, pre_w, gate, act, np.float32(0.37), np.float32(1e-5))
+    _check(h, wh, mag, dt, N)
+    _check(x, wx, np.abs(wx) + mag * np.abs(pre_w.double().cpu().numpy()) /
+           np.sqrt((wh * wh).mean(1, keepdims=True) + 1e-5), dt, N)
+    wh1, _, mag1 = _oracle(y, res, None, None, gate, act, np.float32(0.37), np.float32(1e-5))
+    _check(h1, wh1, mag1, dt, N)
+    assert torch.equal(r2, h) and torch.equal(y2, x)
+
+
+def test_many_rows_apart():
+    """Strided rows through the ring: what lies between them is neither read nor written."""
+    T, N, ld = 640, 1501, 1533
+    for off in (0, 3, 8):
+        y0, res0, post_w, pre_w, gate0 = _make(T, N, torch.bfloat16, "full")
+        bufs = [torch.full((off + (T - 1) * ld + N,), float("nan"), dtype=torch.bfloat16, device="cuda")
+                for _ in range(5)]
+        y, res, h, x, gate = (b[off:].as_strided((T, N), (ld, 1)) for b in bufs)
+        y.copy_(y0), res.copy_(res0), gate.copy_(gate0)
+        h.fill_(7.0), x.fill_(7.0)
+        ops.norm_gate_residual(y, res, h, x, post_w=post_w, pre_w=pre_w, gate=gate, gate_act="sigmoid")
+        finish()
+        wh, wx, mag = _oracle(y0, res0, post_w, pre_w, gate0, "sigmoid", 1.0, np.float32(1e-5))
+        _check(h, wh, mag, torch.bfloat16, N)
+        _check(x, wx, np.abs(wx) + mag, torch.bfloat16, N)
+        for b in (bufs[2], bufs[3]):
+            assert int(torch.isnan(b).sum()) == b.numel() - T * N
+
+
 def test_widest_rows():
     for dt, N in ((torch.bfloat16, 32768), (torch.float32, 16384)):
         y, res, post_w, pre_w, _ = _make(2, N, dt, "none")
@@ -104,6 +148,21 @@ def test_strides_and_alignments(off, ld):
         hole = torch.ones(b.numel(), dtype=torch.bool, device="cuda")
         hole[o:].as_strided((T, N), (ld, 1)).fill_(False)
         assert (b[hole] == 5.0).all()
+
+
+@pytest.mark.parametrize("T", [7, 700])
+@pytest.mark.parametrize("off", [1, 4])
+def test_weights_anywhere(T, off):
+    """Norm weights and a channel gate that do not start on 16 bytes."""
+    for N in (1200, 1203):
+        y, res, post_w, pre_w, gate = _make(T, N, torch.bfloat16, "channel")
+        post_w, pre_w, gate = (torch.cat([t.reshape(-1)[:1].expand(off), t.reshape(-1)])[off:] for t in (post_w, pre_w, gate))
+        h, x = torch.empty_like(y), torch.empty_like(y)
+        ops.norm_gate_residual(y, res, h, x, post_w=post_w, pre_w=pre_w, gate=gate, gate_act="sigmoid")
+        finish()
+        wh, wx, mag = _oracle(y, res, post_w, pre_w, gate, "sigmoid", 1.0, np.float32(1e-5))
+        _check(h, wh, mag, torch.bfloat16, N)
+        _check(x, wx, np.abs(wx) + mag, torch.bfloat16, N)
 
 
 def test_in_place():
