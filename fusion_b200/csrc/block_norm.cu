@@ -198,56 +198,51 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
 }
 
 // Many rows: persistent CTAs, each with a ring of rows that bulk copies fill ahead of the
-// arithmetic, so that loads never wait for a row's two sums and barriers. Aligned rows keep the
-// weights (and a channel gate) in registers over all rows. SHIFT: rows start anywhere, but alike
-// in all row tensors (odd widths); the 16-byte lines that hold a row are copied, its vectors
-// are those lines, and the weights wait in shared memory, two lines shifted together for a vector.
-// What lines hold beside the row is its neighbours', never used; the first row's first line
-// and the last row's last are not copied where they reach past the tensor: those few elements
-// are loaded one by one.
-constexpr int kRingThreads = 256;
+// arithmetic, so that loads never wait for a row's two sums and barriers. The weights (and a
+// channel gate) stay in registers over all rows. A row is up to three 16-byte lines for a thread;
+// narrow rows get small CTAs, more of them on an SM, so that more rows are under way at once
+// (a row's chain of barriers takes about a microsecond whatever its width).
+// SHIFT: rows start anywhere, but alike in all row tensors (odd widths). The lines that hold a row
+// are copied and its vectors are those lines; as the grid is a multiple of 8, all rows of a CTA
+// start alike and the weights are shifted once. What lines hold beside the row is its
+// neighbours', never used; the first row's first line and the last row's last are not copied
+// where they reach past the tensor: those few elements are loaded one by one.
 constexpr int kRingRows = 4 * 148;
+constexpr int kRingLines = 192;  // narrower rows (1101 fp16 by 2443: 11 us) lose here (15 us)
+constexpr int kRingThreads = 256;  // at most
 
-template <typename T, int VPT, bool FULL, bool SHIFT>
+template <typename T, bool FULL, bool SHIFT>
 __global__ void __launch_bounds__(kRingThreads, 2)
     norm_gate_residual_ring_kernel(const NormArgs a, int rows, int stages, int* status) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), VPT = 3;
   __shared__ float red[2][32];
   __shared__ uint64_t bars[8];
   __shared__ volatile int abort_flag;
-  extern __shared__ __align__(16) uint8_t ring[];  // SHIFT: weights; stages x (y | res | gate)
-  const int N = a.N;
+  extern __shared__ __align__(16) uint8_t ring[];  // stages x (y | res | gate)
+  const int N = a.N, nt = blockDim.x;
   const int lines = (N + V - 1) / V + (SHIFT ? 1 : 0);  // at most, of a row
   const uint32_t row_bytes = (uint32_t)lines * 16;
   const uint32_t stage_bytes = row_bytes * (FULL ? 3 : 2);
   const uint32_t bar = smem_u32(bars);
-  // SHIFT: post | pre | channel gate, each a line of zeros, the weights, two lines of zeros
-  const int w_lines = lines + 2;
-  uint4* s_w = reinterpret_cast<uint4*>(ring);
-  uint8_t* stage0 = ring + (SHIFT ? 3 * w_lines * 16 : 0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) mbar_init(bar + 8 * s, 1);
     abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  // elements of a row's first line before the row
-  auto offset_of = [&](long t) {
-    return SHIFT ? (int)((reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(a.y) + t * a.ldy) & 15) /
-                         sizeof(T))
-                 : 0;
-  };
+  // elements of a row's first line before the row, the same for all of this CTA's rows
+  const int off = SHIFT ? (int)((reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(a.y) +
+                                                             blockIdx.x * a.ldy) & 15) / sizeof(T))
+                        : 0;
+  const int row_lines = (N + off + V - 1) / V;
   auto load_row = [&](long t, int s) {
     const uint64_t pol = policy_evict_first();
-    const int off = offset_of(t);
-    int l0 = 0, l1 = (N + off + V - 1) / V;  // lines copied
-    if (SHIFT && t == 0 && off > 0) l0 = 1;
-    if (SHIFT && t == rows - 1) l1 = (N + off) / V;
-    const uint32_t bytes = l1 > l0 ? (uint32_t)(l1 - l0) * 16 : 0;
-    const uint32_t dst = smem_u32(stage0) + s * stage_bytes + l0 * 16;
-    const int from = l0 * V - off;
+    const int l0 = SHIFT && t == 0 && off > 0;
+    const int l1 = SHIFT && t == rows - 1 ? (N + off) / V : row_lines;
+    const uint32_t bytes = (uint32_t)(l1 - l0) * 16;
+    const uint32_t dst = smem_u32(ring) + s * stage_bytes + l0 * 16;
+    const long from = (long)l0 * V - off;
     mbar_arrive_expect_tx(bar + 8 * s, bytes * (FULL ? 3 : 2));
-    if (bytes == 0) return;
     bulk_load(dst, reinterpret_cast<const T*>(a.y) + t * a.ldy + from, bytes, bar + 8 * s, pol);
     bulk_load(dst + row_bytes, reinterpret_cast<const T*>(a.res) + t * a.ldr + from, bytes,
               bar + 8 * s, pol);
@@ -260,86 +255,73 @@ __global__ void __launch_bounds__(kRingThreads, 2)
       const long t = blockIdx.x + (long)s * gridDim.x;
       if (t < rows) load_row(t, s);
     }
-  uint4 keep[SHIFT ? 1 : 3][VPT];  // post, pre, channel gate
-  const T* src[3] = {reinterpret_cast<const T*>(a.post_w), reinterpret_cast<const T*>(a.pre_w),
-                     a.gate_kind == 2 ? reinterpret_cast<const T*>(a.gate) : nullptr};
-  if (SHIFT) {
+  // first element of this thread's line v, negative before the row
+  auto first = [&](int v) { return ((int)threadIdx.x + v * nt) * V - off; };
+  auto whole = [&](int i) { return !SHIFT || (i >= 0 && i + V <= N); };
+  // post_w times a channel gate, and pre_w, of this thread's elements
+  float post[VPT][V];
+  uint4 pre[VPT];
 #pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      if (!src[w]) continue;
-      uint4* d = s_w + w * w_lines;
-      for (int i = threadIdx.x; i < w_lines; i += kRingThreads) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        const int i0 = (i - 1) * V;  // weights of the line
-        if (i0 >= 0 && i0 + V <= N) {
-          u = __ldg(reinterpret_cast<const uint4*>(src[w] + i0));
-        } else if (i0 >= 0) {
-          T* e = reinterpret_cast<T*>(&u);
+  for (int v = 0; v < VPT; ++v) {
+    const int i = first(v);
+    auto take = [&](const void* p) {
+      uint4 u = make_uint4(0, 0, 0, 0);
+      if (!p || i >= N) return u;
+      const T* w = reinterpret_cast<const T*>(p);
+      if (!SHIFT) return __ldg(reinterpret_cast<const uint4*>(w + i));
+      T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-          for (int j = 0; j < V; ++j) e[j] = i0 + j < N ? src[w][i0 + j] : from_f<T>(0.f);
-        }
-        d[i] = u;
-      }
+      for (int j = 0; j < V; ++j)
+        if (i + j >= 0 && i + j < N) e[j] = w[i + j];
+      return u;
+    };
+    pre[v] = take(a.pre_w);
+    unpack_v<T, V>(take(a.post_w), post[v]);
+    float g[V];
+    if (a.gate_kind == 2) unpack_v<T, V>(take(a.gate), g);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!a.post_w) post[v][j] = 1.f;
+      if (a.gate_kind == 2) post[v][j] *= gate_act(g[j], a.act);
     }
-    __syncthreads();
-  } else {
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-      for (int v = 0; v < VPT; ++v) {
-        const int i = threadIdx.x + v * kRingThreads;
-        keep[SHIFT ? 0 : w][v] = src[w] && i < lines ? __ldg(reinterpret_cast<const uint4*>(src[w]) + i)
-                                                     : make_uint4(0, 0, 0, 0);
-      }
   }
   int n = 0;
   for (long t = blockIdx.x; t < rows; t += gridDim.x, ++n) {
     const int s = n % stages;
-    const int off = offset_of(t);
     float scale = a.alpha;
     if (a.gate_kind == 1)
       scale *= gate_act(to_f(reinterpret_cast<const T*>(a.gate)[t * a.ldg]), a.act);
     if (!mbar_wait_bounded(bar + 8 * s, (n / stages) & 1, &abort_flag, status)) break;
-    const uint4* sy = reinterpret_cast<const uint4*>(stage0 + s * stage_bytes);
+    const uint4* sy = reinterpret_cast<const uint4*>(ring + s * stage_bytes);
     const uint4* sr = sy + lines;
     const uint4* sg = sr + lines;
-    auto whole = [&](int i) { return !SHIFT || (i >= 0 && i + V <= N); };  // elements i .. i + V
-    // weights of the vector of line i
-    auto weight = [&](int w, int v, int i, float* f) {
-      if (!SHIFT) {
-        unpack_v<T, V>(keep[SHIFT ? 0 : w][v], f);
-      } else {
-        const uint4* p = s_w + w * w_lines + i;  // lines start one of zeros earlier
-        unpack_v<T, V>(off ? shift_lines<T, V>(p[0], p[1], V - off) : p[1], f);
-      }
-    };
     float f[VPT][V];
     uint4 r[VPT], g[VPT];
     float ss = 0.f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int i = threadIdx.x + v * kRingThreads;
-      const int i0 = i * V - off;
+      const int i = first(v);
       uint4 u = make_uint4(0, 0, 0, 0);
       r[v] = g[v] = u;
-      if (i0 < N) {
-        u = sy[i];
-        r[v] = sr[i];
-        if (FULL) g[v] = sg[i];
-        if (SHIFT && !whole(i0)) {
+      if (i < N) {
+        const int l = threadIdx.x + v * nt;
+        u = sy[l];
+        r[v] = sr[l];
+        if (FULL) g[v] = sg[l];
+        if (SHIFT && !whole(i)) {
           // an end of the row: zeros outside it, and what was not copied (see above)
-          const bool load = (i0 < 0 && t == 0) || (i0 + V > N && t == rows - 1);
+          const bool load = (i < 0 && t == 0) || (i + V > N && t == rows - 1);
           T* e = reinterpret_cast<T*>(&u);
           T* er = reinterpret_cast<T*>(&r[v]);
           T* eg = reinterpret_cast<T*>(&g[v]);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            if (i0 + j < 0 || i0 + j >= N) {
+            if (i + j < 0 || i + j >= N) {
               e[j] = er[j] = eg[j] = from_f<T>(0.f);
             } else if (load) {
-              e[j] = (reinterpret_cast<const T*>(a.y) + t * a.ldy)[i0 + j];
-              er[j] = (reinterpret_cast<const T*>(a.res) + t * a.ldr)[i0 + j];
-              if (FULL) eg[j] = (reinterpret_cast<const T*>(a.gate) + t * a.ldg)[i0 + j];
+              e[j] = (reinterpret_cast<const T*>(a.y) + t * a.ldy)[i + j];
+              er[j] = (reinterpret_cast<const T*>(a.res) + t * a.ldr)[i + j];
+              if (FULL) eg[j] = (reinterpret_cast<const T*>(a.gate) + t * a.ldg)[i + j];
             }
           }
         }
@@ -348,7 +330,8 @@ __global__ void __launch_bounds__(kRingThreads, 2)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss += f[v][j] * f[v][j];
     }
-    ss = cta_sum(ss, red[0]);  // its barrier: the whole CTA has read the stage
+    ss = cta_sum(ss, red[0]);
+    __syncwarp();  // with the sum's barrier: the whole CTA has read the stage
     if (threadIdx.x == 0) {
       const long next = t + (long)stages * gridDim.x;
       if (next < rows) load_row(next, s);
@@ -358,20 +341,12 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     T* h = reinterpret_cast<T*>(a.h) + t * a.ldh;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int i = threadIdx.x + v * kRingThreads;
-      const int i0 = i * V - off;
-      if (i0 >= N) continue;
+      const int i = first(v);
       float w[V];
-      if (a.post_w) {
-        weight(0, v, i, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[v][j] *= w[j];
-      }
-      if (FULL || a.gate_kind == 2) {
-        if (FULL)
-          unpack_v<T, V>(g[v], w);
-        else
-          weight(2, v, i, w);
+      for (int j = 0; j < V; ++j) f[v][j] *= post[v][j];
+      if (FULL) {
+        unpack_v<T, V>(g[v], w);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[v][j] *= gate_act(w[j], a.act);
       }
@@ -381,7 +356,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         f[v][j] = w[j] + scale * f[v][j];
         sh += f[v][j] * f[v][j];
       }
-      store_v<T, V>(h, i0, N, whole(i0), f[v]);
+      if (i < N) store_v<T, V>(h, i, N, whole(i), f[v]);
     }
     if (!a.x) continue;
     sh = cta_sum(sh, red[1]);
@@ -389,36 +364,36 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     T* x = reinterpret_cast<T*>(a.x) + t * a.ldx;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int i = threadIdx.x + v * kRingThreads;
-      const int i0 = i * V - off;
-      if (i0 >= N) continue;
+      const int i = first(v);
       float w[V];
-      weight(1, v, i, w);
+      unpack_v<T, V>(pre[v], w);
 #pragma unroll
       for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
-      store_v<T, V>(x, i0, N, whole(i0), w);
+      if (i < N) store_v<T, V>(x, i, N, whole(i), w);
     }
   }
 }
 
-template <typename T, int VPT, bool FULL, bool SHIFT>
-int launch_ring(const NormArgs& a, int rows, int stages, int bytes, cudaStream_t st, int* status) {
-  auto fn = norm_gate_residual_ring_kernel<T, VPT, FULL, SHIFT>;
-  // the limit is set once, to what two CTAs of an SM may have
+template <typename T, bool FULL, bool SHIFT>
+int launch_ring(const NormArgs& a, int rows, int threads, int stages, int bytes, cudaStream_t st,
+                int* status) {
+  auto fn = norm_gate_residual_ring_kernel<T, FULL, SHIFT>;
+  // the limit is set once, to what the largest CTA may have
   if (int rc = ensure_smem_attr((const void*)fn, 110 * 1024, "norm_gate_residual")) return rc;
-  const int grid = 2 * num_sms();
-  fn<<<grid < rows ? grid : rows, kRingThreads, bytes, st>>>(a, rows, stages, status);
+  // 512 threads on an SM; a multiple of 8 (see the kernel) unless every row has its own CTA
+  const int grid = num_sms() * (2 * kRingThreads / threads) / 8 * 8;
+  fn<<<grid < rows ? grid : rows, threads, bytes, st>>>(a, rows, stages, status);
   return check_launch("norm_gate_residual");
 }
 
-template <typename T, int VPT>
-int launch_ring_of(const NormArgs& a, int rows, int stages, int bytes, bool shift, cudaStream_t st,
-                   int* status) {
+template <typename T>
+int launch_ring_of(const NormArgs& a, int rows, int threads, int stages, int bytes, bool shift,
+                   cudaStream_t st, int* status) {
   if (a.gate_kind == 3)
-    return shift ? launch_ring<T, VPT, true, true>(a, rows, stages, bytes, st, status)
-                 : launch_ring<T, VPT, true, false>(a, rows, stages, bytes, st, status);
-  return shift ? launch_ring<T, VPT, false, true>(a, rows, stages, bytes, st, status)
-               : launch_ring<T, VPT, false, false>(a, rows, stages, bytes, st, status);
+    return shift ? launch_ring<T, true, true>(a, rows, threads, stages, bytes, st, status)
+                 : launch_ring<T, true, false>(a, rows, threads, stages, bytes, st, status);
+  return shift ? launch_ring<T, false, true>(a, rows, threads, stages, bytes, st, status)
+               : launch_ring<T, false, false>(a, rows, threads, stages, bytes, st, status);
 }
 
 template <typename T, int VPT>
@@ -449,21 +424,15 @@ int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
   for (const void* p : wp) w16 = w16 && (!p || aligned16(p));
   const int mode = !w16 ? 2 : on16 ? 0 : alike ? 1 : 2;
   const int nv = (a.N + V - 1) / V + (mode == 1 ? 1 : 0);
-  // the ring: some rows for each CTA, most of its threads busy, two stages at least
+  // the ring: some rows for each CTA, rows of some lines, two stages at least
   const bool shift = mode != 0 || a.N % V != 0;
   const int lines = (a.N + V - 1) / V + (shift ? 1 : 0);
-  if (mode < 2 && rows >= kRingRows && lines > kRingThreads / 2 && lines <= 3 * kRingThreads) {
-    const int fixed = shift ? 3 * (lines + 2) * 16 : 0;
+  if (mode < 2 && rows >= kRingRows && lines >= kRingLines && lines <= 3 * kRingThreads) {
+    const int threads = (lines + 95) / 96 * 32;
     const int stage = lines * 16 * (a.gate_kind == 3 ? 3 : 2);
-    int stages = (108 * 1024 - fixed) / stage;
+    int stages = 216 * 1024 / (2 * kRingThreads / threads) / stage;
     if (stages > 8) stages = 8;
-    if (stages >= 2) {
-      const int bytes = fixed + stages * stage;
-      const int vpt = (lines + kRingThreads - 1) / kRingThreads;
-      return vpt == 1   ? launch_ring_of<T, 1>(a, rows, stages, bytes, shift, st, status)
-             : vpt == 2 ? launch_ring_of<T, 2>(a, rows, stages, bytes, shift, st, status)
-                        : launch_ring_of<T, 3>(a, rows, stages, bytes, shift, st, status);
-    }
+    if (stages >= 2) return launch_ring_of<T>(a, rows, threads, stages, stages * stage, shift, st, status);
   }
   // few rows: as many threads as there are vectors (latency); many: two vectors for each
   int vpt = rows <= 2 * 148 ? 1 : 2;
