@@ -16,7 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib as L
-from . import ops
+from . import fp4, ops
 
 
 @dataclass
@@ -121,3 +121,135 @@ class MoEBlock:
             self.forward(h, r, outs, block_n, ws)
         self._graphs[T] = (g, h, r, outs, ws)
         return self._graphs[T]
+
+
+@dataclass
+class BlockFP4Outputs:
+    out: torch.Tensor          # [T, H] bf16  new residual stream
+    x: torch.Tensor | None     # [T, H] bf16  input of the next block (with next_gamma)
+    h1: torch.Tensor           # [T, H] bf16  h + r
+    topw: torch.Tensor         # [T, k] fp32
+    topi: torch.Tensor         # [T, k] int32
+
+
+class MoEBlockFP4:
+    """The MoE block with 4-bit expert weights, a router of either score, and optionally the norms
+    that some models have around a block:
+
+        h1, x2 = h + r, rmsnorm(h1) * gamma
+        topw, topi = route(x2 gate_w^T)                     (ops.route_topk)
+        y = sum_k topw_k w2[e_k] (SwiGLU(w13[e_k] x2)) + shared    (quantised rows, fp4.ExpertGemmFP4)
+        out = h1 + residual_scale * (rmsnorm(y) * post_gamma | y);  x = rmsnorm(out) * next_gamma
+
+    gamma, post_gamma, next_gamma [H] bf16; gate_w [E, H] fp32 (or bf16); bias [E] fp32 | None; w13 and
+    w2, and w13s / w2s of a shared expert (stacks of one), as ``fp4.quantize_weight`` or a
+    checkpoint gives them: (codes, scale bytes, factors | None). x_scales: fp32 factors [1] of the
+    rows of x2 and of the activations ("nv"; ``calibrate`` sets them from a batch). Expert weights
+    take 0.53 ("mx") or 0.56 ("nv") bytes an element instead of 2. No reference counterpart
+    beyond the block's own composition (glm52/bench/bench_layer.py:365-374)."""
+
+    def __init__(self, gamma, gate_w, bias, w13, w2, fmt: str, w13s=None, w2s=None, *, topk: int = 8,
+                 eps: float = 1e-5, routed_scale: float = 2.5, renorm: bool = True,
+                 score: str = "sigmoid", n_group: int = 1, topk_group: int = 1, post_gamma=None,
+                 next_gamma=None, residual_scale: float = 1.0, x_scales=None):
+        if (w13s is None) != (w2s is None):
+            raise ValueError("a shared expert has both projections")
+        self.gamma, self.bias = gamma, bias
+        if gate_w.dtype == torch.float32:
+            self.wa, self.nplanes = ops.router_split_weight(gate_w), 3
+        else:
+            self.wa, self.nplanes = gate_w.contiguous(), 1
+        self.E, self.H = gate_w.shape
+        self.topk, self.eps, self.routed_scale, self.renorm = topk, eps, routed_scale, renorm
+        self.score, self.n_group, self.topk_group = score, n_group, topk_group
+        self.post_gamma, self.next_gamma, self.residual_scale = post_gamma, next_gamma, residual_scale
+        self.device = gamma.device
+        self.fmt = fmt
+        if fmt == "nv" and x_scales is None:
+            x_scales = tuple(torch.ones(1, device=self.device) for _ in range(2))
+        self.x_scales = x_scales if fmt == "nv" else (None, None)
+        mk = lambda w, i, gate_up: fp4.ExpertGemmFP4(  # noqa: E731
+            w[0], w[1], fmt, gscale=w[2], x_gscale=self.x_scales[i], gate_up=gate_up)
+        self.w13, self.w2 = mk(w13, 0, True), mk(w2, 1, False)
+        self.w13s = mk(w13s, 0, True) if w13s is not None else None
+        self.w2s = mk(w2s, 1, False) if w2s is not None else None
+        self.I = self.w13.cols
+        if self.w13.E != self.E or self.w2.E != self.E or self.w2.K != self.I or self.w2.cols != self.H:
+            raise ValueError("router, w13 and w2 do not fit together")
+
+    def _empty(self, *shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device=self.device)
+
+    def _route(self, h, r):
+        """Norm, router and dispatch layout: h1, x2, topw, topi, the layout and its block_n."""
+        T = h.shape[0]
+        h1, x2 = self._empty(T, self.H), self._empty(T, self.H)
+        ops.add_rmsnorm(h, r, self.gamma, h1, x2, eps=self.eps)
+        nsplit = ops.router_nsplit(T, self.H, self.E, self.nplanes)
+        partial = self._empty(nsplit, T, self.E, dtype=torch.float32)
+        ops.router_logits(x2, self.wa, self.nplanes, partial, nsplit)
+        logits = partial[0]
+        if nsplit > 1:
+            logits = self._empty(T, self.E, dtype=torch.float32)
+            ops.scale_sum_planes(partial, nsplit, None, logits)
+        topw = self._empty(T, self.topk, dtype=torch.float32)
+        topi = self._empty(T, self.topk, dtype=torch.int32)
+        ops.route_topk(logits, topw, topi, score=self.score, bias=self.bias, n_group=self.n_group,
+                       topk_group=self.topk_group, renorm=self.renorm, scale=self.routed_scale)
+        bn = int(L.lib().fus_moe_block_pick_block_n(T, self.E, self.topk))
+        R = T * self.topk
+        cap = -(-(R + min(R, self.E) * (bn - 1)) // bn) * bn
+        layout = (self._empty(cap, dtype=torch.int32), self._empty(cap // bn, dtype=torch.int32),
+                  self._empty(1, dtype=torch.int32))
+        # large batches: an expert's rows spread evenly over its blocks
+        ops.moe_align(topi, self.E, bn, *layout, flags=ops.ALIGN_BALANCED if T > 16 else 0)
+        return h1, x2, topw, topi, layout, bn
+
+    def _experts(self, x2, topi, layout, bn):
+        """Rows [T, k, H] of the routed experts and the shared expert's [T, H] (fp32) or None."""
+        T = x2.shape[0]
+        act = self._empty(layout[0].numel(), self.I)
+        self.w13(x2, act, *layout, bn, topk=self.topk, scatter=False)
+        # a slot without an expert (topi -1, weight 0) is written by no one
+        y = torch.zeros(T * self.topk, self.H, dtype=torch.bfloat16, device=self.device)
+        self.w2(act, y, *layout, bn, gather=False, pairs=T * self.topk)
+        shared = None
+        if self.w13s is not None:
+            act_s, shared = self._empty(T, self.I), self._empty(T, self.H, dtype=torch.float32)
+            self.w13s(x2, act_s)
+            self.w2s(act_s, shared)
+        return act, y.view(T, self.topk, self.H), shared
+
+    def forward(self, h: torch.Tensor, r: torch.Tensor) -> BlockFP4Outputs:
+        """h, r [T, H] bf16. Allocates through torch's caching allocator and never synchronises, so
+        it can be recorded in a CUDA graph."""
+        T = h.shape[0]
+        normed = self.post_gamma is not None or self.next_gamma is not None or self.residual_scale != 1.0
+        x = self._empty(T, self.H) if self.next_gamma is not None else None
+        if T == 0:
+            e = self._empty(0, self.H)
+            return BlockFP4Outputs(e, x, e, self._empty(0, self.topk, dtype=torch.float32),
+                                   self._empty(0, self.topk, dtype=torch.int32))
+        h1, x2, topw, topi, layout, bn = self._route(h, r)
+        _, y, shared = self._experts(x2, topi, layout, bn)
+        out = self._empty(T, self.H)
+        ops.merge(y, topw, None if normed else h1, shared, out, round_mid=False)
+        if normed:
+            ops.norm_gate_residual(out, h1, out, x, post_w=self.post_gamma, pre_w=self.next_gamma,
+                                   alpha=self.residual_scale, eps=self.eps)
+        return BlockFP4Outputs(out, x, h1, topw, topi)
+
+    __call__ = forward
+
+    def calibrate(self, h: torch.Tensor, r: torch.Tensor) -> None:
+        """Sets the factors of x2 and of the activations ("nv") from a batch: their largest
+        magnitudes over 448 * 6, in place, so captured graphs use them too."""
+        if self.fmt != "nv":
+            return
+        h1, x2, topw, topi, layout, bn = self._route(h, r)
+        self.x_scales[0].copy_(x2.abs().amax().float().clamp_min(1e-20) / 2688.0)
+        act, _, _ = self._experts(x2, topi, layout, bn)
+        p = layout[0]
+        live = (p < topi.numel()) & (torch.arange(p.numel(), device=p.device) < layout[2])
+        top = torch.where(live[:, None], act.abs(), 0.0).amax().float()
+        self.x_scales[1].copy_(top.clamp_min(1e-20) / 2688.0)

@@ -69,29 +69,45 @@ class ExpertGemmFP4:
         d.epilogue = ops.FUS_EPI_SWIGLU if gate_up else ops.FUS_EPI_BF16
         self._desc = d
 
-    def __call__(self, x, out, sorted_ids, expert_ids, ntp, block_n: int, *, topk: int = 1,
-                 gather: bool = True, scatter: bool = True, row_scale=None):
+    def __call__(self, x, out, sorted_ids=None, expert_ids=None, ntp=None, block_n: int = 0, *,
+                 topk: int = 1, gather: bool = True, scatter: bool = True, pairs: int | None = None,
+                 row_scale=None):
         """One projection over a dispatch layout (``ops.moe_align`` with block_n).
 
         gather: x [T, K] holds tokens, dispatch row p is x[sorted_ids[p] // topk]; else x
-        [capacity, K] is in dispatch order. scatter: out [T * topk, cols] in pair order (row
+        [capacity, K] is in dispatch order. scatter: out [pairs, cols] in pair order (row
         sorted_ids[p]), else out [capacity, cols] in dispatch order; rows of pads are left as
-        they were. out is bf16 or fp32; row_scale: fp32, one for each row of out."""
+        they were. pairs: T * topk, needed when neither gather nor scatter tells it. out is bf16
+        or fp32; row_scale: fp32, one for each row of out.
+
+        Without sorted_ids the one expert multiplies every row: x [T, K], out [T, cols]."""
         dt, ldx = ops._dtype(x, "x"), ops._rows2d(x, "x")
-        cap = sorted_ids.numel()
-        pairs = x.shape[0] * topk if gather else out.shape[0] if scatter else None
-        if pairs is None:
-            raise ValueError("rows in dispatch order need gather or scatter to name the pairs")
         if x.shape[1] != self.K or out.shape[1] != self.cols:
             raise ValueError(f"x [.., {self.K}] and out [.., {self.cols}] required")
+        if sorted_ids is None:
+            if self.E != 1 or expert_ids is not None or ntp is not None:
+                raise ValueError("without sorted_ids: one expert, no expert_ids, no ntp")
+            cap = x.shape[0]
+            block_n = block_n or dense_block_n(cap)
+            gather = scatter = False
+            spread = 0
+        else:
+            cap = sorted_ids.numel()
+            if gather:
+                pairs = x.shape[0] * topk
+            elif scatter and pairs is None:
+                pairs = out.shape[0]
+            if pairs is None:
+                raise ValueError("rows in and out in dispatch order: pairs (T * topk) required")
+            if block_n < 1 or cap % block_n or expert_ids.numel() < cap // block_n:
+                raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each")
+            for t, what in ((sorted_ids, "sorted_ids"), (expert_ids, "expert_ids"), (ntp, "ntp")):
+                ops._need(t, torch.int32, what)
+            spread = 4 * pairs if gather else 0
         if out.shape[0] < (pairs if scatter else cap) or (not gather and x.shape[0] < cap):
             raise ValueError("too few rows")
-        if expert_ids.numel() < cap // block_n or cap % block_n:
-            raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each")
         if out.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out is bf16 or fp32")
-        for t, what in ((sorted_ids, "sorted_ids"), (expert_ids, "expert_ids"), (ntp, "ntp")):
-            ops._need(t, torch.int32, what)
         ops._need(row_scale, torch.float32, "row_scale")
         if row_scale is not None and row_scale.numel() < out.shape[0]:
             raise ValueError("row_scale: one for each row of out")
@@ -101,15 +117,25 @@ class ExpertGemmFP4:
         # the packed rows: fresh for each call, so calls on other streams and captured graphs
         # never share them
         size = cap * d.ldxq + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n)
-        rows = torch.empty(size + 4 * pairs, dtype=torch.uint8, device=self.device)
+        rows = torch.empty(size + spread, dtype=torch.uint8, device=self.device)
         d.xq = ops._p(rows)
         d.xsf = d.xq + cap * d.ldxq
         d.x_rows, d.block_n = cap, block_n
-        d.expert_ids, d.ntp = ops._p(expert_ids), ops._p(ntp)
-        d.live_ids, d.live_limit, d.scatter = ops._p(sorted_ids), pairs, int(scatter)
+        if sorted_ids is not None:
+            d.expert_ids, d.ntp = ops._p(expert_ids), ops._p(ntp)
+            d.live_ids, d.live_limit, d.scatter = ops._p(sorted_ids), pairs, int(scatter)
         d.row_scale = ops._p(row_scale)
         d.out, d.ldo = ops._p(out), ops._rows2d(out, "out")
         d.out_rows, d.out_dtype = out.shape[0], ops.DT[out.dtype]
         ops._call_on(self._dev, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
-                     x.shape[0], topk if gather else 0, d.xq + size)
+                     x.shape[0], topk if gather else 0, d.xq + size if spread else None)
         return out
+
+
+def dense_block_n(rows: int) -> int:
+    """Token block of a product whose rows all meet one weight: the smallest that holds them,
+    256 at most."""
+    for bn in (16, 32, 64, 128):
+        if rows <= bn:
+            return bn
+    return 256

@@ -287,3 +287,46 @@ def test_empty_batch():
     ops.fp4_quantize(torch.empty(0, 64, device="cuda"), torch.empty(0, 32, dtype=torch.uint8, device="cuda"),
                      torch.empty(0, dtype=torch.uint8, device="cuda"), "nv")
     finish()
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("T,N,K", [(1, 48, 96), (17, 256, 256), (100, 400, 544), (500, 144, 320)])
+def test_dense_product(fmt, T, N, K):
+    """One weight, every row: no layout."""
+    q, s, g, w = _stack(1, N, K, fmt, 4)
+    x = torch.randn(T, K, device="cuda").to(torch.float16)
+    out = torch.full((T + 1, N), 5.0, dtype=torch.float32, device="cuda")
+    fp4.ExpertGemmFP4(q, s, fmt, gscale=g)(x, out)
+    finish()
+    xv = Q.values(*Q.quantize(x.double().cpu().numpy(), fmt), fmt)
+    ref, mag = xv @ w[0].T, np.abs(xv) @ np.abs(w[0]).T
+    got = out.double().cpu().numpy()
+    assert (got[T] == 5.0).all()
+    assert (np.abs(got[:T] - ref) <= (K / 16 + 8) * 2.0 ** -23 * mag + 1e-30).all()
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_large_batch_quantises_tokens_once(fmt):
+    """Enough pairs that tokens are quantised once and written to their pairs' rows: the same bits as
+    one pass over the dispatch order gives. Holes, pads and junk behind the layout included."""
+    T, k, E, N, K, bn = 900, 6, 4, 32, 1024, 256
+    rng = np.random.default_rng(3)
+    topi = rng.integers(0, E, (T, k))
+    ids, eids, total = Q.layout(topi, E, bn, extra=1)
+    hole = ids == 77  # a pair that is not placed
+    ids[hole] = T * k
+    dev = [torch.from_numpy(v).cuda() for v in (ids, eids, np.array([total], dtype=np.int32))]
+    x = torch.randn(T, K, device="cuda").to(torch.bfloat16)
+    q, s, g, _ = _stack(E, N, K, fmt, 8)
+    proj = fp4.ExpertGemmFP4(q, s, fmt, gscale=g)
+    out = torch.full((T * k, N), 3.0, dtype=torch.bfloat16, device="cuda")
+    proj(x, out, *dev, bn, topk=k)
+    # rows already in dispatch order take the other way
+    live = (ids < T * k) & (np.arange(len(ids)) < total)
+    xs = torch.zeros(len(ids), K, dtype=torch.bfloat16, device="cuda")
+    at = torch.from_numpy(np.flatnonzero(live)).cuda()
+    xs[at] = x[torch.from_numpy(ids[live].astype(np.int64)).cuda() // k]
+    want = torch.full((T * k, N), 3.0, dtype=torch.bfloat16, device="cuda")
+    proj(xs, want, *dev, bn, gather=False)
+    finish()
+    assert torch.equal(out, want) and (out[77] == 3.0).all()
