@@ -14,12 +14,10 @@
 // elements = 128 bytes of a row):
 //   warp 0  : producer, one lane: a TMA box of weights and one of token rows (128-byte swizzle),
 //             one bulk copy each of their scale atoms
-//   warp 1  : TMEM owner; one lane issues a stage's four K = 64 MMAs
-//   warp 2  : one lane copies a stage's scales into tensor memory (tcgen05.cp) ahead of the
-//             MMAs, into columns of that stage. Issued by the MMA thread they would run in order
-//             with the MMAs, about 55 cycles each: 12 of them for 512 cycles of MMA (dense
-//             8192 x 4096 x 6144 NV: 290 -> 230 us with 128-token blocks)
-//   warps 4-7: epilogue, TMEM -> registers -> shared (token-major) -> 16-byte stores
+//   warp 1  : TMEM owner; one lane copies a stage's scales into tensor memory (tcgen05.cp, in
+//             order with the MMAs of the same thread) and issues four K = 64 MMAs. Every stage has
+//             scale columns of its own: a copy never waits for the MMAs of the stage before
+//   warps 2-5: epilogue, TMEM -> registers -> shared (token-major) -> 16-byte stores
 // The accumulator is double-buffered: the next unit's MMAs run while the epilogue drains.
 // Blocks up to 64 tokens run here, two CTAs on an SM (bound by HBM: the weights); wider ones on
 // SM pairs, fp4_gemm_pair.cuh.
@@ -77,7 +75,7 @@ struct Cfg {
   static constexpr int SFB_BYTES = CELLS * 512;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
   static constexpr int CHUNK = BN < 32 ? BN : 32;  // token columns of an epilogue step
-  static constexpr int THREADS = 128 + kGroupThreads;
+  static constexpr int THREADS = 64 + kGroupThreads;
   static constexpr int STAGE_OUT = CHUNK * 256;  // staged bf16 rows, two buffers
   static constexpr int EPI_BYTES = 2 * STAGE_OUT + BN * 8;  // ..., row numbers and scales
   static constexpr int CTAS = 2;                              // for an SM (TMEM 256 columns each)
@@ -312,8 +310,7 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
   const uint32_t bar_empty = bar_full + 8 * STAGES;
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // accumulator finished
   const uint32_t bar_free = bar_acc + 8 * C::ACCS;   // accumulator drained
-  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // a stage's scales are in tensor memory
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);
 
@@ -322,7 +319,6 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
-      mbar_init(bar_sf + 8 * s, 1);
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(bar_acc + 8 * b, 1);
@@ -428,12 +424,16 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       const uint32_t acc = tmem + buf * BN;
       for (int k = 0; k < a.nst && ok; ++k, ++it) {
         const int s = it % STAGES;
-        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-             warp_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
+#pragma unroll
+          for (int c = 0; c < C::CELLS; ++c) {
+            tc_cp_scales(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
+            tc_cp_scales(sf + C::SFB_OFF + 4 * c, sSB + s * C::SFB_BYTES + 512 * c);
+          }
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -452,33 +452,9 @@ __global__ void __launch_bounds__((Cfg<BN, FMT>::THREADS), (Cfg<BN, FMT>::CTAS))
       }
       ++n;
     }
-  } else if (warp == 2) {
-    int it = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const int blk = u / a.m_tiles;
-      if (expert_of(blk) < 0) continue;
-      for (int k = 0; k < a.nst; ++k, ++it) {
-        const int s = it % STAGES;
-        // a full stage: the MMAs that read its scale columns before are done
-        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
-#pragma unroll
-          for (int c = 0; c < C::CELLS; ++c) {
-            tc_cp_scales(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
-            tc_cp_scales(sf + C::SFB_OFF + 4 * c, sSB + s * C::SFB_BYTES + 512 * c);
-          }
-          tc_commit(bar_sf + 8 * s);
-        }
-        __syncwarp();
-      }
-    }
-  } else if (warp >= 4) {
+  } else if (warp >= 2) {
     const int q4 = warp & 3;  // the TMEM lanes this warp may read
-    const int et = threadIdx.x - 128;
+    const int et = threadIdx.x - 64;
     constexpr int NI = C::CHUNK / 8;
     uint8_t* stage = smem + STAGES * C::STAGE_BYTES;
     int* s_row = reinterpret_cast<int*>(stage + 2 * C::STAGE_OUT);

@@ -9,9 +9,9 @@
 // against all tokens). 38 KB for 512 cycles.
 //
 // Both CTAs' copies complete on the leader's full barrier (tensor copies of .cta_group::2, the
-// scales too; no multicast). The leader's warp 2 copies both CTAs' scales into their tensor
-// memory (tcgen05.cp.cta_group::2), its warp 1 issues the MMAs; commits free the stage and
-// hand over the accumulators on both CTAs. 256 columns hold them, two buffers of 128-token
+// scales too; no multicast). The leader's warp 1 copies both CTAs' scales into their tensor
+// memory (tcgen05.cp.cta_group::2) and issues the MMAs; commits free the stage and hand over
+// the accumulators on both CTAs. 256 columns hold them, two buffers of 128-token
 // blocks or one of 256: the epilogue reads its half into registers at once and frees the
 // buffer before it converts and stores.
 #pragma once
@@ -30,7 +30,7 @@ struct PairCfg {
   static constexpr int GROUPS = 2;
   static constexpr int COLS_THREAD = BN / GROUPS;  // accumulator columns of a thread
   static constexpr int CHUNK = 32;
-  static constexpr int THREADS = 128 + GROUPS * kGroupThreads;
+  static constexpr int THREADS = 64 + GROUPS * kGroupThreads;
   static constexpr int STAGE_OUT = CHUNK * 256;  // staged bf16 rows of a group, two buffers
   static constexpr int EPI_BYTES = GROUPS * (2 * STAGE_OUT + COLS_THREAD * 8);
   static constexpr int FIT = (226 * 1024 - EPI_BYTES - 1280) / STAGE_BYTES;
@@ -68,13 +68,6 @@ FUS_DEVICE void tc_cp_scales_pair(uint32_t taddr, uint32_t saddr) {
                "l"(scale_desc(saddr))
                : "memory");
 }
-// arrive on this CTA's `bar` once the thread's earlier copies and MMAs of the pair are done
-FUS_DEVICE void tc_commit_pair_local(uint32_t bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-      : "memory");
-}
-
 template <int BN, int FMT, bool SWIGLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::THREADS), 1)
     fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tw,
@@ -97,8 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
   const uint32_t bar_empty = bar_full + 8 * STAGES;  // both
   const uint32_t bar_acc = bar_empty + 8 * STAGES;   // both
   const uint32_t bar_free = bar_acc + 8 * C::ACCS;   // leader's used
-  const uint32_t bar_sf = bar_free + 8 * C::ACCS;    // leader's used
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 2 * C::ACCS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2 * C::ACCS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* group_ok = reinterpret_cast<volatile int*>(tmem_slot + 2);  // [GROUPS]
 
@@ -109,7 +101,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
-      mbar_init(bar_sf + 8 * s, 1);
     }
     for (int b = 0; b < C::ACCS; ++b) {
       mbar_init(bar_acc + 8 * b, 1);
@@ -222,18 +213,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
     for (int u = first; u < units && ok; u += stride) {
       const int blk = u / m_pairs;
       if (expert_of(blk) < 0) continue;
-      const int nm = width_of(live_of(blk));
+      const int live = live_of(blk), nm = width_of(live);
+      // atoms of token scales that hold live rows
+      const int atoms = C::ATOMS > 1 && live <= 128 ? 1 : C::ATOMS;
       const int buf = n % C::ACCS;
       ok = warp_wait_bounded(bar_free + 8 * buf, ((n / C::ACCS) & 1) ^ 1, abort_flag, a.status);
       tc_fence_after();
       for (int k = 0; k < a.nst && ok; ++k, ++it) {
         const int s = it % STAGES;
-        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status) &&
-             warp_wait_bounded(bar_sf + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
+        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
+#pragma unroll
+          for (int c = 0; c < C::CELLS; ++c) {
+            tc_cp_scales_pair(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
+#pragma unroll
+            for (int t = 0; t < C::ATOMS; ++t)
+              if (t < atoms)
+                tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
+                                  sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
+          }
           const int steps = min(4, (a.K - k * kFp4StageK + 63) / 64);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -253,41 +254,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairCfg<BN, FMT>::T
       }
       ++n;
     }
-  } else if (warp == 2 && leader) {
-    // ---- scales into both CTAs' tensor memory ----
-    int it = 0;
-    bool ok = true;
-    for (int u = first; u < units && ok; u += stride) {
-      const int blk = u / m_pairs;
-      if (expert_of(blk) < 0) continue;
-      const int atoms = C::ATOMS > 1 && live_of(blk) <= 128 ? 1 : C::ATOMS;
-      for (int k = 0; k < a.nst; ++k, ++it) {
-        const int s = it % STAGES;
-        // a full stage: the MMAs that read its scale columns before are done
-        ok = warp_wait_bounded(bar_full + 8 * s, (it / STAGES) & 1, abort_flag, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t sf = tmem + C::SF_COL + s * C::SF_COLS;
-#pragma unroll
-          for (int c = 0; c < C::CELLS; ++c) {
-            tc_cp_scales_pair(sf + 4 * c, sSA + s * C::SFA_BYTES + 512 * c);
-#pragma unroll
-            for (int t = 0; t < C::ATOMS; ++t)
-              if (t < atoms)
-                tc_cp_scales_pair(sf + C::SFB_OFF + 4 * (c * C::ATOMS + t),
-                                  sSB + s * C::SFB_BYTES + 512 * (c * C::ATOMS + t));
-          }
-          tc_commit_pair_local(bar_sf + 8 * s);
-        }
-        __syncwarp();
-      }
-    }
-  } else if (warp >= 4) {
+  } else if (warp >= 2) {
     // ---- epilogue (both CTAs): each group has half of the columns ----
     const int q4 = warp & 3;
-    const int grp = (warp - 4) >> 2;
-    const int et = threadIdx.x - 128 - grp * kGroupThreads;
+    const int grp = (warp - 2) >> 2;
+    const int et = threadIdx.x - 64 - grp * kGroupThreads;
     constexpr int NI = C::CHUNK / 8, NCH = C::COLS_THREAD / C::CHUNK;
     uint8_t* stage = smem + STAGES * C::STAGE_BYTES + grp * (2 * C::STAGE_OUT + C::COLS_THREAD * 8);
     int* s_row = reinterpret_cast<int*>(stage + 2 * C::STAGE_OUT);
