@@ -280,14 +280,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int o = kLanes / 4; o < kLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
     if (!live) continue;
-    for (int slot = 0; slot < (SPREAD ? id_div : 1); ++slot) {
-      int d = p;
-      if (SPREAD) {
-        const int id = p * id_div + slot;
-        if (id >= id_limit) break;
-        d = __ldg(pos + id);
-        if (d < 0 || d >= x_rows || d >= placed || __ldg(ids + d) != id) continue;
-      }
+    auto put = [&](int d) {
       if (data) *reinterpret_cast<uint2*>(q + (long)d * ldq) = c;
       if (tile_log2 == 0) {
         if (k < K && (FMT == FUS_FP4_NV || (threadIdx.x & 1) == 0))
@@ -296,6 +289,28 @@ __global__ void __launch_bounds__(256)
         *reinterpret_cast<uint32_t*>(cells + (d >> tile_log2) * per_tile +
                                      fp4_row_offset(d & (tile - 1))) = word;
       }
+    };
+    if (!SPREAD) {
+      put(p);
+      continue;
+    }
+    // the places of four pairs at a time: their loads do not wait for one another
+    for (int s0 = 0; s0 < id_div; s0 += 4) {
+      int d[4];
+      bool is[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int id = p * id_div + s0 + u;
+        is[u] = s0 + u < id_div && id < id_limit;
+        d[u] = is[u] ? __ldg(pos + id) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        is[u] = is[u] && d[u] >= 0 && d[u] < x_rows && d[u] < placed &&
+                __ldg(ids + d[u]) == p * id_div + s0 + u;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (is[u]) put(d[u]);
     }
   }
 }
