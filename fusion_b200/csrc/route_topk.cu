@@ -235,7 +235,7 @@ __device__ __noinline__ int rank_exact(const RouteArgs& a, const T* row, float t
 template <typename T, int NPL, bool SOFTMAX, bool GROUPED>
 __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs a) {
   __shared__ __align__(16) float row_c[kWarps][NPL * 32], row_l[kWarps][NPL * 32];  // lane-major
-  __shared__ float2 cand[kWarps][32];                                 // (choice, id)
+  __shared__ unsigned long long cand[kWarps][32];  // choice (ordered) and id (lower is larger)
   __shared__ float sorted[kWarps][33];
   __shared__ int place[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
     // all twice. softmax: the sum of up to 1024 terms adds some 2^-19 of a score.
     tol = SOFTMAX ? 8e-6f : 9e-7f;
   }
-  float best;
+  float best, second = -INFINITY;  // of this lane (second: GROUPED only)
   if (GROUPED) {
     float a1 = c[0], a2 = -INFINITY;
 #pragma unroll
@@ -323,18 +323,22 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
       a1 = fmaxf(a1, c[j]);
     }
     best = a1;
+    second = a2;
     for (int o = 1; o < a.lpg; o <<= 1) {
       const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
       a2 = fmaxf(fminf(a1, b1), fmaxf(a2, b2));
       a1 = fmaxf(a1, b1);
     }
     const float g = a2 > -INFINITY ? a1 + a2 : a1;
+    // each lane of a group compares with its share of the others
     int better = 0;
-#pragma unroll 4
-    for (int q = 0; q < a.n_group; ++q) {
-      const float og = __shfl_sync(kAll, g, q * a.lpg);
-      better += og > g || (og == g && q < group);
+    const int sub = lane & (a.lpg - 1);
+    for (int q0 = 0; q0 < a.n_group; q0 += a.lpg) {
+      const int q = q0 + sub;
+      const float og = __shfl_sync(kAll, g, q << a.lpg_log2);
+      better += q < a.n_group && (og > g || (og == g && q < group));
     }
+    for (int o = 1; o < a.lpg; o <<= 1) better += __shfl_xor_sync(kAll, better, o);
     if (a.topk_group < a.n_group) {
       // the last group in and the first one out: too near to tell apart in fp32?
       const bool real = group < a.n_group;
@@ -345,7 +349,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
         better = group_rank_exact<T>(a, row, top, e0, n, group);
     }
     if (better >= a.topk_group) {
-      best = -INFINITY;
+      best = second = -INFINITY;
 #pragma unroll
       for (int j = 0; j < NPL; ++j) c[j] = -INFINITY;
     }
@@ -354,15 +358,20 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
 #pragma unroll
     for (int j = 1; j < NPL; ++j) best = fmaxf(best, c[j]);
   }
-  // k-th largest lane maximum (equal maxima leave together: the bound only gets lower)
+  // k-th largest of the lanes' largest (GROUPED: two largest, as few lanes are left) choices.
+  // Equal ones leave together: the bound only gets lower.
   uint32_t mine = key_of(best), bound = 0;
+  uint32_t then = GROUPED ? key_of(second) : 0;
 #pragma unroll 4
   for (int s = 0; s < a.topk; ++s) {
     bound = __reduce_max_sync(kAll, mine);
-    if (mine == bound) mine = 0;
+    if (mine == bound) {
+      mine = then;
+      if (GROUPED) then = 0;
+    }
   }
   const float kth = value_of(bound);
-  const bool few = !(bound > key_of(-INFINITY));  // fewer than k lanes with a finite choice
+  const bool few = !(bound > key_of(-INFINITY));  // fewer than k finite ones among them
   const float limit = kth - tol * (1.f + fabsf(kth));
   uint32_t left = 0;  // this lane's candidates
 #pragma unroll
@@ -399,23 +408,25 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
     route_row_exact<T>(a, t, lane);
     return;
   }
+  // a candidate for each lane of a run of W lanes, the other runs scan their share for it
+  const int W = count <= 8 ? 8 : count <= 16 ? 16 : 32;
+  const int ci = lane & (W - 1);
   float choice = -INFINITY, logit = 0.f;
   int id = 0x7fffffff;
-  if (lane < count) {
-    const int at = place[warp][lane];
+  if (ci < count) {
+    const int at = place[warp][ci];
     choice = row_c[warp][at];
     logit = row_l[warp][at];
     const int from = at / NPL;
     id = (GROUPED ? (from >> a.lpg_log2) * a.gsz + (from & (a.lpg - 1)) * NPL : from * NPL) + at % NPL;
-    cand[warp][lane] = make_float2(choice, __int_as_float(id));
   }
+  const unsigned long long key = (unsigned long long)key_of(choice) << 32 | (uint32_t)~id;
+  if (lane < count) cand[warp][lane] = key;
   __syncwarp();
   int rank = 0;
 #pragma unroll 4
-  for (int q = 0; q < count; ++q) {
-    const float2 o = cand[warp][q];
-    rank += o.x > choice || (o.x == choice && __float_as_int(o.y) < id);
-  }
+  for (int q = lane / W; q < count; q += 32 / W) rank += cand[warp][q] > key;
+  for (int o = W; o < 32; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
   if (!plain) {
     // neighbours in the order, the first one out among them, too near to tell apart?
     if (lane < count) sorted[warp][rank] = choice;
