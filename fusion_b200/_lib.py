@@ -215,6 +215,7 @@ SIGNATURES: dict[str, tuple] = {
                                      i64, i32, i32, i32, f32, vp, vp]),
     "fus_route_topk": (i32, [vp, i32, i64, vp, i32, i32, i32, vp, vp, i32, i32, i32, f32, i32, vp,
                              vp]),
+    "fus_clear_holes": (i32, [vp, i32, vp, i64, i32, vp]),
     "fus_fp4_scale_bytes": (sz, [i32, i64, i32, i32]),
     "fus_fp4_quantize": (i32, [vp, i32, i64, i32, i32, i32, vp, i64, vp, i32, i32, vp, i64, i32,
                                vp, i64, vp, vp, vp]),

@@ -210,8 +210,8 @@ class MoEBlockFP4:
         T = x2.shape[0]
         act = self._empty(layout[0].numel(), self.I)
         self.w13(x2, act, *layout, bn, topk=self.topk, scatter=False)
-        # a slot without an expert (topi -1, weight 0) is written by no one
-        y = torch.zeros(T * self.topk, self.H, dtype=torch.bfloat16, device=self.device)
+        y = self._empty(T * self.topk, self.H)
+        ops.clear_holes(y, topi)  # a slot without an expert (weight 0) is written by no one else
         self.w2(act, y, *layout, bn, gather=False, pairs=T * self.topk)
         shared = None
         if self.w13s is not None:
@@ -223,6 +223,10 @@ class MoEBlockFP4:
     def forward(self, h: torch.Tensor, r: torch.Tensor) -> BlockFP4Outputs:
         """h, r [T, H] bf16. Allocates through torch's caching allocator and never synchronises, so
         it can be recorded in a CUDA graph."""
+        with torch.cuda.device(self.device):
+            return self._forward(h, r)
+
+    def _forward(self, h, r) -> BlockFP4Outputs:
         T = h.shape[0]
         normed = self.post_gamma is not None or self.next_gamma is not None or self.residual_scale != 1.0
         x = self._empty(T, self.H) if self.next_gamma is not None else None
@@ -244,7 +248,7 @@ class MoEBlockFP4:
     def calibrate(self, h: torch.Tensor, r: torch.Tensor) -> None:
         """Sets the factors of x2 and of the activations ("nv") from a batch: their largest
         magnitudes over 448 * 6, in place, so captured graphs use them too."""
-        if self.fmt != "nv":
+        if self.fmt != "nv" or h.shape[0] == 0:
             return
         h1, x2, topw, topi, layout, bn = self._route(h, r)
         self.x_scales[0].copy_(x2.abs().amax().float().clamp_min(1e-20) / 2688.0)

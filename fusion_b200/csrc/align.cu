@@ -272,6 +272,20 @@ __global__ void permute_rows_kernel(const __nv_bfloat16* __restrict__ src, long 
   }
 }
 
+// zeros in the rows of pairs without an expert: a warp looks at 32 ids, then writes the rows it
+// found (normally none)
+__global__ void clear_holes_kernel(const int* __restrict__ ids, int n, uint8_t* __restrict__ y,
+                                   long row_bytes, int nv) {
+  const int lane = threadIdx.x & 31;
+  const int i0 = (blockIdx.x * blockDim.x + threadIdx.x) & ~31;
+  const int i = i0 + lane;
+  unsigned holes = __ballot_sync(0xffffffffu, i < n && __ldg(ids + i) < 0);
+  for (; holes; holes &= holes - 1) {
+    uint4* d = reinterpret_cast<uint4*>(y + (long)(i0 + __ffs(holes) - 1) * row_bytes);
+    for (int v = lane; v < nv; v += 32) d[v] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 size_t small_smem_bytes(int E) {
   return sizeof(int) * ((size_t)kAlignWarps * E + 2 * E + kAlignThreads + 2 * kAlignSmallMax);
 }
@@ -361,6 +375,16 @@ extern "C" int fus_moe_align(const int* ids, int numel, int E, int block_m, int*
                              void* workspace, size_t ws_bytes, void* stream, int* status) {
   return fus_moe_align_ex(ids, numel, E, block_m, sorted_ids, sorted_cap, expert_ids, blocks_cap,
                           ntp, nullptr, 0, workspace, ws_bytes, stream, status);
+}
+
+extern "C" int fus_clear_holes(const int* ids, int n, void* y, long ldy, int H, void* stream) {
+  if (n < 0 || H < 1 || H % 8) return set_error(FUS_E_INVALID, "clear_holes: bad sizes");
+  if (n == 0) return FUS_OK;
+  if (!ids || !y || !aligned16(y) || ldy % 8 || ldy < H)
+    return set_error(FUS_E_INVALID, "clear_holes: rows must be 16-byte aligned");
+  clear_holes_kernel<<<(n + 255) / 256, 256, 0, as_stream(stream)>>>(
+      ids, n, reinterpret_cast<uint8_t*>(y), ldy * 2, H / 8);
+  return check_launch("clear_holes");
 }
 
 extern "C" int fus_permute_rows(const void* src, long ld_src, const int* sorted_ids, const int* ntp,

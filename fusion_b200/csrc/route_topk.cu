@@ -10,7 +10,7 @@
 // largest expert from below, so only experts at or above it (about k + 2 of 256) are
 // compacted into shared memory, one to a lane, and ranked against one another.
 //
-// The ids are those of exact arithmetic on the logits. Without bias and groups the logits are
+// The ids are those of 64-bit arithmetic on the logits. Without bias and groups the logits are
 // ranked themselves (the score is monotone in them). Otherwise fp32 scores rank, and where two
 // choices that decide something lie within their error of each other (a few tokens in a
 // thousand) the warp decides again in fp64: the groups from all choices, the experts from the
@@ -91,11 +91,13 @@ __device__ __noinline__ void route_row_exact(const RouteArgs& a, long t, int lan
     const double l = clean(to_f(row[e]));
     return a.softmax ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l));
   };
-  double c[32];  // this lane's choices (local memory)
+  const bool plain = !a.bias && a.n_group == 1;  // the logits rank themselves
+  double c[32];                                  // this lane's choices (local memory)
   for (int j = 0; j < n; ++j) {
     const int e = e0 + j;
-    c[j] = clean(to_f(row[e])) > -INFINITY ? score(e) + (a.bias ? (double)__ldg(a.bias + e) : 0.0)
-                                           : -INFINITY;
+    const float l = clean(to_f(row[e]));
+    c[j] = plain || !(l > -INFINITY) ? (double)l
+                                     : score(e) + (a.bias ? (double)__ldg(a.bias + e) : 0.0);
   }
   bool in = true;
   if (a.n_group > 1) {

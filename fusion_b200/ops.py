@@ -444,6 +444,20 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
              topk_group, _p(topw), _p(topi), T, E, k, scale, int(renorm))
 
 
+def clear_holes(y, ids):
+    """Zeros in the rows of y [n, H] (bf16) whose id (int32, n of them) is negative: slots that
+    ``route_topk`` left without an expert, which no product writes."""
+    if y.dtype != torch.bfloat16:
+        raise TypeError("clear_holes: bf16 rows required")
+    ldy = _rows2d(y, "clear_holes: y")
+    if ids.numel() != y.shape[0]:
+        raise ValueError(f"clear_holes: {ids.numel()} ids for {y.shape[0]} rows")
+    _need(ids, torch.int32, "clear_holes: ids")
+    dev = _device_of(y, ids)
+    with torch.cuda.device(dev):
+        L.call("fus_clear_holes", _p(ids), ids.numel(), _p(y), ldy, y.shape[1], _stream())
+
+
 def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
     """Bytes of the scales of `rows` rows; ``tile`` is the dispatch block of a product's rows
     (or 0: row-major)."""

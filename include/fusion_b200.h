@@ -156,15 +156,20 @@ int fus_router_topk_grouped(const float* partial, int nsplit, const float* bias,
  *   n_group > 1: only experts of the topk_group groups (consecutive ids) with the largest
  *   sum of their two largest c may be chosen (ties: lower group; fus_router_topk_grouped
  *   keeps the others with choice 0, this one never chooses them)
- *   ids = top-k of c, descending, ties to the lower id, as exact arithmetic orders them;
- *   w = s[ids]; if renorm: w /= max(sum(w), 1e-20); w *= scale
+ *   ids = top-k of c, descending, ties to the lower id, as 64-bit arithmetic orders them
+ *   (without bias and groups by l itself); w = s[ids]; if renorm: w /= max(sum(w), 1e-20);
+ *   w *= scale
  * A logit of -infinity or NaN masks its expert. Slots without an expert left: id -1 (a hole
- * of fus_moe_align), weight 0. bias [E] fp32 or NULL, finite. */
+ * of fus_moe_align), weight 0; fus_clear_holes zeroes the expert rows that no one writes then.
+ * bias [E] fp32 or NULL, finite. */
 #define FUS_SCORE_SIGMOID 0
 #define FUS_SCORE_SOFTMAX 1
 int fus_route_topk(const void* logits, int dtype, long ld, const float* bias, int score,
                    int n_group, int topk_group, float* topw, int* topi, int T, int E, int topk,
                    float scale, int renorm, void* stream, int* status);
+
+/* y[i] = 0 (H bf16, row stride ldy) for every i < n with ids[i] < 0. H % 8 == 0, 16-byte rows. */
+int fus_clear_holes(const int* ids, int n, void* y, long ldy, int H, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Dispatch layout (glm52/reference.py:85-128 moe_align_block_size, sglang layout):

@@ -120,6 +120,9 @@ def test_without_norms_and_masked_router():
     sorted_ids, eids, ntp = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (T * topk + E * 15, (T * topk + E * 15) // 16, 1))
     cap = sorted_ids.numel() // 16 * 16
     ops.moe_align(topi, E, 16, sorted_ids[:cap], eids, ntp)
+    # rows that nothing writes must not be what memory held: fill the pool with NaN first
+    junk = [torch.full((T * topk, H), float("nan"), dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    del junk
     _, y, _ = blk._experts(x2, topi, (sorted_ids[:cap], eids, ntp), 16)
     finish()
     assert (topi[:, :2].cpu() == torch.tensor([7, 3])).all() and (topi[:, 2:] == -1).all()

@@ -114,6 +114,19 @@ def test_masked_experts_and_empty_rows(score, bias):
         _run(logits, 6, b, score, n_group=groups, topk_group=max(1, groups // 2))
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_scores_that_saturate(score):
+    """Logits whose scores are 1 (or 0) in any precision still rank by themselves, also in rows with
+    more ties than candidates."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    logits = 40 + 20 * torch.randn(40, 256, device="cuda", generator=gen).round()
+    logits[::2] = logits[::2].clamp(0, 60)
+    logits[1::4] -= 2000
+    logits[3] = 40 + torch.arange(256, device="cuda") % 7
+    _run(logits, 8, None, score)
+    _run(logits, 20, None, score, renorm=False)
+
+
 def test_large_bias_and_logits():
     gen = torch.Generator(device="cuda").manual_seed(9)
     logits = 60 * torch.randn(50, 128, device="cuda", generator=gen)

@@ -58,6 +58,22 @@ def test_norm_gate_residual():
     _refused(call(y=None), "null")
 
 
+def test_clear_holes():
+    def call(ids=P, n=4, y=P, ldy=64, H=64):
+        return L.lib().fus_clear_holes(ids, n, y, ldy, H, None)
+
+    assert call(n=0) == 0
+    _refused(call(n=-1), "sizes")
+    _refused(call(H=60), "sizes")
+    _refused(call(y=P + 8), "aligned")
+    _refused(call(ldy=56), "aligned")
+    _refused(call(ids=None), "aligned")
+    with pytest.raises(TypeError):
+        ops.clear_holes(torch.zeros(4, 64), torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        ops.clear_holes(torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32))
+
+
 def test_python_refusals():
     x = torch.zeros(4, 64)
     w, i = torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.int32)
