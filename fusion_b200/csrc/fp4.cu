@@ -46,15 +46,16 @@ FUS_DEVICE void load16(const T* p, bool vec, uint32_t* r) {
 template <typename T>
 FUS_DEVICE uint32_t top16(const uint32_t* r) {
   uint32_t top = 0;
-  if (sizeof(T) == 2) {  // two 16-bit magnitudes at a time
+  if constexpr (sizeof(T) == 2) {  // two 16-bit magnitudes at a time
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = __vmaxu2(top, r[i] & 0x7fff7fffu);
     const uint16_t m = (uint16_t)max(top & 0xffffu, top >> 16);
     return __float_as_uint(to_f(*reinterpret_cast<const T*>(&m)));
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) top = max(top, r[i] & 0x7fffffffu);
-  return top;
+    for (int i = 0; i < 16; ++i) top = max(top, r[i] & 0x7fffffffu);
+    return top;
+  }
 }
 
 // element j, by selection (no indexed registers)
@@ -290,27 +291,27 @@ __global__ void __launch_bounds__(256)
                                      fp4_row_offset(d & (tile - 1))) = word;
       }
     };
-    if (!SPREAD) {
+    if constexpr (!SPREAD) {
       put(p);
-      continue;
-    }
-    // the places of four pairs at a time: their loads do not wait for one another
-    for (int s0 = 0; s0 < id_div; s0 += 4) {
-      int d[4];
-      bool is[4];
+    } else {
+      // the places of four pairs at a time: their loads do not wait for one another
+      for (int s0 = 0; s0 < id_div; s0 += 4) {
+        int d[4];
+        bool is[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int id = p * id_div + s0 + u;
-        is[u] = s0 + u < id_div && id < id_limit;
-        d[u] = is[u] ? __ldg(pos + id) : -1;
+        for (int u = 0; u < 4; ++u) {
+          const int id = p * id_div + s0 + u;
+          is[u] = s0 + u < id_div && id < id_limit;
+          d[u] = is[u] ? __ldg(pos + id) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          is[u] = is[u] && d[u] >= 0 && d[u] < x_rows && d[u] < placed &&
+                  __ldg(ids + d[u]) == p * id_div + s0 + u;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (is[u]) put(d[u]);
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        is[u] = is[u] && d[u] >= 0 && d[u] < x_rows && d[u] < placed &&
-                __ldg(ids + d[u]) == p * id_div + s0 + u;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (is[u]) put(d[u]);
     }
   }
 }
