@@ -627,7 +627,7 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   } else {
     rc = make_tmap_u8_2d(&tw, d->wq, row, rows, row, 128, 128);
   }
-  for (int i = 0; i < 4 && !rc; ++i)
+  for (int i = 0; i < (d->block_n <= 64 ? 1 : 4) && !rc; ++i)
     rc = make_tmap_u8_2d(&tx.m[i], d->xq, row, (uint64_t)d->x_rows, (uint64_t)d->ldxq, 128,
                          d->block_n <= 64 ? d->block_n : 32 * (i + 1));
   if (rc) return rc;

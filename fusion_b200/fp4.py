@@ -16,6 +16,8 @@ import torch
 from . import _lib as L
 from . import ops
 
+_OUT = {torch.bfloat16: 0, torch.float32: 1}  # FUS_DT_* of an output
+
 
 def quantize_weight(w: torch.Tensor, fmt: str):
     """A bf16 / fp16 / fp32 weight stack [E, N, K] in 4 bits, as a checkpoint would hold it:
@@ -81,55 +83,72 @@ class ExpertGemmFP4:
         or fp32; row_scale: fp32, one for each row of out.
 
         Without sorted_ids the one expert multiplies every row: x [T, K], out [T, cols]."""
-        dt, ldx = ops._dtype(x, "x"), ops._rows2d(x, "x")
-        if x.shape[1] != self.K or out.shape[1] != self.cols:
-            raise ValueError(f"x [.., {self.K}] and out [.., {self.cols}] required")
+        dev = self._dev
+        xs, os = x.stride(), out.stride()
+        T, rows = x.shape[0], out.shape[0]
+        dt, odt = ops.DT.get(x.dtype), _OUT.get(out.dtype)
+        if (dt is None or odt is None or x.shape != (T, self.K) or out.shape != (rows, self.cols)
+                or xs[1] != 1 or os[1] != 1 or x.get_device() != dev or out.get_device() != dev
+                or row_scale is not None and (
+                    row_scale.dtype is not torch.float32 or row_scale.numel() < rows
+                    or row_scale.get_device() != dev or not row_scale.is_contiguous())):
+            self._refuse(x, out, row_scale)
+        d = L.Fp4GemmDesc.from_buffer_copy(self._desc)
+        spread = 0
         if sorted_ids is None:
             if self.E != 1 or expert_ids is not None or ntp is not None:
                 raise ValueError("without sorted_ids: one expert, no expert_ids, no ntp")
-            cap = x.shape[0]
+            cap = T
             block_n = block_n or dense_block_n(cap)
             gather = scatter = False
-            spread = 0
         else:
+            for t in (sorted_ids, expert_ids, ntp):
+                if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+                    ops._need(t, torch.int32, "sorted_ids, expert_ids and ntp")
+                    raise ValueError(f"tensors must be on {self.device}, with the weights")
             cap = sorted_ids.numel()
-            if gather:
-                pairs = x.shape[0] * topk
-            elif scatter and pairs is None:
-                pairs = out.shape[0]
-            if pairs is None:
-                raise ValueError("rows in and out in dispatch order: pairs (T * topk) required")
             if block_n < 1 or cap % block_n or expert_ids.numel() < cap // block_n:
                 raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each")
-            for t, what in ((sorted_ids, "sorted_ids"), (expert_ids, "expert_ids"), (ntp, "ntp")):
-                ops._need(t, torch.int32, what)
-            spread = 4 * pairs if gather else 0
-        if out.shape[0] < (pairs if scatter else cap) or (not gather and x.shape[0] < cap):
+            if gather:
+                pairs = T * topk
+                spread = 4 * pairs
+            elif pairs is None:
+                if not scatter:
+                    raise ValueError("rows in and out in dispatch order: pairs (T * topk) required")
+                pairs = rows
+            d.expert_ids, d.ntp = expert_ids.data_ptr(), ntp.data_ptr()
+            d.live_ids, d.live_limit, d.scatter = sorted_ids.data_ptr(), pairs, scatter
+        if rows < (pairs if scatter else cap) or not gather and T < cap:
             raise ValueError("too few rows")
-        if out.dtype not in (torch.bfloat16, torch.float32):
+        # the packed rows: fresh for each call, so calls on other streams and captured graphs
+        # never share them
+        packed = cap * d.ldxq
+        size = packed + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n)
+        ws = torch.empty(size + spread, dtype=torch.uint8, device=self.device).data_ptr()
+        d.xq, d.xsf = ws, ws + packed
+        d.x_rows, d.block_n = cap, block_n
+        if row_scale is not None:
+            d.row_scale = row_scale.data_ptr()
+        d.out, d.ldo = out.data_ptr(), os[0] if rows > 1 else self.cols
+        d.out_rows, d.out_dtype = rows, odt
+        ops._call_on(dev, "fus_fp4_expert_gemm", C.byref(d), x.data_ptr(), dt,
+                     xs[0] if T > 1 else self.K, T, topk if gather else 0,
+                     ws + size if spread else None)
+        return out
+
+    def _refuse(self, x, out, row_scale) -> None:
+        ops._dtype(x, "x")
+        if out.dtype not in _OUT:
             raise TypeError("out is bf16 or fp32")
+        if x.shape != (len(x), self.K) or out.shape != (len(out), self.cols):
+            raise ValueError(f"x [.., {self.K}] and out [.., {self.cols}] required")
+        ops._rows2d(x, "x")
+        ops._rows2d(out, "out")
         ops._need(row_scale, torch.float32, "row_scale")
         if row_scale is not None and row_scale.numel() < out.shape[0]:
             raise ValueError("row_scale: one for each row of out")
-        if ops._device_of(x, out, sorted_ids, expert_ids, ntp, row_scale) != self._dev:
+        if ops._device_of(x, out, row_scale) != self._dev:
             raise ValueError(f"tensors must be on {self.device}, with the weights")
-        d = L.Fp4GemmDesc.from_buffer_copy(self._desc)
-        # the packed rows: fresh for each call, so calls on other streams and captured graphs
-        # never share them
-        size = cap * d.ldxq + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n)
-        rows = torch.empty(size + spread, dtype=torch.uint8, device=self.device)
-        d.xq = ops._p(rows)
-        d.xsf = d.xq + cap * d.ldxq
-        d.x_rows, d.block_n = cap, block_n
-        if sorted_ids is not None:
-            d.expert_ids, d.ntp = ops._p(expert_ids), ops._p(ntp)
-            d.live_ids, d.live_limit, d.scatter = ops._p(sorted_ids), pairs, int(scatter)
-        d.row_scale = ops._p(row_scale)
-        d.out, d.ldo = ops._p(out), ops._rows2d(out, "out")
-        d.out_rows, d.out_dtype = out.shape[0], ops.DT[out.dtype]
-        ops._call_on(self._dev, "fus_fp4_expert_gemm", C.byref(d), ops._p(x), dt, ldx,
-                     x.shape[0], topk if gather else 0, d.xq + size if spread else None)
-        return out
 
 
 def dense_block_n(rows: int) -> int:

@@ -322,14 +322,18 @@ def fp8_block_dequant(src, scale, dst, block=(128, 128)):
 
 # -------------------------------------------------------------------------------------
 # operators over tensors of any device: the call runs on that device, on its current stream.
-# At a few tokens the host's work is what a call costs, so the checks read each property of
-# a tensor once and the stream and status word are looked up without building objects.
+# At a few tokens the host's work is what a call costs: each function tests everything it
+# asks of its arguments in one condition, and only a call that fails it goes through the
+# checks that say what is wrong.
 DT = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}  # FUS_DT_*
 FP4_FORMATS = {"mx": 0, "nv": 1}  # FUS_FP4_*
 FP4_BLOCK = {"mx": 32, "nv": 16}  # elements that share a scale
 
+_I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
 _fns: dict = {}
 _status_ptr: dict[int, int] = {}
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -372,7 +376,7 @@ def _device_of(t: torch.Tensor, *others) -> int:
 
 def _call_on(dev: int, name: str, *args) -> None:
     """The entry point with device `dev` current, on its current stream, with its status word."""
-    if dev != torch._C._cuda_getDevice():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             return _call_on(dev, name, *args)
     fn = _fns.get(name)
@@ -381,7 +385,7 @@ def _call_on(dev: int, name: str, *args) -> None:
     status = _status_ptr.get(dev)
     if status is None:
         status = _status_ptr[dev] = status_tensor(dev).data_ptr()
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev), status)
+    rc = fn(*args, _raw_stream(dev), status)
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {L.last_error()}")
 
@@ -396,35 +400,65 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
     [T, N] rows (bf16, fp16 or fp32 throughout). post_w None: y unnormalised; x None: h only.
     gate: [T, 1], [1, N] or [N], or [T, N]; gate_act "none", "sigmoid" or "tanh". h may be res
     or y itself, x may be y."""
-    what = "norm_gate_residual"
-    dt = _dtype(y, what)
-    shape, dtype = y.shape, y.dtype
+    shape, dtype, dev = y.shape, y.dtype, y.get_device()
+    dt = DT.get(dtype)
+    ys, rs, hs = y.stride(), res.stride(), h.stride()
+    if (dt is None or dev < 0 or len(shape) != 2 or ys[1] != 1
+            or res.shape != shape or res.dtype is not dtype or rs[1] != 1 or res.get_device() != dev
+            or h.shape != shape or h.dtype is not dtype or hs[1] != 1 or h.get_device() != dev):
+        _refuse_norm(y, res, h, x, post_w, pre_w, gate)
     T, N = shape
-    for t in (res, h, x):
-        if t is not None and (t.dtype != dtype or t.shape != shape):
-            raise ValueError(f"{what}: res, h and x must have y's type and shape")
-    for w in (post_w, pre_w):
-        _need(w, dtype, "norm_gate_residual: weight", (N,))
-    kind, ldg = 0, 0
+    px = ppre = ppost = pgate = None
+    ldx = ldg = kind = 0
+    if x is not None:
+        if x.shape != shape or x.dtype is not dtype or x.stride()[1] != 1 or x.get_device() != dev:
+            _refuse_norm(y, res, h, x, post_w, pre_w, gate)
+        px, ldx = x.data_ptr(), x.stride()[0] if T > 1 else N
+    if post_w is not None:
+        if (post_w.shape != (N,) or post_w.dtype is not dtype or post_w.get_device() != dev
+                or not post_w.is_contiguous()):
+            _refuse_norm(y, res, h, x, post_w, pre_w, gate)
+        ppost = post_w.data_ptr()
+    if pre_w is not None:
+        if (pre_w.shape != (N,) or pre_w.dtype is not dtype or pre_w.get_device() != dev
+                or not pre_w.is_contiguous()):
+            _refuse_norm(y, res, h, x, post_w, pre_w, gate)
+        ppre = pre_w.data_ptr()
     if gate is not None:
-        if gate.dtype != y.dtype:
-            raise TypeError(f"{what}: gate must have y's type")
+        if gate.dtype is not dtype or gate.get_device() != dev:
+            _refuse_norm(y, res, h, x, post_w, pre_w, gate)
         if gate.dim() == 1:
             gate = gate[None]
-        if gate.shape == (T, N):
-            kind, ldg = 3, _rows2d(gate, f"{what}: gate")
+        what = "norm_gate_residual: gate"
+        if gate.shape == shape:
+            kind, ldg = 3, _rows2d(gate, what)
         elif gate.shape == (1, N):
             kind = 2
-            _rows2d(gate, f"{what}: gate")
+            _rows2d(gate, what)
         elif gate.shape == (T, 1):
             kind, ldg = 1, gate.stride(0)
         else:
-            raise ValueError(f"{what}: gate of shape {tuple(gate.shape)} for {(T, N)}")
-    dev = _device_of(y, res, h, x, post_w, pre_w, gate)
-    _call_on(dev, "fus_norm_gate_residual", _p(y), _rows2d(y, what), _p(res),
-             _rows2d(res, what), _p(post_w), _p(gate), ldg, kind, GATE_ACTS[gate_act], alpha,
-             _p(h), _rows2d(h, what), _p(pre_w), _p(x), _rows2d(x, what) if x is not None else 0,
-             T, N, dt, eps)
+            raise ValueError(f"{what} of shape {tuple(gate.shape)} for {(T, N)}")
+        pgate = gate.data_ptr()
+    one = T <= 1
+    _call_on(dev, "fus_norm_gate_residual", y.data_ptr(), N if one else ys[0], res.data_ptr(),
+             N if one else rs[0], ppost, pgate, ldg, kind, GATE_ACTS[gate_act], alpha, h.data_ptr(),
+             N if one else hs[0], ppre, px, ldx, T, N, dt, eps)
+
+
+def _refuse_norm(y, res, h, x, post_w, pre_w, gate) -> None:
+    what = "norm_gate_residual"
+    _dtype(y, what)
+    for t in (y, res, h, x):
+        if t is not None and (t.dtype != y.dtype or t.shape != y.shape):
+            raise ValueError(f"{what}: res, h and x must have y's type and shape")
+        if t is not None:
+            _rows2d(t, what)
+    for w in (post_w, pre_w):
+        _need(w, y.dtype, f"{what}: weight", (y.shape[1],))
+    if gate is not None and gate.dtype != y.dtype:
+        raise TypeError(f"{what}: gate must have y's type")
+    _device_of(y, res, h, x, post_w, pre_w, gate)
 
 
 def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group: int = 1,
@@ -435,13 +469,22 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
     chosen weights' sum. -inf or NaN logits mask experts; slots left over get id -1, weight 0."""
     T, E = logits.shape
     k = topi.shape[1] if topi.dim() == 2 else 0
-    dt, ld = _dtype(logits, "route_topk"), _rows2d(logits, "route_topk: logits")
-    _need(topi, torch.int32, "route_topk: topi", (T, k))
-    _need(topw, torch.float32, "route_topk: topw", (T, k))
-    _need(bias, torch.float32, "route_topk: bias", (E,))
-    dev = _device_of(logits, topw, topi, bias)
-    _call_on(dev, "fus_route_topk", _p(logits), dt, ld, _p(bias), SCORES[score], n_group,
-             topk_group, _p(topw), _p(topi), T, E, k, scale, int(renorm))
+    st, dt, dev = logits.stride(), DT.get(logits.dtype), logits.get_device()
+    if (dt is None or dev < 0 or st[1] != 1
+            or topi.shape != (T, k) or topi.dtype is not _I32 or topi.get_device() != dev
+            or topw.shape != (T, k) or topw.dtype is not _F32 or topw.get_device() != dev
+            or not topi.is_contiguous() or not topw.is_contiguous()
+            or bias is not None and (bias.shape != (E,) or bias.dtype is not _F32
+                                     or bias.get_device() != dev or not bias.is_contiguous())):
+        _dtype(logits, "route_topk")
+        _rows2d(logits, "route_topk: logits")
+        _need(topi, _I32, "route_topk: topi", (T, k))
+        _need(topw, _F32, "route_topk: topw", (T, k))
+        _need(bias, _F32, "route_topk: bias", (E,))
+        _device_of(logits, topw, topi, bias)
+    _call_on(dev, "fus_route_topk", logits.data_ptr(), dt, st[0] if T > 1 else E,
+             None if bias is None else bias.data_ptr(), SCORES[score], n_group, topk_group,
+             topw.data_ptr(), topi.data_ptr(), T, E, k, scale, renorm)
 
 
 def clear_holes(y, ids):
@@ -470,23 +513,36 @@ def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
     return -(-rows // tile) * -(-K // 256) * (64 // n) * (tile // 128 or 1) * 512
 
 
-def _fp4_args(q, sf, rows: int, K: int, fmt: str, tile: int, gscale, what: str) -> tuple:
+def _refuse_fp4(values, q, sf, rows: int, K: int, fmt: str, tile: int, gscale, ids, ntp,
+                what: str) -> None:
+    _dtype(values, what)
+    _rows2d(values, what)
     if fmt not in FP4_FORMATS:
         raise ValueError(f"{what}: format {fmt!r} not in {sorted(FP4_FORMATS)}")
-    if q.dtype != torch.uint8 or sf.dtype != torch.uint8:
+    if q.dtype != _U8 or sf.dtype != _U8:
         raise TypeError(f"{what}: packed values and scales are uint8")
     if q.shape != (rows, K // 2):
         raise ValueError(f"{what}: packed values of shape {tuple(q.shape)}, not {(rows, K // 2)}")
+    _rows2d(q, what)
     need = fp4_scale_bytes(rows, K, fmt, tile)
     if not sf.is_contiguous() or sf.numel() < need:
         raise ValueError(f"{what}: scales need {need} contiguous bytes")
-    _need(gscale, torch.float32, what)
-    per = 0
-    if gscale is not None:
-        if gscale.numel() < 1 or rows % gscale.numel():
-            raise ValueError(f"{what}: {gscale.numel()} factors for {rows} rows")
-        per = rows // gscale.numel() if gscale.numel() > 1 else 0
-    return _rows2d(q, what), per
+    _need(gscale, _F32, what)
+    if ids is not None:
+        _need(ids, _I32, f"{what}: ids", (rows,))
+    _need(ntp, _I32, f"{what}: ntp")
+    _device_of(values, q, sf, gscale, ids, ntp)
+
+
+def _factors(gscale, rows: int, dev: int, what: str) -> tuple:
+    """Address of the factors and rows that share one (0: all)."""
+    if gscale.dtype is not _F32 or gscale.get_device() != dev or not gscale.is_contiguous():
+        _need(gscale, _F32, what)
+        raise ValueError(f"{what}: factors on another device")
+    n = gscale.numel()
+    if n < 1 or rows % n:
+        raise ValueError(f"{what}: {n} factors for {rows} rows")
+    return gscale.data_ptr(), rows // n if n > 1 else 0
 
 
 def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, id_div: int = 1,
@@ -495,25 +551,36 @@ def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, 
     (``fp4_scale_bytes``). ``fmt`` "mx" or "nv"; gscale (nv): fp32 factors, one or one for each
     equal run of rows. With ``ids`` (int32, one for each row of q) row p is x[ids[p] // id_div];
     rows whose id is not in [0, id_limit) keep what they held, as do rows from ntp[0] on."""
-    dt, ldx = _dtype(x, "fp4_quantize"), _rows2d(x, "fp4_quantize: x")
-    K, rows = x.shape[1], q.shape[0]
-    dev = _device_of(x, q, sf, gscale, ids, ntp)
-    ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_quantize")
-    if ids is not None:
-        _need(ids, torch.int32, "fp4_quantize: ids", (rows,))
-    _need(ntp, torch.int32, "fp4_quantize: ntp")
-    _call_on(dev, "fus_fp4_quantize", _p(x), dt, ldx, x.shape[0], K, FP4_FORMATS[fmt],
-             _p(gscale), per, _p(ids), id_div, id_limit, _p(ntp), rows, tile, _p(q), ldq, _p(sf))
+    R, K = x.shape
+    rows = q.shape[0]
+    xs, qs, dt, dev = x.stride(), q.stride(), DT.get(x.dtype), x.get_device()
+    if (dt is None or dev < 0 or xs[1] != 1 or fmt not in FP4_FORMATS
+            or q.shape != (rows, K // 2) or qs[1] != 1 or q.dtype is not _U8 or q.get_device() != dev
+            or sf.dtype is not _U8 or sf.get_device() != dev or not sf.is_contiguous()
+            or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile)
+            or ids is not None and (ids.dtype is not _I32 or ids.shape != (rows,)
+                                    or ids.get_device() != dev or not ids.is_contiguous())
+            or ntp is not None and (ntp.dtype is not _I32 or ntp.get_device() != dev)):
+        _refuse_fp4(x, q, sf, rows, K, fmt, tile, gscale, ids, ntp, "fp4_quantize")
+    g, per = (None, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_quantize")
+    _call_on(dev, "fus_fp4_quantize", x.data_ptr(), dt, xs[0] if R > 1 else K, R, K,
+             FP4_FORMATS[fmt], g, per, None if ids is None else ids.data_ptr(), id_div, id_limit,
+             None if ntp is None else ntp.data_ptr(), rows, tile, q.data_ptr(),
+             qs[0] if rows > 1 else K // 2, sf.data_ptr())
 
 
 def fp4_dequantize(q, sf, out, fmt: str, *, tile: int = 128, gscale=None):
     """The values of packed rows: out [rows, K] (bf16, fp16 or fp32) = q * scale (* factor)."""
-    dt, ldo = _dtype(out, "fp4_dequantize"), _rows2d(out, "fp4_dequantize: out")
     rows, K = out.shape
-    dev = _device_of(out, q, sf, gscale)
-    ldq, per = _fp4_args(q, sf, rows, K, fmt, tile, gscale, "fp4_dequantize")
-    _call_on(dev, "fus_fp4_dequantize", _p(q), ldq, _p(sf), FP4_FORMATS[fmt], tile, rows, K,
-             _p(gscale), per, _p(out), dt, ldo)
+    os, qs, dt, dev = out.stride(), q.stride(), DT.get(out.dtype), out.get_device()
+    if (dt is None or dev < 0 or os[1] != 1 or fmt not in FP4_FORMATS
+            or q.shape != (rows, K // 2) or qs[1] != 1 or q.dtype is not _U8 or q.get_device() != dev
+            or sf.dtype is not _U8 or sf.get_device() != dev or not sf.is_contiguous()
+            or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile)):
+        _refuse_fp4(out, q, sf, rows, K, fmt, tile, gscale, None, None, "fp4_dequantize")
+    g, per = (None, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_dequantize")
+    _call_on(dev, "fus_fp4_dequantize", q.data_ptr(), qs[0] if rows > 1 else K // 2, sf.data_ptr(),
+             FP4_FORMATS[fmt], tile, rows, K, g, per, out.data_ptr(), dt, os[0] if rows > 1 else K)
 
 
 def fp4_pack_scales(scales, fmt: str, gate_up: bool = False) -> torch.Tensor:
