@@ -60,6 +60,10 @@ FUS_DEVICE uint4 pack_v(const float* f) {
   return u;
 }
 
+FUS_DEVICE uint4 operator&(const uint4& a, const uint4& b) {
+  return make_uint4(a.x & b.x, a.y & b.y, a.z & b.z, a.w & b.w);
+}
+
 // V elements (16 bytes) from p + i for i in [i0, i0 + V) within [0, N); whole: one load
 template <typename T, int V>
 FUS_DEVICE void load_v(const T* p, int i0, int N, bool whole, float* f) {
@@ -113,6 +117,32 @@ FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, const float* f) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if (i0 + j >= 0 && i0 + j < N) p[i0 + j] = from_f<T>(f[j]);
+  }
+}
+
+// The 16-byte line at p, of which elements [lo, hi) belong to the row (lo == 0 or hi == V): at
+// most three stores. One warp has an end of the row and its CTA's next barrier waits for it.
+template <typename T, int V>
+FUS_DEVICE void store_end(T* p, int lo, int hi, const uint4& u) {
+  if (sizeof(T) == 4) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j >= lo && j < hi) reinterpret_cast<uint32_t*>(p)[j] = w[j];
+    return;
+  }
+  uint16_t* q = reinterpret_cast<uint16_t*>(p);
+  if (lo > 0) {  // half, word, two words
+    const uint32_t w = lo & 4 ? (lo & 2 ? u.w : u.z) : (lo & 2 ? u.y : u.x);
+    if (lo & 1) q[lo] = (uint16_t)(w >> 16);
+    const int up = lo + (lo & 1);
+    if ((up & 3) == 2) *reinterpret_cast<uint32_t*>(q + up) = up == 2 ? u.y : u.w;
+    if (up <= 4) *reinterpret_cast<uint2*>(q + 4) = make_uint2(u.z, u.w);
+  } else {  // two words, word, half
+    if (hi & 4) *reinterpret_cast<uint2*>(q) = make_uint2(u.x, u.y);
+    if (hi & 2) *reinterpret_cast<uint32_t*>(q + (hi & 4)) = hi & 4 ? u.z : u.x;
+    const uint32_t w = hi & 4 ? (hi & 2 ? u.w : u.z) : (hi & 2 ? u.y : u.x);
+    if (hi & 1) q[hi - 1] = (uint16_t)w;
   }
 }
 
@@ -207,8 +237,11 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
 // start alike and the weights are shifted once. What lines hold beside the row is its
 // neighbours', never used; the first row's first line and the last row's last are not copied
 // where they reach past the tensor: those few elements are loaded one by one.
-constexpr int kRingRows = 4 * 148;
-constexpr int kRingLines = 192;  // narrower rows (1101 fp16 by 2443: 11 us) lose here (15 us)
+// Rows that use it: four for an SM of 192 lines or more; narrower ones, to 64 lines, once there are
+// 14 for an SM (fp16, ring against not: 2443 x 521 8.7 and 11.9 us, 8192 x 1021 26.6 and 48.6;
+// but 1200 x 1504 6.5 and 5.1, 8192 x 256 9.0 and 7.2).
+constexpr int kRingRows = 4 * 148, kRingLines = 192;
+constexpr int kNarrowRows = 14 * 148, kNarrowLines = 64;
 constexpr int kRingThreads = 256;  // at most
 
 template <typename T, bool FULL, bool SHIFT>
@@ -218,6 +251,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
   __shared__ float red[2][32];
   __shared__ uint64_t bars[8];
   __shared__ volatile int abort_flag;
+  __shared__ __align__(16) uint4 inside[2];  // SHIFT: ones where the row's first, last line hold it
   extern __shared__ __align__(16) uint8_t ring[];  // stages x (y | res | gate)
   const int N = a.N, nt = blockDim.x;
   const int lines = (N + V - 1) / V + (SHIFT ? 1 : 0);  // at most, of a row
@@ -229,12 +263,17 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     abort_flag = 0;
     fence_mbar_init();
   }
-  __syncthreads();
   // elements of a row's first line before the row, the same for all of this CTA's rows
   const int off = SHIFT ? (int)((reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(a.y) +
                                                              blockIdx.x * a.ldy) & 15) / sizeof(T))
                         : 0;
   const int row_lines = (N + off + V - 1) / V;
+  if (SHIFT && threadIdx.x < 32) {  // each byte
+    const int end = threadIdx.x >> 4, j = (threadIdx.x & 15) / (int)sizeof(T);
+    const bool in = end == 0 ? j >= off : j < N + off - (row_lines - 1) * V;
+    reinterpret_cast<uint8_t*>(inside)[threadIdx.x] = in ? 0xff : 0;
+  }
+  __syncthreads();
   auto load_row = [&](long t, int s) {
     const uint64_t pol = policy_evict_first();
     const int l0 = SHIFT && t == 0 && off > 0;
@@ -258,6 +297,14 @@ __global__ void __launch_bounds__(kRingThreads, 2)
   // first element of this thread's line v, negative before the row
   auto first = [&](int v) { return ((int)threadIdx.x + v * nt) * V - off; };
   auto whole = [&](int i) { return !SHIFT || (i >= 0 && i + V <= N); };
+  // not kept in L2 for long (8192 x 6144 bf16: 76 -> 69 us)
+  auto put = [&](T* p, int i, const float* f) {
+    const uint4 u = pack_v<T, V>(f);
+    if (whole(i))
+      __stcs(reinterpret_cast<uint4*>(p + i), u);
+    else
+      store_end<T, V>(p + i, i < 0 ? -i : 0, N - i < V ? N - i : V, u);
+  };
   // post_w times a channel gate, and pre_w, of this thread's elements
   float post[VPT][V];
   uint4 pre[VPT];
@@ -309,21 +356,23 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         r[v] = sr[l];
         if (FULL) g[v] = sg[l];
         if (SHIFT && !whole(i)) {
-          // an end of the row: zeros outside it, and what was not copied (see above)
-          const bool load = (i < 0 && t == 0) || (i + V > N && t == rows - 1);
-          T* e = reinterpret_cast<T*>(&u);
-          T* er = reinterpret_cast<T*>(&r[v]);
-          T* eg = reinterpret_cast<T*>(&g[v]);
+          // an end of the row: what was not copied (see above), and zeros outside the row
+          if ((i < 0 && t == 0) || (i + V > N && t == rows - 1)) {
+            T* e = reinterpret_cast<T*>(&u);
+            T* er = reinterpret_cast<T*>(&r[v]);
+            T* eg = reinterpret_cast<T*>(&g[v]);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            if (i + j < 0 || i + j >= N) {
-              e[j] = er[j] = eg[j] = from_f<T>(0.f);
-            } else if (load) {
-              e[j] = (reinterpret_cast<const T*>(a.y) + t * a.ldy)[i + j];
-              er[j] = (reinterpret_cast<const T*>(a.res) + t * a.ldr)[i + j];
-              if (FULL) eg[j] = (reinterpret_cast<const T*>(a.gate) + t * a.ldg)[i + j];
-            }
+            for (int j = 0; j < V; ++j)
+              if (i + j >= 0 && i + j < N) {
+                e[j] = (reinterpret_cast<const T*>(a.y) + t * a.ldy)[i + j];
+                er[j] = (reinterpret_cast<const T*>(a.res) + t * a.ldr)[i + j];
+                if (FULL) eg[j] = (reinterpret_cast<const T*>(a.gate) + t * a.ldg)[i + j];
+              }
           }
+          const uint4 in = inside[i >= 0];
+          u = u & in;
+          r[v] = r[v] & in;
+          if (FULL) g[v] = g[v] & in;
         }
       }
       unpack_v<T, V>(u, f[v]);
@@ -356,7 +405,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
         f[v][j] = w[j] + scale * f[v][j];
         sh += f[v][j] * f[v][j];
       }
-      if (i < N) store_v<T, V>(h, i, N, whole(i), f[v]);
+      if (i < N) put(h, i, f[v]);
     }
     if (!a.x) continue;
     sh = cta_sum(sh, red[1]);
@@ -369,7 +418,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
       unpack_v<T, V>(pre[v], w);
 #pragma unroll
       for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
-      if (i < N) store_v<T, V>(x, i, N, whole(i), w);
+      if (i < N) put(x, i, w);
     }
   }
 }
@@ -427,7 +476,8 @@ int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
   // the ring: some rows for each CTA, rows of some lines, two stages at least
   const bool shift = mode != 0 || a.N % V != 0;
   const int lines = (a.N + V - 1) / V + (shift ? 1 : 0);
-  if (mode < 2 && rows >= kRingRows && lines >= kRingLines && lines <= 3 * kRingThreads) {
+  if (mode < 2 && lines <= 3 * kRingThreads &&
+      ((rows >= kRingRows && lines >= kRingLines) || (rows >= kNarrowRows && lines >= kNarrowLines))) {
     const int threads = (lines + 95) / 96 * 32;
     const int stage = lines * 16 * (a.gate_kind == 3 ? 3 : 2);
     int stages = 216 * 1024 / (2 * kRingThreads / threads) / stage;

@@ -83,6 +83,33 @@ def test_many_rows(dtype, kind, act, T, N):
     assert torch.equal(r2, h) and torch.equal(y2, x)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("kind,act", [("none", "none"), ("channel", "tanh"), ("full", "sigmoid")])
+@pytest.mark.parametrize("T,N", [(2071, 521), (2072, 505), (2072, 512), (3001, 1021), (2503, 259), (2200, 253)])
+def test_many_narrow_rows(dtype, kind, act, T, N):
+    test_many_rows(dtype, kind, act, T, N)
+
+
+@pytest.mark.parametrize("ld,first", [(523, 0), (524, 1), (525, 2), (526, 3), (527, 4), (528, 5), (529, 6), (530, 7)])
+@pytest.mark.parametrize("N", [515, 521, 523])
+def test_every_end_of_a_row(N, ld, first):
+    """Rows that start and end at every place of a 16-byte line; what lies beside them stays."""
+    T = 2080
+    y0, res0, post_w, pre_w, _ = _make(T, N, torch.float16, "none")
+    bufs = [torch.full((first + T * ld,), 5.0, dtype=torch.float16, device="cuda") for _ in range(4)]
+    y, res, h, x = (b[first:].as_strided((T, N), (ld, 1)) for b in bufs)
+    y.copy_(y0), res.copy_(res0)
+    ops.norm_gate_residual(y, res, h, x, post_w=post_w, pre_w=pre_w)
+    finish()
+    wh, wx, mag = _oracle(y0, res0, post_w, pre_w, None, "none", 1.0, np.float32(1e-5))
+    _check(h, wh, mag, torch.float16, N)
+    _check(x, wx, np.abs(wx) + mag, torch.float16, N)
+    for b, got in ((bufs[2], h), (bufs[3], x)):
+        gone = b.clone()
+        gone[first:].as_strided((T, N), (ld, 1)).fill_(5.0)
+        assert bool((gone == 5.0).all())
+
+
 def test_many_rows_apart():
     """Strided rows through the ring: what lies between them is neither read nor written."""
     T, N, ld = 640, 1501, 1533
