@@ -202,9 +202,9 @@ __global__ void __launch_bounds__(256)
   const int p0 = blockIdx.x * blockDim.y * iters + threadIdx.y;
   constexpr int W = 8 * sizeof(T) / 2;
   constexpr int HALF = W / 2;
-  // MX: the row after the one at work is on its way (24.8 -> 22.9 us at 8192 x 6144). NV needs the
-  // registers for occupancy instead (48.4 -> 40 us from fp32).
-  constexpr bool kAhead = FMT == FUS_FP4_MX;
+  // The row after the one at work is on its way (8192 x 6144 bf16: MX 24.8 -> 22.9 us, NV 36 -> 34).
+  // NV from fp32 needs those registers for occupancy instead (48.4 -> 40 us).
+  constexpr bool kAhead = FMT == FUS_FP4_MX || sizeof(T) == 2;
   uint32_t next[W];
   bool next_live = false;
   auto fetch = [&](int p) {
