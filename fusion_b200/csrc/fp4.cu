@@ -74,20 +74,25 @@ FUS_DEVICE float pick16(const uint32_t* r, int j) {
   return to_f(*reinterpret_cast<const T*>(v));
 }
 
-// eight e2m1 codes of f * m, the first in the low four bits
+// eight e2m1 codes of f * m, the first in the low four bits; two products an instruction
 template <typename T>
 FUS_DEVICE uint32_t cvt8(const uint32_t* r, float m) {
   const T* f = reinterpret_cast<const T*>(r);
   uint32_t v;
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t.reg .b64 s, p;\n\t.reg .f32 lo, hi;\n\t"
+      "mov.b64 s, {%9, %9};\n\t"
+      "mov.b64 p, {%1, %2};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {lo, hi}, p;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, hi, lo;\n\t"
+      "mov.b64 p, {%3, %4};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {lo, hi}, p;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, hi, lo;\n\t"
+      "mov.b64 p, {%5, %6};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {lo, hi}, p;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, hi, lo;\n\t"
+      "mov.b64 p, {%7, %8};\n\tmul.rn.f32x2 p, p, s;\n\tmov.b64 {lo, hi}, p;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, hi, lo;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(v)
-      : "f"(to_f(f[0]) * m), "f"(to_f(f[1]) * m), "f"(to_f(f[2]) * m), "f"(to_f(f[3]) * m),
-        "f"(to_f(f[4]) * m), "f"(to_f(f[5]) * m), "f"(to_f(f[6]) * m), "f"(to_f(f[7]) * m));
+      : "f"(to_f(f[0])), "f"(to_f(f[1])), "f"(to_f(f[2])), "f"(to_f(f[3])), "f"(to_f(f[4])),
+        "f"(to_f(f[5])), "f"(to_f(f[6])), "f"(to_f(f[7])), "f"(m));
   return v;
 }
 
