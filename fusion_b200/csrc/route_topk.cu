@@ -190,17 +190,17 @@ struct ExactRow {
   }
 };
 
-// rank of this lane's group among the groups
+// rank of this lane's group among the groups. `in`: this lane's experts that may be one of its two
+// largest (bit j for expert j), `l` their logits.
 template <typename T>
 __device__ __noinline__ int group_rank_exact(const RouteArgs& a, const T* row, float top, int e0,
-                                             int n, int group) {
+                                             int n, int group, uint32_t in, const float* l) {
   const ExactRow x(a, row, e0, n, top);
   double a1 = -INFINITY, a2 = -INFINITY;
-#pragma unroll 1
-  for (int j = 0; j < n; ++j) {
-    const float l = clean(to_f(row[e0 + j]));
-    if (!(l > -INFINITY)) continue;
-    const double v = x.score(l) + (a.bias ? (double)__ldg(a.bias + e0 + j) : 0.0);
+  for (; in; in &= in - 1) {
+    const int j = __ffs(in) - 1;
+    if (!(l[j] > -INFINITY)) continue;
+    const double v = x.score(l[j]) + (a.bias ? (double)__ldg(a.bias + e0 + j) : 0.0);
     a2 = fmax(a2, fmin(a1, v));
     a1 = fmax(a1, v);
   }
@@ -235,7 +235,7 @@ __device__ __noinline__ int rank_exact(const RouteArgs& a, const T* row, float t
 }
 
 template <typename T, int NPL, bool SOFTMAX, bool GROUPED>
-__global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const __grid_constant__ RouteArgs a) {
   __shared__ __align__(16) float row_c[kWarps][NPL * 32], row_l[kWarps][NPL * 32];  // lane-major
   __shared__ unsigned long long cand[kWarps][32];  // choice (ordered) and id (lower is larger)
   __shared__ float sorted[kWarps][33];
@@ -326,34 +326,43 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const RouteArgs
     }
     best = a1;
     second = a2;
-    for (int o = 1; o < a.lpg; o <<= 1) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      if (o >= a.lpg) break;
       const float b1 = __shfl_xor_sync(kAll, a1, o), b2 = __shfl_xor_sync(kAll, a2, o);
       a2 = fmaxf(fminf(a1, b1), fmaxf(a2, b2));
       a1 = fmaxf(a1, b1);
     }
     const float g = a2 > -INFINITY ? a1 + a2 : a1;
-    // each lane of a group compares with its share of the others
-    int better = 0;
-    const int sub = lane & (a.lpg - 1);
-    for (int q0 = 0; q0 < a.n_group; q0 += a.lpg) {
-      const int q = q0 + sub;
-      const float og = __shfl_sync(kAll, g, q << a.lpg_log2);
-      better += q < a.n_group && (og > g || (og == g && q < group));
-    }
-    for (int o = 1; o < a.lpg; o <<= 1) better += __shfl_xor_sync(kAll, better, o);
     if (a.topk_group < a.n_group) {
-      // the last group in and the first one out: too near to tell apart in fp32?
-      const bool real = group < a.n_group;
-      const int in = __ffs(__ballot_sync(kAll, real && better == a.topk_group - 1)) - 1;
-      const int out = __ffs(__ballot_sync(kAll, real && better == a.topk_group)) - 1;
-      const float gi = __shfl_sync(kAll, g, in), go = __shfl_sync(kAll, g, out);
-      if (gi - go <= 2.f * tol * (1.f + fabsf(gi)))
-        better = group_rank_exact<T>(a, row, top, e0, n, group);
-    }
-    if (better >= a.topk_group) {
-      best = second = -INFINITY;
+      // the best groups leave one by one; equal ones leave together and are too many then
+      const uint32_t gkey = group < a.n_group ? key_of(g) : 0;
+      uint32_t mine = gkey, last = 0;
+#pragma unroll 4
+      for (int s = 0; s < a.topk_group; ++s) {
+        last = __reduce_max_sync(kAll, mine);
+        if (mine == last) mine = 0;
+      }
+      bool in = mine != gkey;
+      const float gi = value_of(last), go = value_of(__reduce_max_sync(kAll, mine));
+      // too near to tell apart in fp32? (no group left: go is a NaN)
+      if (gi - go <= 2.f * tol * (1.f + fabsf(gi)) ||
+          __popc(__ballot_sync(kAll, in)) != a.topk_group << a.lpg_log2) {
+        const float from = second - tol * (1.f + fabsf(second));
+        uint32_t two = 0;
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) c[j] = -INFINITY;
+        for (int j = 0; j < NPL; ++j) {
+          two |= j < n && !(c[j] < from) ? 1u << j : 0u;
+          row_l[warp][lane * NPL + j] = l[j];
+        }
+        in = group_rank_exact<T>(a, row, top, e0, n, group, two, &row_l[warp][lane * NPL]) <
+             a.topk_group;
+      }
+      if (!in) {
+        best = second = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) c[j] = -INFINITY;
+      }
     }
   } else {
     best = c[0];
