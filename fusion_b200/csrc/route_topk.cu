@@ -432,11 +432,12 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const __grid_co
     id = (GROUPED ? (from >> a.lpg_log2) * a.gsz + (from & (a.lpg - 1)) * NPL : from * NPL) + at % NPL;
   }
   const unsigned long long key = (unsigned long long)key_of(choice) << 32 | (uint32_t)~id;
-  if (lane < count) cand[warp][lane] = key;
+  cand[warp][lane] = lane < count ? key : 0;  // the same trips for all lanes: zeros outrank nobody
   __syncwarp();
   int rank = 0;
+  const unsigned long long* other = &cand[warp][lane / W];
 #pragma unroll 4
-  for (int q = lane / W; q < count; q += 32 / W) rank += cand[warp][q] > key;
+  for (int q = 0; q < count; q += 32 / W) rank += other[q] > key;
   for (int o = W; o < 32; o <<= 1) rank += __shfl_xor_sync(kAll, rank, o);
   if (!plain) {
     // neighbours in the order, the first one out among them, too near to tell apart?
