@@ -480,7 +480,8 @@ int launch_norm(const NormArgs& a, int rows, cudaStream_t st, int* status) {
       ((rows >= kRingRows && lines >= kRingLines) || (rows >= kNarrowRows && lines >= kNarrowLines))) {
     const int threads = (lines + 95) / 96 * 32;
     const int stage = lines * 16 * (a.gate_kind == 3 ? 3 : 2);
-    int stages = 216 * 1024 / (2 * kRingThreads / threads) / stage;
+    // all of an SM's CTAs resident at once: each has 1 KB reserved and some 400 bytes static beside
+    int stages = (222 * 1024 / (2 * kRingThreads / threads) - 1536) / stage;
     if (stages > 8) stages = 8;
     if (stages >= 2) return launch_ring_of<T>(a, rows, threads, stages, stages * stage, shift, st, status);
   }
