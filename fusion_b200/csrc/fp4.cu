@@ -516,7 +516,7 @@ extern "C" int fus_fp4_quantize(const void* x, int dtype, long ldx, int x_rows, 
                                 int id_limit, const int* ntp, long rows, int tile, void* q,
                                 long ldq, void* sf, void* stream, int* status) {
   if (int rc = check_common("fp4_quantize", fmt, dtype, rows, K, tile)) return rc;
-  if (rows == 0) return FUS_OK;
+  if (rows == 0 || (ids && id_div > 0 && id_limit == 0)) return FUS_OK;  // no live row
   if (!x || !q || !sf) return set_error(FUS_E_INVALID, "fp4_quantize: null pointer");
   if (x_rows < 1 || ldx < K || ldx > 0x7fffffffL) return set_error(FUS_E_INVALID, "fp4_quantize: bad source rows");
   if (!ids && rows > x_rows)

@@ -101,14 +101,19 @@ class ExpertGemmFP4:
             cap = T
             block_n = block_n or dense_block_n(cap)
             gather = scatter = False
+            if max(T, rows) > ops.INT_MAX:
+                raise ValueError("too many rows")
         else:
             for t in (sorted_ids, expert_ids, ntp):
                 if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
                     ops._need(t, torch.int32, "sorted_ids, expert_ids and ntp")
                     raise ValueError(f"tensors must be on {self.device}, with the weights")
             cap = sorted_ids.numel()
-            if block_n < 1 or cap % block_n or expert_ids.numel() < cap // block_n:
-                raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each")
+            if block_n < 1 or cap % block_n or expert_ids.numel() < cap // block_n or ntp.numel() < 1:
+                raise ValueError("sorted_ids must hold whole blocks, expert_ids one id for each, "
+                                 "ntp the padded total")
+            if topk < 1 or pairs is not None and pairs < 0:
+                raise ValueError(f"topk={topk}, pairs={pairs} not possible")
             if gather:
                 pairs = T * topk
                 spread = 4 * pairs
@@ -116,6 +121,10 @@ class ExpertGemmFP4:
                 if not scatter:
                     raise ValueError("rows in and out in dispatch order: pairs (T * topk) required")
                 pairs = rows
+            if max(cap, rows, pairs) > ops.INT_MAX:
+                raise ValueError("too many rows")
+            if pairs == 0:
+                return out
             d.expert_ids, d.ntp = expert_ids.data_ptr(), ntp.data_ptr()
             d.live_ids, d.live_limit, d.scatter = sorted_ids.data_ptr(), pairs, scatter
         if rows < (pairs if scatter else cap) or not gather and T < cap:

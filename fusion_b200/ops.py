@@ -330,6 +330,7 @@ FP4_FORMATS = {"mx": 0, "nv": 1}  # FUS_FP4_*
 FP4_BLOCK = {"mx": 32, "nv": 16}  # elements that share a scale
 
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
+INT_MAX = 0x7FFFFFFF  # row counts and widths are C ints
 _fns: dict = {}
 _status_ptr: dict[int, int] = {}
 _current_device = torch._C._cuda_getDevice
@@ -403,7 +404,7 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
     shape, dtype, dev = y.shape, y.dtype, y.get_device()
     dt = DT.get(dtype)
     ys, rs, hs = y.stride(), res.stride(), h.stride()
-    if (dt is None or dev < 0 or len(shape) != 2 or ys[1] != 1
+    if (dt is None or dev < 0 or len(shape) != 2 or max(shape) > INT_MAX or ys[1] != 1
             or res.shape != shape or res.dtype is not dtype or rs[1] != 1 or res.get_device() != dev
             or h.shape != shape or h.dtype is not dtype or hs[1] != 1 or h.get_device() != dev):
         _refuse_norm(y, res, h, x, post_w, pre_w, gate)
@@ -449,6 +450,8 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
 def _refuse_norm(y, res, h, x, post_w, pre_w, gate) -> None:
     what = "norm_gate_residual"
     _dtype(y, what)
+    if max(y.shape, default=0) > INT_MAX:
+        raise ValueError(f"{what}: {tuple(y.shape)} is too large")
     for t in (y, res, h, x):
         if t is not None and (t.dtype != y.dtype or t.shape != y.shape):
             raise ValueError(f"{what}: res, h and x must have y's type and shape")
@@ -470,13 +473,15 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
     T, E = logits.shape
     k = topi.shape[1] if topi.dim() == 2 else 0
     st, dt, dev = logits.stride(), DT.get(logits.dtype), logits.get_device()
-    if (dt is None or dev < 0 or st[1] != 1
+    if (dt is None or dev < 0 or T > INT_MAX or E > INT_MAX or st[1] != 1
             or topi.shape != (T, k) or topi.dtype is not _I32 or topi.get_device() != dev
             or topw.shape != (T, k) or topw.dtype is not _F32 or topw.get_device() != dev
             or not topi.is_contiguous() or not topw.is_contiguous()
             or bias is not None and (bias.shape != (E,) or bias.dtype is not _F32
                                      or bias.get_device() != dev or not bias.is_contiguous())):
         _dtype(logits, "route_topk")
+        if max(T, E) > INT_MAX:
+            raise ValueError(f"route_topk: {(T, E)} is too large")
         _rows2d(logits, "route_topk: logits")
         _need(topi, _I32, "route_topk: topi", (T, k))
         _need(topw, _F32, "route_topk: topw", (T, k))
@@ -516,6 +521,8 @@ def fp4_scale_bytes(rows: int, K: int, fmt: str, tile: int = 128) -> int:
 def _refuse_fp4(values, q, sf, rows: int, K: int, fmt: str, tile: int, gscale, ids, ntp,
                 what: str) -> None:
     _dtype(values, what)
+    if max(rows, *values.shape) > INT_MAX:
+        raise ValueError(f"{what}: {tuple(values.shape)} is too large")
     _rows2d(values, what)
     if fmt not in FP4_FORMATS:
         raise ValueError(f"{what}: format {fmt!r} not in {sorted(FP4_FORMATS)}")
@@ -531,6 +538,8 @@ def _refuse_fp4(values, q, sf, rows: int, K: int, fmt: str, tile: int, gscale, i
     if ids is not None:
         _need(ids, _I32, f"{what}: ids", (rows,))
     _need(ntp, _I32, f"{what}: ntp")
+    if ntp is not None and ntp.numel() < 1:
+        raise ValueError(f"{what}: ntp is empty")
     _device_of(values, q, sf, gscale, ids, ntp)
 
 
@@ -554,17 +563,19 @@ def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, 
     R, K = x.shape
     rows = q.shape[0]
     xs, qs, dt, dev = x.stride(), q.stride(), DT.get(x.dtype), x.get_device()
-    if (dt is None or dev < 0 or xs[1] != 1 or fmt not in FP4_FORMATS
+    if (dt is None or dev < 0 or max(R, K, rows) > INT_MAX or xs[1] != 1 or fmt not in FP4_FORMATS
             or q.shape != (rows, K // 2) or qs[1] != 1 or q.dtype is not _U8 or q.get_device() != dev
             or sf.dtype is not _U8 or sf.get_device() != dev or not sf.is_contiguous()
             or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile)
             or ids is not None and (ids.dtype is not _I32 or ids.shape != (rows,)
                                     or ids.get_device() != dev or not ids.is_contiguous())
-            or ntp is not None and (ntp.dtype is not _I32 or ntp.get_device() != dev)):
+            or ntp is not None and (ntp.dtype is not _I32 or ntp.get_device() != dev
+                                    or ntp.numel() < 1)):
         _refuse_fp4(x, q, sf, rows, K, fmt, tile, gscale, ids, ntp, "fp4_quantize")
     g, per = (None, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_quantize")
     _call_on(dev, "fus_fp4_quantize", x.data_ptr(), dt, xs[0] if R > 1 else K, R, K,
-             FP4_FORMATS[fmt], g, per, None if ids is None else ids.data_ptr(), id_div, id_limit,
+             FP4_FORMATS[fmt], g, per, None if ids is None else ids.data_ptr(), id_div,
+             min(id_limit, INT_MAX),
              None if ntp is None else ntp.data_ptr(), rows, tile, q.data_ptr(),
              qs[0] if rows > 1 else K // 2, sf.data_ptr())
 
@@ -573,7 +584,7 @@ def fp4_dequantize(q, sf, out, fmt: str, *, tile: int = 128, gscale=None):
     """The values of packed rows: out [rows, K] (bf16, fp16 or fp32) = q * scale (* factor)."""
     rows, K = out.shape
     os, qs, dt, dev = out.stride(), q.stride(), DT.get(out.dtype), out.get_device()
-    if (dt is None or dev < 0 or os[1] != 1 or fmt not in FP4_FORMATS
+    if (dt is None or dev < 0 or max(rows, K) > INT_MAX or os[1] != 1 or fmt not in FP4_FORMATS
             or q.shape != (rows, K // 2) or qs[1] != 1 or q.dtype is not _U8 or q.get_device() != dev
             or sf.dtype is not _U8 or sf.get_device() != dev or not sf.is_contiguous()
             or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile)):

@@ -124,3 +124,32 @@ def test_python_refusals():
         ops.fp4_quantize(x, ok[0], ok[1][:8], "mx")
     with pytest.raises(ValueError):
         ops.fp4_quantize(x.T, *ok, "mx")
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Counts are C ints: what would wrap around is refused before anything else is looked at."""
+    huge, wide = torch.zeros(1, 64).expand(2 ** 32, 64), torch.zeros(4, 1).expand(4, 2 ** 32)
+    q, sf = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4096, dtype=torch.uint8)
+    for x in (huge, wide):
+        with pytest.raises(ValueError, match="too large"):
+            ops.fp4_quantize(x, q, sf, "mx")
+        with pytest.raises(ValueError, match="too large"):
+            ops.fp4_dequantize(q, sf, x, "mx")
+        with pytest.raises(ValueError, match="too large"):
+            ops.norm_gate_residual(x, x, x)
+        with pytest.raises(ValueError, match="too large"):
+            ops.route_topk(x, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int32))
+
+
+def test_no_live_rows():
+    """An empty batch has ids (all pads) and no source: nothing to do, nothing refused."""
+    def call(x, x_rows, div, limit):
+        return L.lib().fus_fp4_quantize(x, 0, 64, x_rows, 64, 1, None, 0, P, div, limit, None, 16, 16,
+                                        P, 32, P, None, None)
+
+    assert call(None, 0, 8, 0) == 0 and call(P, 4, 1, 0) == 0
+    _refused(call(None, 0, 8, 8), "null")
+    _refused(call(P, 0, 8, 8), "source rows")
+    with pytest.raises(ValueError, match="ntp"):
+        ops.fp4_quantize(torch.zeros(4, 64), torch.zeros(4, 32, dtype=torch.uint8),
+                         torch.zeros(4096, dtype=torch.uint8), "mx", ntp=torch.zeros(0, dtype=torch.int32))

@@ -330,3 +330,25 @@ def test_large_batch_quantises_tokens_once(fmt):
     proj(xs, want, *dev, bn, gather=False)
     finish()
     assert torch.equal(out, want) and (out[77] == 3.0).all()
+
+
+def test_expert_product_refuses_and_leaves():
+    """No slots, negative pairs, an empty total; an empty batch leaves a longer output as it was."""
+    E, N, K, bn = 2, 64, 64, 16
+    q, s, g, _ = _stack(E, N, K, "nv", 3)
+    proj = fp4.ExpertGemmFP4(q, s, "nv", gscale=g)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    lay = (torch.zeros(16, dtype=torch.int32, device="cuda"), i32(0), i32(16))
+    x = torch.zeros(4, K, dtype=torch.bfloat16, device="cuda")
+    out = torch.full((16, N), 7.0, dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(topk=0), dict(topk=-1), dict(gather=False, pairs=-1)):
+        with pytest.raises(ValueError, match="not possible"):
+            proj(x, out, *lay, bn, **bad)
+    with pytest.raises(ValueError, match="padded total"):
+        proj(x, out, lay[0], lay[1], lay[2][:0], bn, topk=4)
+    proj(x[:0], out, *lay, bn, topk=4)
+    ops.fp4_quantize(x, torch.zeros(16, K // 2, dtype=torch.uint8, device="cuda"),
+                     torch.zeros(ops.fp4_scale_bytes(16, K, "nv", bn), dtype=torch.uint8, device="cuda"),
+                     "nv", tile=bn, ids=lay[0], id_limit=2 ** 40)
+    finish()
+    assert bool((out == 7.0).all())
