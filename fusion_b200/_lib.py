@@ -7,6 +7,7 @@ call raises. Build it with ``python -m fusion_b200.build``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -224,6 +225,11 @@ SIGNATURES: dict[str, tuple] = {
     "fus_fp4_pack_scales": (i32, [vp, i32, i32, i32, i32, i32, vp, vp]),
     "fus_fp4_grouped_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, vp]),
     "fus_fp4_expert_gemm": (i32, [C.POINTER(Fp4GemmDesc), vp, i32, i64, i32, i32, vp, vp, vp]),
+    "fus_norm_gate_residual_packed": (i32, [C.c_char_p]),
+    "fus_route_topk_packed": (i32, [C.c_char_p]),
+    "fus_fp4_quantize_packed": (i32, [C.c_char_p]),
+    "fus_fp4_dequantize_packed": (i32, [C.c_char_p]),
+    "fus_fp4_expert_gemm_packed": (i32, [C.c_char_p]),
     "fus_fold_weight": (i32, [vp, vp, vp, i64, i32, i32, i64, vp, vp]),
     "fus_scale_sum_planes": (i32, [vp, i32, i64, i32, i32, vp, vp, i64, vp, vp]),
     "fus_ep_p2p_decode_forward": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp, vp]),
@@ -258,6 +264,14 @@ def lib() -> C.CDLL:
 def last_error() -> str:
     msg = lib().fus_last_error()
     return msg.decode() if msg else ""
+
+
+def packed(name: str):
+    """The packed form of an entry point and the function that packs its arguments (pointers as
+    integers, 0 for NULL)."""
+    words = struct.Struct("=" + "".join(
+        "d" if t is f32 else "q" if t in (i32, i64) else "Q" for t in SIGNATURES[name][1]))
+    return getattr(lib(), name + "_packed"), words.pack
 
 
 def call(name: str, *args) -> int:

@@ -140,9 +140,9 @@ class ExpertGemmFP4:
             d.row_scale = row_scale.data_ptr()
         d.out, d.ldo = out.data_ptr(), os[0] if rows > 1 else self.cols
         d.out_rows, d.out_dtype = rows, odt
-        ops._call_on(dev, "fus_fp4_expert_gemm", C.byref(d), x.data_ptr(), dt,
+        ops._call_on(dev, "fus_fp4_expert_gemm", C.addressof(d), x.data_ptr(), dt,
                      xs[0] if T > 1 else self.K, T, topk if gather else 0,
-                     ws + size if spread else None)
+                     ws + size if spread else 0)
         return out
 
     def _refuse(self, x, out, row_scale) -> None:

@@ -376,17 +376,18 @@ def _device_of(t: torch.Tensor, *others) -> int:
 
 
 def _call_on(dev: int, name: str, *args) -> None:
-    """The entry point with device `dev` current, on its current stream, with its status word."""
+    """The entry point with device `dev` current, on its current stream, with its status word.
+    Addresses are integers, 0 for none."""
     if dev != _current_device():
         with torch.cuda.device(dev):
             return _call_on(dev, name, *args)
     fn = _fns.get(name)
     if fn is None:
-        fn = _fns[name] = getattr(L.lib(), name)
+        fn = _fns[name] = L.packed(name)
     status = _status_ptr.get(dev)
     if status is None:
         status = _status_ptr[dev] = status_tensor(dev).data_ptr()
-    rc = fn(*args, _raw_stream(dev), status)
+    rc = fn[0](fn[1](*args, _raw_stream(dev), status))
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {L.last_error()}")
 
@@ -409,7 +410,7 @@ def norm_gate_residual(y, res, h, x=None, *, post_w=None, pre_w=None, gate=None,
             or h.shape != shape or h.dtype is not dtype or hs[1] != 1 or h.get_device() != dev):
         _refuse_norm(y, res, h, x, post_w, pre_w, gate)
     T, N = shape
-    px = ppre = ppost = pgate = None
+    px = ppre = ppost = pgate = 0
     ldx = ldg = kind = 0
     if x is not None:
         if x.shape != shape or x.dtype is not dtype or x.stride()[1] != 1 or x.get_device() != dev:
@@ -488,7 +489,7 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
         _need(bias, _F32, "route_topk: bias", (E,))
         _device_of(logits, topw, topi, bias)
     _call_on(dev, "fus_route_topk", logits.data_ptr(), dt, st[0] if T > 1 else E,
-             None if bias is None else bias.data_ptr(), SCORES[score], n_group, topk_group,
+             0 if bias is None else bias.data_ptr(), SCORES[score], n_group, topk_group,
              topw.data_ptr(), topi.data_ptr(), T, E, k, scale, renorm)
 
 
@@ -572,11 +573,11 @@ def fp4_quantize(x, q, sf, fmt: str, *, tile: int = 128, gscale=None, ids=None, 
             or ntp is not None and (ntp.dtype is not _I32 or ntp.get_device() != dev
                                     or ntp.numel() < 1)):
         _refuse_fp4(x, q, sf, rows, K, fmt, tile, gscale, ids, ntp, "fp4_quantize")
-    g, per = (None, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_quantize")
+    g, per = (0, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_quantize")
     _call_on(dev, "fus_fp4_quantize", x.data_ptr(), dt, xs[0] if R > 1 else K, R, K,
-             FP4_FORMATS[fmt], g, per, None if ids is None else ids.data_ptr(), id_div,
+             FP4_FORMATS[fmt], g, per, 0 if ids is None else ids.data_ptr(), id_div,
              min(id_limit, INT_MAX),
-             None if ntp is None else ntp.data_ptr(), rows, tile, q.data_ptr(),
+             0 if ntp is None else ntp.data_ptr(), rows, tile, q.data_ptr(),
              qs[0] if rows > 1 else K // 2, sf.data_ptr())
 
 
@@ -589,7 +590,7 @@ def fp4_dequantize(q, sf, out, fmt: str, *, tile: int = 128, gscale=None):
             or sf.dtype is not _U8 or sf.get_device() != dev or not sf.is_contiguous()
             or sf.numel() < fp4_scale_bytes(rows, K, fmt, tile)):
         _refuse_fp4(out, q, sf, rows, K, fmt, tile, gscale, None, None, "fp4_dequantize")
-    g, per = (None, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_dequantize")
+    g, per = (0, 0) if gscale is None else _factors(gscale, rows, dev, "fp4_dequantize")
     _call_on(dev, "fus_fp4_dequantize", q.data_ptr(), qs[0] if rows > 1 else K // 2, sf.data_ptr(),
              FP4_FORMATS[fmt], tile, rows, K, g, per, out.data_ptr(), dt, os[0] if rows > 1 else K)
 

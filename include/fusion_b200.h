@@ -454,6 +454,15 @@ int fus_fp4_grouped_gemm(const fus_fp4_gemm_desc* d, void* stream, int* status);
 int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, int x_dtype, long ldx,
                         int src_rows, int gather_div, int* pair_ws, void* stream, int* status);
 
+/* Packed forms, for hosts that pay for each argument: `words` holds the arguments of the entry of
+ * the same name in order, eight bytes each: pointers and integers as they are (64-bit), floats
+ * as doubles. An integer that does not fit the entry's type is refused. */
+int fus_norm_gate_residual_packed(const void* words);
+int fus_route_topk_packed(const void* words);
+int fus_fp4_quantize_packed(const void* words);
+int fus_fp4_dequantize_packed(const void* words);
+int fus_fp4_expert_gemm_packed(const void* words);
+
 /* ---------------------------------------------------------------------------------
  * Element-wise / merge kernels
  * ------------------------------------------------------------------------------- */

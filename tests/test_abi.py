@@ -142,3 +142,27 @@ def test_missing_library_fails_loudly(monkeypatch, tmp_path):
         L.lib()
     with pytest.raises(RuntimeError, match="not built"):
         L.call("fus_version")
+
+
+def test_packed_forms():
+    """The packed form of an entry takes the same arguments, and refuses what does not fit."""
+    names = [n for n in _declared() if n.endswith("_packed")]
+    assert len(names) >= 5
+    for name in names:
+        entry = name[: -len("_packed")]
+        fn, pack = L.packed(entry)
+        args = L.SIGNATURES[entry][1]
+        assert len(pack(*[0] * len(args))) == 8 * len(args)
+        ints = [i for i, t in enumerate(args) if t is ctypes.c_int]
+        for i in ints:
+            assert fn(pack(*[2 ** 31 if j == i else 0 for j in range(len(args))])) == -1
+            assert f"argument {i} out of range" in L.last_error()
+        assert fn(None) == -1 and "null words" in L.last_error()
+    # every argument arrives in its place: refusals that name what they got
+    fn, pack = L.packed("fus_route_topk")
+    assert fn(pack(4096, 1, 64, 0, 0, 1, 1, 4096, 4096, 4, 33, 34, 2.5, True, 0, 0)) == -1
+    assert "T=4 E=33 topk=34" in L.last_error()
+    assert fn(pack(4096, 1, 64, 0, 0, 1, 1, 4096, 4096, 0, 64, 8, 2.5, True, 0, 0)) == 0
+    fn, pack = L.packed("fus_fp4_quantize")
+    assert fn(pack(4096, 0, 64, 4, 64, 1, 0, 0, 0, 1, 0, 0, 5, 16, 4096, 32, 4096, 0, 0)) == -1
+    assert "5 rows of 4" in L.last_error()
