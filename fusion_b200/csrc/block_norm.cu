@@ -109,17 +109,6 @@ FUS_DEVICE void load_w(const T* p, int i0, int N, bool whole, int off, float* f)
     for (int j = 0; j < V; ++j) f[j] = i0 + j >= 0 && i0 + j < N ? to_f(p[i0 + j]) : 0.f;
   }
 }
-template <typename T, int V>
-FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, const float* f) {
-  if (whole) {
-    *reinterpret_cast<uint4*>(p + i0) = pack_v<T, V>(f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (i0 + j >= 0 && i0 + j < N) p[i0 + j] = from_f<T>(f[j]);
-  }
-}
-
 // The 16-byte line at p, of which elements [lo, hi) belong to the row (lo == 0 or hi == V): at
 // most three stores. One warp has an end of the row and its CTA's next barrier waits for it.
 template <typename T, int V>
@@ -143,6 +132,20 @@ FUS_DEVICE void store_end(T* p, int lo, int hi, const uint4& u) {
     if (hi & 2) *reinterpret_cast<uint32_t*>(q + (hi & 4)) = hi & 4 ? u.z : u.x;
     const uint32_t w = hi & 4 ? (hi & 2 ? u.w : u.z) : (hi & 2 ? u.y : u.x);
     if (hi & 1) q[hi - 1] = (uint16_t)w;
+  }
+}
+
+// lines: p + i0 starts on 16 bytes
+template <typename T, int V>
+FUS_DEVICE void store_v(T* p, int i0, int N, bool whole, bool lines, const float* f) {
+  if (whole) {
+    *reinterpret_cast<uint4*>(p + i0) = pack_v<T, V>(f);
+  } else if (lines && (i0 >= 0 || i0 + V <= N)) {
+    store_end<T, V>(p + i0, i0 < 0 ? -i0 : 0, N - i0 < V ? N - i0 : V, pack_v<T, V>(f));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i0 + j >= 0 && i0 + j < N) p[i0 + j] = from_f<T>(f[j]);
   }
 }
 
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
       f[v][j] = r[v][j] + scale * f[v][j];
       sh += f[v][j] * f[v][j];
     }
-    store_v<T, V>(h, i, N, whole(i), f[v]);
+    store_v<T, V>(h, i, N, whole(i), MODE == 1, f[v]);
   }
   if (!a.x) return;
   sh = cta_sum(sh, red[1]);
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(1024) norm_gate_residual_kernel(const NormArgs
     load_w<T, V>(reinterpret_cast<const T*>(a.pre_w), i, N, whole(i), off, w);
 #pragma unroll
     for (int j = 0; j < V; ++j) w[j] *= f[v][j] * rstd;
-    store_v<T, V>(x, i, N, whole(i), w);
+    store_v<T, V>(x, i, N, whole(i), MODE == 1, w);
   }
 }
 
