@@ -177,3 +177,26 @@ def test_feeds_the_dispatch_layout():
     finish()
     placed = sorted_ids[: int(ntp.item())].cpu().numpy()
     assert sorted(placed[placed < 48]) == [p for p in range(48) if p // 4 != 3]
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("E,n_group,topk_group,k", [(64, 8, 4, 4), (256, 8, 4, 8), (160, 5, 2, 6), (96, 32, 7, 6),
+                                                    (128, 16, 16, 8), (1024, 2, 1, 9)])
+def test_close_groups(score, with_bias, E, n_group, topk_group, k):
+    """Groups whose two largest logits differ by a few units in the last place or not at all, groups
+    with one expert or none: decided as 64-bit arithmetic decides them."""
+    rng = np.random.default_rng(E + n_group)
+    T, size = 600, E // n_group
+    l = rng.normal(-2.0, 0.5, (T, n_group, size)).astype(np.float32)
+    steps = rng.integers(-2, 3, (T, n_group, 2)).astype(np.float32)
+    for t in range(T):
+        for g in range(n_group):
+            at = rng.choice(size, 2, replace=False)
+            l[t, g, at[0]] = np.float32(1.25) * (1 + steps[t, g, 0] * 2.0 ** -22)
+            l[t, g, at[1]] = np.float32(0.75) * (1 + steps[t, g, 1] * 2.0 ** -22)
+    one = rng.random((T, n_group)) < 0.1
+    l[np.repeat(one[..., None], size, 2) & (l < 1.0)] = -np.inf  # one expert is left
+    l[rng.random((T, n_group)) < 0.1] = -np.inf
+    bias = torch.full((E,), 0.125, device="cuda") if with_bias else None
+    _run(torch.from_numpy(l.reshape(T, E)).cuda(), k, bias, score, n_group, topk_group)
