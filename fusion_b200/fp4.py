@@ -130,10 +130,12 @@ class ExpertGemmFP4:
         if rows < (pairs if scatter else cap) or not gather and T < cap:
             raise ValueError("too few rows")
         # the packed rows: fresh for each call, so calls on other streams and captured graphs
-        # never share them
+        # never share them; `buf` holds them until the launches have returned (another thread's
+        # allocation on this stream would be given their memory before)
         packed = cap * d.ldxq
         size = packed + ops.fp4_scale_bytes(cap, self.K, self.fmt, block_n)
-        ws = torch.empty(size + spread, dtype=torch.uint8, device=self.device).data_ptr()
+        buf = torch.empty(size + spread, dtype=torch.uint8, device=self.device)
+        ws = buf.data_ptr()
         d.xq, d.xsf = ws, ws + packed
         d.x_rows, d.block_n = cap, block_n
         if row_scale is not None:
@@ -143,6 +145,7 @@ class ExpertGemmFP4:
         ops._call_on(dev, "fus_fp4_expert_gemm", C.addressof(d), x.data_ptr(), dt,
                      xs[0] if T > 1 else self.K, T, topk if gather else 0,
                      ws + size if spread else 0)
+        del buf
         return out
 
     def _refuse(self, x, out, row_scale) -> None:

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 import numpy as np
 import pytest
@@ -153,3 +154,37 @@ def test_no_live_rows():
     with pytest.raises(ValueError, match="ntp"):
         ops.fp4_quantize(torch.zeros(4, 64), torch.zeros(4, 32, dtype=torch.uint8),
                          torch.zeros(4096, dtype=torch.uint8), "mx", ntp=torch.zeros(0, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dense", [True, False])
+def test_workspace_outlives_the_launches(monkeypatch, dense):
+    """The packed rows belong to a call until its kernels are on the stream: memory that went back
+    to the allocator before could be given to another thread's call on the same stream."""
+    made, seen = [], []
+
+    class Torch:
+        def __getattr__(self, name):
+            return getattr(torch, name)
+
+        @staticmethod
+        def empty(*args, **kw):
+            t = torch.empty(*args, **kw)
+            made.append((weakref.ref(t), t.data_ptr()))
+            return t
+
+    def launch(dev, name, desc, *args):
+        d = L.Fp4GemmDesc.from_address(desc)
+        seen.append([r() is not None and p == d.xq for r, p in made])
+
+    g = fp4.ExpertGemmFP4.__new__(fp4.ExpertGemmFP4)  # host tensors: nothing is launched
+    g.E, g.K, g.cols, g.fmt, g.device, g._dev = 1, 64, 32, "nv", torch.device("cpu"), -1
+    g._desc = L.Fp4GemmDesc(K=64, ldxq=32)
+    monkeypatch.setattr(fp4, "torch", Torch())
+    monkeypatch.setattr(ops, "_call_on", launch)
+    x, out = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.bfloat16)
+    if dense:
+        g(x, out)
+    else:
+        i = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+        g(x, out, i(16), i(1), i(1), 16)
+    assert seen == [[True]]

@@ -3,6 +3,8 @@ byte bit for bit, products within the rounding of their sums."""
 
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -352,3 +354,36 @@ def test_expert_product_refuses_and_leaves():
                      "nv", tile=bn, ids=lay[0], id_limit=2 ** 40)
     finish()
     assert bool((out == 7.0).all())
+
+
+@pytest.mark.parametrize("T,bn", [(3, 16), (400, 128)])
+def test_two_threads_on_one_stream(T, bn):
+    """Threads share the default stream: their calls' launches fall between one another, and each
+    call's packed rows stay its own."""
+    E, N, K, k = 4, 256, 1024, 2
+    q, s, g, _ = _stack(E, N, K, "nv", 7)
+    proj = fp4.ExpertGemmFP4(q, s, "nv", gscale=g, gate_up=True)
+    rng = np.random.default_rng(T)
+    topi = np.stack([rng.choice(E, k, replace=False) for _ in range(T)])
+    ids, eids, total = Q.layout(topi, E, bn)
+    dev = [torch.from_numpy(v).cuda() for v in (ids, eids, np.array([total], dtype=np.int32))]
+    xs = [torch.randn(T, K, device="cuda").to(torch.bfloat16) for _ in range(3)]
+    new = lambda: torch.empty(T * k, N // 2, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    want = [proj(x, new(), *dev, bn, topk=k) for x in xs]
+    outs = [[new() for _ in range(60)] for _ in xs]
+    finish()
+    start = threading.Barrier(len(xs))
+
+    def calls(x, mine):
+        start.wait()
+        for out in mine:
+            proj(x, out, *dev, bn, topk=k)
+
+    threads = [threading.Thread(target=calls, args=a) for a in zip(xs, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    finish()
+    for mine, w in zip(outs, want):
+        assert all(torch.equal(out, w) for out in mine)
