@@ -34,7 +34,8 @@ FUS_DEVICE float gate_act(float g, int act) {
   return g;
 }
 
-// sum over the CTA; `red` holds one float for each warp and is free again after the next sum
+// sum over the CTA; `red` holds one float for each warp and is free again after the next sum, over
+// another `red`: that sum's barrier tells that every warp has read this one's
 FUS_DEVICE float cta_sum(float v, float* red) {
   v = warp_sum(v);
   const int nw = blockDim.x >> 5;
@@ -382,7 +383,8 @@ __global__ void __launch_bounds__(kRingThreads, 2)
 #pragma unroll
       for (int j = 0; j < V; ++j) ss += f[v][j] * f[v][j];
     }
-    ss = cta_sum(ss, red[0]);
+    // the row's second sum, or without one the next row's first, takes the other array
+    ss = cta_sum(ss, red[a.x ? 0 : n & 1]);
     __syncwarp();  // with the sum's barrier: the whole CTA has read the stage
     if (threadIdx.x == 0) {
       const long next = t + (long)stages * gridDim.x;

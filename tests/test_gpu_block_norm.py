@@ -233,3 +233,22 @@ def test_graph_on_another_stream_and_empty_batch():
     assert torch.equal(h, h2) and torch.equal(x, x2)
     ops.norm_gate_residual(y[:0], res[:0], h[:0], x[:0], post_w=post_w, pre_w=pre_w)
     finish()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,N", [(8000, 1536), (4001, 6144), (3001, 5003), (9001, 515), (6000, 512)])
+def test_many_rows_without_the_next_norm(dtype, T, N):
+    """Many rows of a CTA one after another, one sum each: the sums do not run into one another. The
+    same arithmetic with the next norm gives the same h, bit for bit."""
+    dt = DTYPES[dtype]
+    y, res, post_w, pre_w, gate = _make(T, N, dt, "token")
+    y *= torch.exp(torch.randn(T, 1, device="cuda")).to(dt)  # every row a sum of its own
+    want, x = torch.empty_like(y), torch.empty_like(y)
+    ops.norm_gate_residual(y, res, want, x, post_w=post_w, pre_w=pre_w, gate=gate, gate_act="sigmoid", alpha=0.37)
+    for _ in range(5):
+        h = torch.full_like(y, 9.0)
+        ops.norm_gate_residual(y, res, h, post_w=post_w, gate=gate, gate_act="sigmoid", alpha=0.37)
+        assert torch.equal(h, want)
+    finish()
+    wh, _, mag = _oracle(y, res, post_w, None, gate, "sigmoid", np.float32(0.37), np.float32(1e-5))
+    _check(h, wh, mag, dt, N)
