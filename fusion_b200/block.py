@@ -246,8 +246,9 @@ class MoEBlockFP4:
     __call__ = forward
 
     def calibrate(self, h: torch.Tensor, r: torch.Tensor) -> None:
-        """Sets the factors of x2 and of the activations ("nv") from a batch: their largest
-        magnitudes over 448 * 6, in place, so captured graphs use them too."""
+        """Sets the factors of x2 and of the activations ("nv"; the routed experts' and the shared
+        one's have the same) from a batch: their largest magnitudes over 448 * 6, in place, so
+        captured graphs use them too."""
         if self.fmt != "nv" or h.shape[0] == 0:
             return
         h1, x2, topw, topi, layout, bn = self._route(h, r)
@@ -256,4 +257,8 @@ class MoEBlockFP4:
         p = layout[0]
         live = (p < topi.numel()) & (torch.arange(p.numel(), device=p.device) < layout[2])
         top = torch.where(live[:, None], act.abs(), 0.0).amax().float()
+        if self.w13s is not None:
+            act_s = self._empty(h.shape[0], self.I)
+            self.w13s(x2, act_s)
+            top = torch.maximum(top, act_s.abs().amax().float())
         self.x_scales[1].copy_(top.clamp_min(1e-20) / 2688.0)

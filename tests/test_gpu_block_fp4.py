@@ -156,3 +156,34 @@ def test_empty_batch():
     e = torch.empty(0, 256, dtype=torch.bfloat16, device="cuda")
     o = blk(e, e)
     assert o.out.shape == (0, 256) and o.x.shape == (0, 256)
+
+
+@pytest.mark.parametrize("times", [0.2, 1.0, 8.0])
+def test_calibration_covers_the_shared_expert(times):
+    """The shared expert's activations have the routed ones' factor: it holds the largest of both, and
+    no block that the down projection reads is cut off. Each value is off by half the widest
+    step of its block (1 of a scale, which is a sixth of the largest within 2^-4), by 2^-4 of the
+    largest where the scale was rounded down, and by the smallest scale's half step (2^-10)."""
+    T, E, H, I, topk = 33, 128, 256, 96, 4
+    w = _weights(E, H, I, "nv", True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    gate_up = times * 0.05 * torch.randn(1, 2 * I, H, device="cuda", generator=g)
+    w["w13s"] = fp4.quantize_weight(gate_up.to(torch.bfloat16), "nv")
+    blk = MoEBlockFP4(**w, topk=topk)
+    h, r = (torch.randn(T, H, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    blk.calibrate(h, r)
+    _, x2, _, topi, layout, bn = blk._route(h, r)
+    act, _, shared = blk._experts(x2, topi, layout, bn)
+    act_s = torch.empty(T, I, dtype=torch.bfloat16, device="cuda")
+    blk.w13s(x2, act_s)
+    finish()
+    ids = layout[0][: int(layout[2].item())]
+    routed = act[: ids.numel()][ids < T * topk]
+    a = _np(act_s)
+    factor = float(blk.x_scales[1].item())
+    assert factor == float(np.float32(max(float(routed.abs().max()), np.abs(a).max())) / np.float32(2688.0))
+    block = np.abs(a).reshape(T, I // 16, 16).max(-1)
+    off = np.repeat(np.maximum(block * (1 + 2.0 ** -4) / 6, block * 2.0 ** -4) + 6 * factor * 2.0 ** -10, 16, axis=-1)
+    w2s = _value(w["w2s"], "nv")[0]
+    bound = off @ np.abs(w2s).T + (I / 16 + 8) * 2.0 ** -23 * ((np.abs(a) + off) @ np.abs(w2s).T) + 1e-30
+    assert (np.abs(_np(shared) - a @ w2s.T) <= bound).all()
