@@ -155,15 +155,16 @@ class MoEBlockFP4:
         if (w13s is None) != (w2s is None):
             raise ValueError("a shared expert has both projections")
         self.gamma, self.bias = gamma, bias
+        self.device = gamma.device
         if gate_w.dtype == torch.float32:
-            self.wa, self.nplanes = ops.router_split_weight(gate_w), 3
+            with torch.cuda.device(self.device):
+                self.wa, self.nplanes = ops.router_split_weight(gate_w), 3
         else:
             self.wa, self.nplanes = gate_w.contiguous(), 1
         self.E, self.H = gate_w.shape
         self.topk, self.eps, self.routed_scale, self.renorm = topk, eps, routed_scale, renorm
         self.score, self.n_group, self.topk_group = score, n_group, topk_group
         self.post_gamma, self.next_gamma, self.residual_scale = post_gamma, next_gamma, residual_scale
-        self.device = gamma.device
         self.fmt = fmt
         if fmt == "nv" and x_scales is None:
             x_scales = tuple(torch.ones(1, device=self.device) for _ in range(2))
@@ -251,6 +252,10 @@ class MoEBlockFP4:
         captured graphs use them too."""
         if self.fmt != "nv" or h.shape[0] == 0:
             return
+        with torch.cuda.device(self.device):
+            self._calibrate(h, r)
+
+    def _calibrate(self, h, r) -> None:
         h1, x2, topw, topi, layout, bn = self._route(h, r)
         self.x_scales[0].copy_(x2.abs().amax().float().clamp_min(1e-20) / 2688.0)
         act, _, _ = self._experts(x2, topi, layout, bn)

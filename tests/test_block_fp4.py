@@ -1,0 +1,65 @@
+"""The 4-bit MoE block's host side: the device its calls run on and what it refuses."""
+
+from __future__ import annotations
+
+import contextlib
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from fusion_b200 import fp4, ops
+from fusion_b200.block import MoEBlockFP4
+
+E, H, I = 4, 64, 32
+
+
+@pytest.fixture
+def current(monkeypatch):
+    """The devices made current, innermost last."""
+    stack = []
+
+    @contextlib.contextmanager
+    def device(d):
+        stack.append(d)
+        yield
+        stack.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", device)
+    return stack
+
+
+def _block(monkeypatch, **kw):
+    """A block on the host: projections that only know their sizes, nothing is launched."""
+    def projection(q, scales, fmt, gscale=None, x_gscale=None, gate_up=False):
+        return SimpleNamespace(E=q.shape[0], N=q.shape[1], K=2 * q.shape[2], gate_up=gate_up,
+                               cols=q.shape[1] // 2 if gate_up else q.shape[1])
+
+    monkeypatch.setattr(fp4, "ExpertGemmFP4", projection)
+    stack = lambda e, n, k: (torch.zeros(e, n, k // 2, dtype=torch.uint8), None, None)  # noqa: E731
+    args = dict(gamma=torch.ones(H, dtype=torch.bfloat16), gate_w=torch.zeros(E, H), bias=None,
+                w13=stack(E, 2 * I, H), w2=stack(E, H, I), fmt="nv")
+    return MoEBlockFP4(**(args | {k: stack(*v) if type(v) is tuple else v for k, v in kw.items()}))
+
+
+def test_every_launch_is_under_the_blocks_device(monkeypatch, current):
+    class Reached(Exception):
+        pass
+
+    def launch(*args, **kw):
+        raise Reached(list(current))
+
+    monkeypatch.setattr(ops, "router_split_weight", launch)
+    with pytest.raises(Reached) as got:
+        _block(monkeypatch)
+    assert got.value.args[0] == [torch.device("cpu")]
+    del current[:]
+    monkeypatch.setattr(ops, "router_split_weight", lambda w: torch.zeros(E, 3 * H, dtype=torch.bfloat16))
+    blk = _block(monkeypatch)
+    blk._route = launch
+    h = torch.zeros(2, H, dtype=torch.bfloat16)
+    for call in (blk.forward, blk.calibrate):
+        del current[:]
+        with pytest.raises(Reached) as got:
+            call(h, h)
+        assert got.value.args[0] == [blk.device]
