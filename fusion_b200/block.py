@@ -181,6 +181,16 @@ class MoEBlockFP4:
     def _empty(self, *shape, dtype=torch.bfloat16):
         return torch.empty(*shape, dtype=dtype, device=self.device)
 
+    def _check(self, h, r) -> None:
+        for t, what in ((h, "h"), (r, "r")):
+            if t.dtype != torch.bfloat16:
+                raise TypeError(f"{what}: bf16 required, not {t.dtype}")
+            if t.dim() != 2 or t.shape != (h.shape[0], self.H):
+                raise ValueError(f"{what} of shape {tuple(t.shape)}: [T, {self.H}] required, h and r alike")
+            ops._rows2d(t, what)
+            if t.device != self.device:
+                raise ValueError(f"{what} is on {t.device}, the block on {self.device}")
+
     def _route(self, h, r):
         """Norm, router and dispatch layout: h1, x2, topw, topi, the layout and its block_n."""
         T = h.shape[0]
@@ -224,6 +234,7 @@ class MoEBlockFP4:
     def forward(self, h: torch.Tensor, r: torch.Tensor) -> BlockFP4Outputs:
         """h, r [T, H] bf16. Allocates through torch's caching allocator and never synchronises, so
         it can be recorded in a CUDA graph."""
+        self._check(h, r)
         with torch.cuda.device(self.device):
             return self._forward(h, r)
 
@@ -250,6 +261,7 @@ class MoEBlockFP4:
         """Sets the factors of x2 and of the activations ("nv"; the routed experts' and the shared
         one's have the same) from a batch: their largest magnitudes over 448 * 6, in place, so
         captured graphs use them too."""
+        self._check(h, r)
         if self.fmt != "nv" or h.shape[0] == 0:
             return
         with torch.cuda.device(self.device):

@@ -63,3 +63,19 @@ def test_every_launch_is_under_the_blocks_device(monkeypatch, current):
         with pytest.raises(Reached) as got:
             call(h, h)
         assert got.value.args[0] == [blk.device]
+
+
+@pytest.mark.parametrize("call", ["forward", "calibrate"])
+def test_inputs_that_do_not_fit_are_refused(monkeypatch, current, call):
+    """Nothing past the end of h or r is read: both are [T, H] bf16 on the block's device."""
+    monkeypatch.setattr(ops, "router_split_weight", lambda w: torch.zeros(E, 3 * H, dtype=torch.bfloat16))
+    blk = _block(monkeypatch)
+    blk._route = lambda *a: pytest.fail("launched")
+    h = torch.zeros(4, H, dtype=torch.bfloat16)
+    for a, b in ((h, h[:3]), (h[:3], h), (h[:, :32], h[:, :32]), (h[0], h[0]), (h, h[:, :32]), (h[None], h[None]),
+                 (h.view(2, 2 * H)[:, ::2], h[:2]), (h, h.to("meta")), (h.to("meta"), h.to("meta"))):
+        with pytest.raises(ValueError):
+            getattr(blk, call)(a, b)
+    for a, b in ((h.float(), h), (h, h.half())):
+        with pytest.raises(TypeError):
+            getattr(blk, call)(a, b)
