@@ -154,20 +154,31 @@ class MoEBlockFP4:
                  next_gamma=None, residual_scale: float = 1.0, x_scales=None):
         if (w13s is None) != (w2s is None):
             raise ValueError("a shared expert has both projections")
+        if gate_w.dim() != 2 or gate_w.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("gate_w: [E, H] fp32 or bf16 required")
+        self.E, self.H = gate_w.shape
+        for w, what in ((gamma, "gamma"), (post_gamma, "post_gamma"), (next_gamma, "next_gamma")):
+            ops._need(w, torch.bfloat16, what, (self.H,))
+        ops._need(bias, torch.float32, "bias", (self.E,))
         self.gamma, self.bias = gamma, bias
         self.device = gamma.device
+        for w in (gate_w, bias, post_gamma, next_gamma):
+            if w is not None and w.device != self.device:
+                raise ValueError(f"tensors on {self.device} and {w.device}")
         if gate_w.dtype == torch.float32:
             with torch.cuda.device(self.device):
                 self.wa, self.nplanes = ops.router_split_weight(gate_w), 3
         else:
             self.wa, self.nplanes = gate_w.contiguous(), 1
-        self.E, self.H = gate_w.shape
         self.topk, self.eps, self.routed_scale, self.renorm = topk, eps, routed_scale, renorm
         self.score, self.n_group, self.topk_group = score, n_group, topk_group
         self.post_gamma, self.next_gamma, self.residual_scale = post_gamma, next_gamma, residual_scale
         self.fmt = fmt
-        if fmt == "nv" and x_scales is None:
-            x_scales = tuple(torch.ones(1, device=self.device) for _ in range(2))
+        if fmt == "nv":
+            x_scales = (None, None) if x_scales is None else x_scales
+            if len(x_scales) != 2:
+                raise ValueError("x_scales: one factor for the rows of x2, one for the activations")
+            x_scales = tuple(torch.ones(1, device=self.device) if s is None else s for s in x_scales)
         self.x_scales = x_scales if fmt == "nv" else (None, None)
         mk = lambda w, i, gate_up: fp4.ExpertGemmFP4(  # noqa: E731
             w[0], w[1], fmt, gscale=w[2], x_gscale=self.x_scales[i], gate_up=gate_up)
@@ -175,8 +186,11 @@ class MoEBlockFP4:
         self.w13s = mk(w13s, 0, True) if w13s is not None else None
         self.w2s = mk(w2s, 1, False) if w2s is not None else None
         self.I = self.w13.cols
-        if self.w13.E != self.E or self.w2.E != self.E or self.w2.K != self.I or self.w2.cols != self.H:
+        size = lambda w: (w.E, w.K, w.cols)  # noqa: E731
+        if size(self.w13) != (self.E, self.H, self.I) or size(self.w2) != (self.E, self.I, self.H):
             raise ValueError("router, w13 and w2 do not fit together")
+        if w13s is not None and (size(self.w13s) != (1, self.H, self.I) or size(self.w2s) != (1, self.I, self.H)):
+            raise ValueError("the shared expert's projections do not fit the block's")
 
     def _empty(self, *shape, dtype=torch.bfloat16):
         return torch.empty(*shape, dtype=dtype, device=self.device)

@@ -39,7 +39,7 @@ def _block(monkeypatch, **kw):
     stack = lambda e, n, k: (torch.zeros(e, n, k // 2, dtype=torch.uint8), None, None)  # noqa: E731
     args = dict(gamma=torch.ones(H, dtype=torch.bfloat16), gate_w=torch.zeros(E, H), bias=None,
                 w13=stack(E, 2 * I, H), w2=stack(E, H, I), fmt="nv")
-    return MoEBlockFP4(**(args | {k: stack(*v) if type(v) is tuple else v for k, v in kw.items()}))
+    return MoEBlockFP4(**(args | {k: stack(*v) if k in ("w13", "w2", "w13s", "w2s") else v for k, v in kw.items()}))
 
 
 def test_every_launch_is_under_the_blocks_device(monkeypatch, current):
@@ -79,3 +79,27 @@ def test_inputs_that_do_not_fit_are_refused(monkeypatch, current, call):
     for a, b in ((h.float(), h), (h, h.half())):
         with pytest.raises(TypeError):
             getattr(blk, call)(a, b)
+
+
+def test_weights_that_do_not_fit_are_refused(monkeypatch, current):
+    """Nothing past the end of a norm's weights or the bias is read, no projection of another size is
+    taken."""
+    monkeypatch.setattr(ops, "router_split_weight", lambda w: torch.zeros(*w.shape[:1], 3 * w.shape[1]))
+    one = torch.ones(H, dtype=torch.bfloat16)
+    good = _block(monkeypatch, w13s=(1, 2 * I, H), w2s=(1, H, I), post_gamma=one, next_gamma=one,
+                  bias=torch.zeros(E), x_scales=(torch.ones(1), torch.ones(1)))
+    assert (good.E, good.H, good.I) == (E, H, I)
+    half = _block(monkeypatch, x_scales=(torch.full((1,), 3.0), None))  # no factor: 1
+    assert [float(s) for s in half.x_scales] == [3.0, 1.0]
+    for bad in ({"gamma": one[:32]}, {"post_gamma": one[:32]}, {"next_gamma": torch.ones(2 * H, dtype=torch.bfloat16)[::2]},
+                {"bias": torch.zeros(E - 1)}, {"bias": torch.zeros(E, device="meta")},
+                {"w13": (E, 2 * I, 2 * H)}, {"w13": (E + 1, 2 * I, H)}, {"w2": (E, H, 2 * I)}, {"w2": (E, 2 * H, I)},
+                {"w13s": (1, 2 * I, H)}, {"w13s": (2, 2 * I, H), "w2s": (1, H, I)},
+                {"w13s": (1, 4 * I, H), "w2s": (1, H, 2 * I)}, {"w13s": (1, 2 * I, H), "w2s": (1, 2 * H, I)},
+                {"x_scales": (torch.ones(1),)}):
+        with pytest.raises(ValueError):
+            _block(monkeypatch, **bad)
+    for bad in ({"gamma": one.float()}, {"post_gamma": one.half()}, {"bias": torch.zeros(E).half()},
+                {"gate_w": torch.zeros(E, H).half()}, {"gate_w": torch.zeros(H)}):
+        with pytest.raises(TypeError):
+            _block(monkeypatch, **bad)
