@@ -110,9 +110,11 @@ FUS_DEVICE float rcp_approx(float v) {  // within 2^-23 of 1 / v
   return r;
 }
 
-// e4m3 byte nearest to a / (6 g), ties to even; g is far from fp32's ends, inv6g = 1 / (6 g)
+// e4m3 byte nearest to a / (6 g), ties to even, at most 448; g is far from fp32's ends, inv6g =
+// 1 / (6 g). The quotient need not be: all that is past 448 is held there, infinity too, before it
+// is moved by its error (infinity less infinity would be a NaN).
 FUS_DEVICE uint32_t nv_scale(float a, float g, float inv6g) {
-  const float t = a * inv6g;
+  const float t = fminf(a * inv6g, 512.0f);
   constexpr float kEps = 1.0f / (1 << 21);
   const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(t - t * kEps, t + t * kEps),
                                                 __NV_SATFINITE, __NV_E4M3);

@@ -387,3 +387,16 @@ def test_two_threads_on_one_stream(T, bn):
     finish()
     for mine, w in zip(outs, want):
         assert all(torch.equal(out, w) for out in mine)
+
+
+@pytest.mark.parametrize("dtype,g", [("bf16", 2e-30), ("fp32", 1e-28), ("bf16", 0.04), ("fp16", 2e-30)])
+def test_quantize_nv_values_past_the_factor(dtype, g):
+    """Finite values whose quotient by the factor is past e4m3's largest, and past fp32's: the scale
+    is 448, the codes saturate."""
+    dt = DTYPES[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(24, 96, device="cuda", generator=gen)
+    x[::3] *= torch.finfo(dt).max / 8
+    x[1::3, ::5] *= torch.finfo(dt).max / 8
+    gt = torch.tensor([g], device="cuda")
+    _check(x.to(dt), "nv", 32, gt, float(gt.item()))
