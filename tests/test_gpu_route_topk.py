@@ -200,3 +200,20 @@ def test_close_groups(score, with_bias, E, n_group, topk_group, k):
     l[rng.random((T, n_group)) < 0.1] = -np.inf
     bias = torch.full((E,), 0.125, device="cuda") if with_bias else None
     _run(torch.from_numpy(l.reshape(T, E)).cuda(), k, bias, score, n_group, topk_group)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size", [8, 32])
+@pytest.mark.parametrize("topk_group", [1, 2, 4])
+@pytest.mark.parametrize("large,step", [(100.0, 1e-4), (1000.0, 1e-4), (1000.0, 1e-3), (10000.0, 1e-2)])
+def test_groups_whose_choices_cancel(score, size, topk_group, large, step):
+    """Biases of either sign: a group's two largest choices are large, their sum is not. fp32 cannot
+    tell such sums apart where their magnitudes' last places are, whatever the sum's are."""
+    gen = torch.Generator(device="cuda").manual_seed(size)
+    T, G = 500, 8
+    # scores some `step` apart: a softmax's are smaller by the number of experts
+    step *= 0.24 * G * size if score == "softmax" else 1.0
+    logits = 0.3 + step * torch.randn(T, G * size, device="cuda", generator=gen)
+    bias = torch.full((G, size), -large, device="cuda")
+    bias[:, 2] = large
+    _run(logits, topk_group, bias.reshape(-1), score, n_group=G, topk_group=topk_group)
