@@ -424,7 +424,8 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const __grid_co
     count += __popc(m);
   }
   __syncwarp();
-  if (few || count > 32) {
+  // (fewer than k: the bound is infinity, by a bias, and its limit a NaN)
+  if (few || count > 32 || count < a.topk) {
     route_row_exact<T>(a, t, lane);
     return;
   }

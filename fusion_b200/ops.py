@@ -469,8 +469,9 @@ def route_topk(logits, topw, topi, *, score: str = "sigmoid", bias=None, n_group
                topk_group: int = 1, renorm: bool = True, scale: float = 1.0):
     """Experts of each token from router logits [T, E] (bf16, fp16 or fp32): topi [T, k] int32
     and their weights topw [T, k] fp32. score "sigmoid" or "softmax"; bias [E] fp32 counts in the
-    choice only; n_group / topk_group limit the choice to the best groups; renorm divides by the
-    chosen weights' sum. -inf or NaN logits mask experts; slots left over get id -1, weight 0."""
+    choice only (+inf: first, -inf: out, not NaN); n_group / topk_group limit the choice to the best
+    groups; renorm divides by the chosen weights' sum. -inf or NaN logits mask experts; slots left
+    over get id -1, weight 0."""
     T, E = logits.shape
     k = topi.shape[1] if topi.dim() == 2 else 0
     st, dt, dev = logits.stride(), DT.get(logits.dtype), logits.get_device()

@@ -161,7 +161,7 @@ int fus_router_topk_grouped(const float* partial, int nsplit, const float* bias,
  *   w *= scale
  * A logit of -infinity or NaN masks its expert. Slots without an expert left: id -1 (a hole
  * of fus_moe_align), weight 0; fus_clear_holes zeroes the expert rows that no one writes then.
- * bias [E] fp32 or NULL, finite. */
+ * bias [E] fp32 or NULL, not NaN; +infinity puts an expert first, -infinity leaves it out. */
 #define FUS_SCORE_SIGMOID 0
 #define FUS_SCORE_SOFTMAX 1
 int fus_route_topk(const void* logits, int dtype, long ld, const float* bias, int score,

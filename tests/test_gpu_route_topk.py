@@ -217,3 +217,33 @@ def test_groups_whose_choices_cancel(score, size, topk_group, large, step):
     bias = torch.full((G, size), -large, device="cuda")
     bias[:, 2] = large
     _run(logits, topk_group, bias.reshape(-1), score, n_group=G, topk_group=topk_group)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("groups", [1, 4])
+@pytest.mark.parametrize("k", [1, 3])
+@pytest.mark.parametrize("first,out", [((), (0, 9, 63)), ((5,), ()), ((40, 7), (3,)), ((50, 40, 7, 8), ()),
+                                       ((1, 2, 17, 18, 19, 30, 31), (0, 3))])
+def test_infinite_bias(score, groups, k, first, out):
+    """A bias of +infinity puts an expert first (several: the lower id), of -infinity leaves it out."""
+    gen = torch.Generator(device="cuda").manual_seed(len(first))
+    T, E = 70, 64
+    logits = torch.randn(T, E, device="cuda", generator=gen)
+    bias = 0.1 * torch.randn(E, device="cuda", generator=gen)
+    bias[list(first)], bias[list(out)] = float("inf"), -float("inf")
+    w = torch.full((T, k), 9.0, device="cuda")
+    i = torch.full((T, k), 9, dtype=torch.int32, device="cuda")
+    topk_group = max(1, groups // 2)
+    ops.route_topk(logits, w, i, score=score, bias=bias, n_group=groups, topk_group=topk_group)
+    finish()
+    e = np.exp(logits.double().cpu().numpy())
+    s = e / (1 + e) if score == "sigmoid" else e / e.sum(1, keepdims=True)
+    c = (s + bias.double().cpu().numpy()).reshape(T, groups, -1)
+    best = -np.sort(-c, -1)[..., :2].sum(-1)
+    drop = np.argsort(-best, 1, kind="stable")[:, topk_group:]
+    np.put_along_axis(c, drop[..., None], -np.inf, 1)
+    ids = np.argsort(-c.reshape(T, E), 1, kind="stable")[:, :k]
+    want = np.take_along_axis(s, ids, 1)
+    want /= want.sum(1, keepdims=True)
+    np.testing.assert_array_equal(i.cpu().numpy(), ids)
+    assert (np.abs(w.double().cpu().numpy() - want) <= 2.0 ** -17 * want).all()
