@@ -378,7 +378,8 @@ extern "C" int fus_moe_align(const int* ids, int numel, int E, int block_m, int*
 }
 
 extern "C" int fus_clear_holes(const int* ids, int n, void* y, long ldy, int H, void* stream) {
-  if (n < 0 || H < 1 || H % 8) return set_error(FUS_E_INVALID, "clear_holes: bad sizes");
+  if (n < 0 || n > kMaxRows || H < 1 || H % 8)
+    return set_error(FUS_E_INVALID, "clear_holes: bad sizes");
   if (n == 0) return FUS_OK;
   if (!ids || !y || !aligned16(y) || ldy % 8 || ldy < H)
     return set_error(FUS_E_INVALID, "clear_holes: rows must be 16-byte aligned");

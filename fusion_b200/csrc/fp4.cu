@@ -477,7 +477,7 @@ int check_common(const char* what, int fmt, int dtype, long rows, int K, int til
     return set_error(FUS_E_INVALID, "%s: unknown format %d", what, fmt);
   if (!dtype_known(dtype))
     return set_error(FUS_E_INVALID, "%s: unknown dtype %d", what, dtype);
-  if (rows < 0 || rows > 0x7fffffffL) return set_error(FUS_E_INVALID, "%s: bad row count", what);
+  if (rows < 0 || rows > kMaxRows) return set_error(FUS_E_INVALID, "%s: bad row count", what);
   if (K <= 0 || K % 32)
     return set_error(FUS_E_INVALID, "%s: K=%d must be a positive multiple of 32", what, K);
   if (tile != 0 && !valid_tile(tile))

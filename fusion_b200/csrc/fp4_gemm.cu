@@ -557,7 +557,8 @@ int check_gemm(const fus_fp4_gemm_desc* d) {
   if (d->block_n != 16 && d->block_n != 32 && d->block_n != 64 && d->block_n != 128 &&
       d->block_n != 256)
     return set_error(FUS_E_INVALID, "fp4_gemm: block_n %d not in {16,32,64,128,256}", d->block_n);
-  if (d->x_rows < 0 || d->out_rows < 0) return set_error(FUS_E_INVALID, "fp4_gemm: bad row counts");
+  if (d->x_rows < 0 || d->x_rows > kMaxRows || d->out_rows < 0)
+    return set_error(FUS_E_INVALID, "fp4_gemm: bad row counts");
   if (d->out_dtype != FUS_DT_BF16 && d->out_dtype != FUS_DT_F32)
     return set_error(FUS_E_INVALID, "fp4_gemm: output is FUS_DT_BF16 or FUS_DT_F32");
   if (d->x_rows == 0) return FUS_OK;
@@ -612,7 +613,7 @@ int gemm_launch(const fus_fp4_gemm_desc* d, int pdl, void* stream, int* status) 
   a.pdl = pdl;
   a.status = status;
   const long units = (long)blocks * a.m_tiles;
-  if (units > 0x7fffffffL) return set_error(FUS_E_UNSUPPORTED, "fp4_gemm: too many tiles");
+  if (units > kMaxRows) return set_error(FUS_E_UNSUPPORTED, "fp4_gemm: too many tiles");
   CUtensorMap tw;
   TokenMaps tx;
   const uint64_t row = (uint64_t)d->K / 2, rows = (uint64_t)d->n_experts * d->w_rows;

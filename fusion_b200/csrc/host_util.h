@@ -81,6 +81,10 @@ int fp4_quantize_spread(const void* x, int dtype, long ldx, int T, int K, int fm
                         const int* ids, int per_token, int limit, const int* ntp, int cap, int tile,
                         int* pos, void* q, long ldq, void* sf, void* stream, int* status);
 
+// Rows of a call whose kernels count them in 32 bits: the threads of the last CTA count past the
+// last row, by less than what is missing here to 2^31.
+constexpr long kMaxRows = 0x7fff0000L;
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }

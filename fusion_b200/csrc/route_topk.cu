@@ -500,7 +500,7 @@ extern "C" int fus_route_topk(const void* logits, int dtype, long ld, const floa
                               int T, int E, int topk, float scale, int renorm, void* stream,
                               int* status) {
   (void)status;
-  if (T < 0 || E < 1 || topk < 1 || topk > 32 || topk > E)
+  if (T < 0 || T > kMaxRows || E < 1 || topk < 1 || topk > 32 || topk > E)
     return set_error(FUS_E_INVALID, "route_topk: T=%d E=%d topk=%d (topk <= 32, <= E)", T, E, topk);
   if (!dtype_known(dtype)) return set_error(FUS_E_INVALID, "route_topk: dtype %d", dtype);
   if (score != FUS_SCORE_SIGMOID && score != FUS_SCORE_SOFTMAX)

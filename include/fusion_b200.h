@@ -390,7 +390,8 @@ int fus_fp8_block_dequant(const void* src, const float* scale, long scale_ld, vo
  * of exact arithmetic. A block with an infinity or a NaN gets the NaN scale. K % 32 == 0.
  * Scale layouts: tile = 0 row-major [rows, K / n] bytes, as checkpoints store them; tile in
  * {16, 32, 64, 128, 256}: the atoms the tensor cores read, one run for each `tile` rows (a
- * dispatch block), fus_fp4_scale_bytes(fmt, rows, K, tile) bytes, 16-byte aligned.
+ * dispatch block), fus_fp4_scale_bytes(fmt, rows, K, tile) bytes, 16-byte aligned. Calls have
+ * 2^31 - 2^16 rows at most.
  *
  * fus_fp4_quantize: row p of q [rows, ldq bytes] = x[ids ? ids[p] / id_div : p]; rows with
  *   ids[p] outside [0, id_limit) (dispatch pads) and rows from ntp[0] on keep what they

@@ -188,3 +188,18 @@ def test_workspace_outlives_the_launches(monkeypatch, dense):
         i = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
         g(x, out, i(16), i(1), i(1), 16)
     assert seen == [[True]]
+
+
+def test_rows_that_the_last_cta_would_count_past_32_bits():
+    top = 0x7FFF0000  # the last allowed count; its launch is not tried here
+    for rows in (top + 1, 2 ** 31 - 1):
+        _refused(L.lib().fus_fp4_quantize(P, 0, 64, 4, 64, 1, None, 0, P, 1, 4, None, rows, 16, P, 32, P,
+                                          None, None), "row count")
+        _refused(L.lib().fus_fp4_dequantize(P, 32, P, 1, 16, rows, 64, None, 0, P, 0, 64, None, None), "row count")
+        d = L.Fp4GemmDesc(wq=P, wsf=P, n_experts=1, w_rows=64, K=64, fmt=1, xq=P, ldxq=32, xsf=P, x_rows=rows,
+                          block_n=16, out=P, ldo=64, out_rows=20)
+        _refused(L.lib().fus_fp4_grouped_gemm(ctypes.byref(d), None, None), "row counts")
+        _refused(L.lib().fus_fp4_expert_gemm(ctypes.byref(d), P, 0, 64, 4, 0, None, None, None), "row counts")
+    # and tiles: rows in blocks times the weight's tiles
+    d.x_rows, d.w_rows, d.ldo = 2 ** 27, 2 ** 15, 2 ** 15
+    _refused(L.lib().fus_fp4_grouped_gemm(ctypes.byref(d), None, None), "too many tiles")

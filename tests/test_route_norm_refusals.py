@@ -86,3 +86,9 @@ def test_python_refusals():
                      ((x, x, x), {"gate": torch.zeros(4, 1).half()}), ((x.T, x.T, x.T), {})):
         with pytest.raises((ValueError, TypeError)):
             ops.norm_gate_residual(*args, **kw)
+
+
+def test_rows_that_the_last_cta_would_count_past_32_bits():
+    for n in (0x7FFF0001, 2 ** 31 - 1):
+        _refused(L.lib().fus_route_topk(P, 1, 64, None, 0, 1, 1, P, P, n, 64, 8, 1.0, 1, None, None), f"T={n}")
+        _refused(L.lib().fus_clear_holes(P, n, P, 64, 64, None), "sizes")
