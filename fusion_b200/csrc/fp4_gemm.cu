@@ -659,6 +659,9 @@ extern "C" int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, in
   if (gather_div > 0 && ((long)src_rows * gather_div < d->live_limit ||
                          (long)src_rows * gather_div > 0x7fffffffL))
     return set_error(FUS_E_INVALID, "fp4_expert_gemm: %d rows for %d pairs", src_rows, d->live_limit);
+  // No pairs: the quantiser would launch nothing, and the product, launched as its dependent, would
+  // overlap whatever ran before.
+  if (gather_div > 0 && d->live_limit <= 0) return FUS_OK;
   // Large batches: a token is quantised once and written to its pairs' rows (two launches: the
   // places, then the rows). One pass over the dispatch order, which quantises a token for each
   // of its pairs, has a launch less (2.2 us) and more to compute (1.4 to 2.2 million elements a

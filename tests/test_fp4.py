@@ -203,3 +203,11 @@ def test_rows_that_the_last_cta_would_count_past_32_bits():
     # and tiles: rows in blocks times the weight's tiles
     d.x_rows, d.w_rows, d.ldo = 2 ** 27, 2 ** 15, 2 ** 15
     _refused(L.lib().fus_fp4_grouped_gemm(ctypes.byref(d), None, None), "too many tiles")
+
+
+def test_expert_product_without_pairs_launches_nothing():
+    """The product starts while its quantiser runs; without one there is nothing it may overlap."""
+    d = L.Fp4GemmDesc(wq=P, wsf=P, n_experts=2, w_rows=64, K=64, fmt=1, xq=P, ldxq=32, xsf=P, x_rows=32,
+                      block_n=16, expert_ids=P, ntp=P, live_ids=P, live_limit=0, scatter=1, out=P, ldo=64, out_rows=20)
+    for rows, div in ((0, 8), (4, 8), (4, 1)):
+        assert L.lib().fus_fp4_expert_gemm(ctypes.byref(d), P, 0, 64, rows, div, P, None, None) == 0
