@@ -53,7 +53,18 @@ def status_tensor(device: torch.device | int | None = None) -> torch.Tensor:
                        (device if isinstance(device, int) else device.index or 0))
     t = _status.get(dev.index)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=dev)
+        # On a stream of its own, finished here: a first call that is being recorded in a graph must
+        # not record this too, or every replay would clear the word. (Allocating beside a
+        # capture wants this thread's capture mode relaxed, CU_STREAM_CAPTURE_MODE_RELAXED.)
+        side = torch.cuda.Stream(dev)
+        exchange, mode = C.CDLL("libcuda.so.1").cuThreadExchangeStreamCaptureMode, C.c_int(2)
+        exchange(C.byref(mode))
+        try:
+            with torch.cuda.stream(side):
+                t = torch.zeros(1, dtype=torch.int32, device=dev)
+            side.synchronize()
+        finally:
+            exchange(C.byref(mode))
         _status[dev.index] = t
     return t
 

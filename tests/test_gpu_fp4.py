@@ -3,6 +3,9 @@ byte bit for bit, products within the rounding of their sums."""
 
 from __future__ import annotations
 
+import pathlib
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -400,3 +403,31 @@ def test_quantize_nv_values_past_the_factor(dtype, g):
     x[1::3, ::5] *= torch.finfo(dt).max / 8
     gt = torch.tensor([g], device="cuda")
     _check(x.to(dt), "nv", 32, gt, float(gt.item()))
+
+
+def test_first_call_captured():
+    """A process whose first call is recorded in a graph: replays do not clear what other calls
+    reported (the status word belongs to the process, not to the graph)."""
+    code = """
+import torch
+from fusion_b200 import fp4, ops
+q, s = torch.zeros(2, 32, 32, dtype=torch.uint8, device="cuda"), torch.zeros(2, 32, 4, dtype=torch.uint8, device="cuda")
+i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+x, w, i = torch.randn(4, 16, device="cuda"), torch.empty(4, 2, device="cuda"), torch.empty(4, 2, dtype=torch.int32, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    ops.route_topk(x, w, i)
+graph.replay()
+ops.check_status()
+assert (w.sum(1) - 1).abs().max() < 1e-6
+ids = torch.full((16,), 1, dtype=torch.int32, device="cuda")
+ids[0] = 0
+out = torch.zeros(1, 32, dtype=torch.bfloat16, device="cuda")
+fp4.ExpertGemmFP4(q, s, "nv")(torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda"), out, ids, i32(7), i32(16), 16)
+graph.replay()
+torch.cuda.synchronize()
+assert ops.read_status() == ops.ERR_BAD_EXPERT
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=200,
+                         cwd=pathlib.Path(__file__).parent.parent)
+    assert run.returncode == 0, run.stderr[-2000:]
