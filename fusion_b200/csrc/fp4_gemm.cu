@@ -665,11 +665,16 @@ extern "C" int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, in
   // Large batches: a token is quantised once and written to its pairs' rows (two launches: the
   // places, then the rows). One pass over the dispatch order, which quantises a token for each
   // of its pairs, has a launch less (2.2 us) and more to compute (1.4 to 2.2 million elements a
-  // us). NV, spread / one pass: 8192 pairs of 1024 tokens, K 6144 121 / 144 us with the product,
-  // 1024 of 128, K 6144 91.8 / 95.8, 1024 of 128, K 2048 19.1 / 16.9.
+  // us). NV, spread / one pass: 8192 pairs of 1024 tokens, K 6144 121 / 144 us with the product.
+  // With a narrow product (32 experts x 256 rows), called eagerly, at 2, 4 and 6 Mi saved elements,
+  // 8 pairs a token: K 2048 NV 16.1 / 16.5, 18.5 / 18.6, 20.6 / 24.6 us, MX 16.3 / 15.3, 18.5 / 16.6,
+  // 18.6 / 20.7; K 6144 NV 19.7 / 26.2, 21.7 / 28.8, 22.5 / 30.9, MX 18.7 / 24.8, 22.0 / 26.7,
+  // 22.4 / 26.9: the border is where long rows no longer lose and short ones begin to gain. Replayed
+  // in a graph, without the host's launch, spreading is ahead from 1 Mi on (K 2048 NV 10.3 / 12.8).
   const bool spread = pair_ws && gather_div > 1 &&
                       ((long)d->live_limit - src_rows) * d->K >= kSpreadElements;
-  // rows in dispatch order: pads are skipped by their id, gathered or not
+  // Gathered rows skip pads by their ids. Rows that are in dispatch order already are quantised as
+  // they lie, pads too: what they hold reaches no output (a token is a column of its own).
   if (spread) {
     // the checks of fus_fp4_quantize, on no rows
     if (int rc = fus_fp4_quantize(x, x_dtype, ldx, src_rows, d->K, d->fmt, d->xg, 0, nullptr, 1, 0,

@@ -74,7 +74,8 @@ class ExpertGemmFP4:
     def __call__(self, x, out, sorted_ids=None, expert_ids=None, ntp=None, block_n: int = 0, *,
                  topk: int = 1, gather: bool = True, scatter: bool = True, pairs: int | None = None,
                  row_scale=None):
-        """One projection over a dispatch layout (``ops.moe_align`` with block_n).
+        """One projection over a dispatch layout (``ops.moe_align`` with block_n: pads end a block, a
+        pair stands at most once).
 
         gather: x [T, K] holds tokens, dispatch row p is x[sorted_ids[p] // topk]; else x
         [capacity, K] is in dispatch order. scatter: out [pairs, cols] in pair order (row

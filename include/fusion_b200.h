@@ -93,7 +93,8 @@ int fus_add_rmsnorm(const void* x, long ldx, const void* res, long ldr, const vo
  *   h = res + alpha * act(gate) * v
  *   x = h * rsqrt(mean(h^2) + eps) * pre_w       (x and pre_w NULL: not computed)
  * [T, N] rows, all of `dtype`, any N to 32768 (16384 fp32) and any alignment (16-byte rows are
- * fastest); fp32 arithmetic, h and x rounded once each, x from the unrounded h. gate: none,
+ * fastest; weights off 16 bytes, or rows that start unlike one another, take to 4 times as long);
+ * fp32 arithmetic, h and x rounded once each, x from the unrounded h. gate: none,
  * one for a token (gate[t * ldg]), for a channel (gate[n]) or for an element. h may be res
  * or y, x may be y (the same rows and strides). */
 #define FUS_GATE_NONE 0
@@ -161,6 +162,8 @@ int fus_router_topk_grouped(const float* partial, int nsplit, const float* bias,
  *   w *= scale
  * A logit of -infinity or NaN masks its expert. Slots without an expert left: id -1 (a hole
  * of fus_moe_align), weight 0; fus_clear_holes zeroes the expert rows that no one writes then.
+ * Slow (6 to 14 times): topk near 32 or past a third of the experts; 32 groups of which fewer than
+ * topk / 2 are kept.
  * bias [E] fp32 or NULL, not NaN; +infinity puts an expert first, -infinity leaves it out. */
 #define FUS_SCORE_SIGMOID 0
 #define FUS_SCORE_SOFTMAX 1
@@ -417,7 +420,8 @@ int fus_fp4_pack_scales(const void* scales, int fmt, int n_experts, int w_rows, 
 /* Grouped product of 4-bit rows with 4-bit expert weights on the block-scaled tensor
  * cores, the 4-bit form of fus_grouped_gemm: rows of xq in dispatch order, block b of
  * `block_n` rows meets expert expert_ids[b] (NULL: one expert); rows from ntp[0] on and
- * rows whose live_ids entry is not below live_limit (pads, which end a block) give no output.
+ * rows whose live_ids entry is not below live_limit give no output. The layout is fus_moe_align's:
+ * pads end a block, an id stands at most once.
  *   FUS_EPI_BF16   out[r, n] = wg[e] * xg * row_scale[r] * acc      n < w_rows
  *   FUS_EPI_SWIGLU out[r, f] = row_scale[r] * silu(y[r, f]) * y[r, w_rows/2 + f],
  *                  y = wg[e] * xg * acc in fp32; f < w_rows / 2
