@@ -65,7 +65,7 @@ def status_tensor(device: torch.device | int | None = None) -> torch.Tensor:
             side.synchronize()
         finally:
             exchange(C.byref(mode))
-        _status[dev.index] = t
+        t = _status.setdefault(dev.index, t)  # another thread's, if it was first
     return t
 
 

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import contextlib
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -92,3 +95,20 @@ def test_rows_that_the_last_cta_would_count_past_32_bits():
     for n in (0x7FFF0001, 2 ** 31 - 1):
         _refused(L.lib().fus_route_topk(P, 1, 64, None, 0, 1, 1, P, P, n, 64, 8, 1.0, 1, None, None), f"T={n}")
         _refused(L.lib().fus_clear_holes(P, n, P, 64, 64, None), "sizes")
+
+
+def test_one_status_word_for_two_first_calls(monkeypatch):
+    """Two threads that find no status word make one each; both go on with the first, whose address
+    kernels may have by then."""
+    first, late = torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+
+    def zeros(*args, **kw):
+        ops._status[7] = first  # the other thread's, meanwhile
+        return late
+
+    monkeypatch.setattr(torch.cuda, "Stream", lambda dev: SimpleNamespace(synchronize=lambda: None))
+    monkeypatch.setattr(torch.cuda, "stream", contextlib.nullcontext)
+    monkeypatch.setattr(ops.C, "CDLL", lambda name: SimpleNamespace(cuThreadExchangeStreamCaptureMode=lambda m: 0))
+    monkeypatch.setattr(ops, "_status", {})
+    monkeypatch.setattr(torch, "zeros", zeros)
+    assert ops.status_tensor(7) is first and ops._status[7] is first
