@@ -350,15 +350,10 @@ __global__ void __launch_bounds__(kWarps * 32) route_topk_kernel(const __grid_co
       }
       bool in = mine != gkey;
       const float gi = value_of(last), go = value_of(__reduce_max_sync(kAll, mine));
-      // What a sum is off by goes with the magnitudes of its two choices. Without a bias they are
-      // scores: the sum is no smaller. With one they may cancel: the largest of the groups'.
-      float mag = gi;
-      if (a.bias) {
-        mag = a2 > -INFINITY ? fabsf(a1) + fabsf(a2) : a1 > -INFINITY ? fabsf(a1) : 0.f;
-        mag = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(mag)));
-      }
-      // too near to tell apart in fp32? (no group left: go is a NaN)
-      if (gi - go <= 2.f * tol * (1.f + fabsf(mag)) ||
+      // Too near to tell apart in fp32, by any group's error? (No group left: go is a NaN.) What a sum
+      // is off by goes with the magnitudes of its two choices, which may cancel in it.
+      const float mag = fabsf(a1) + (a2 > -INFINITY ? fabsf(a2) : 0.f);
+      if (__any_sync(kAll, g > -INFINITY && gi - go <= 2.f * tol * (1.f + mag)) ||
           __popc(__ballot_sync(kAll, in)) != a.topk_group << a.lpg_log2) {
         const float from = second - tol * (1.f + fabsf(second));
         uint32_t two = 0;
