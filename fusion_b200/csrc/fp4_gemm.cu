@@ -669,8 +669,8 @@ extern "C" int fus_fp4_expert_gemm(const fus_fp4_gemm_desc* d, const void* x, in
   // With a narrow product (32 experts x 256 rows), called eagerly, at 2, 4 and 6 Mi saved elements,
   // 8 pairs a token: K 2048 NV 16.1 / 16.5, 18.5 / 18.6, 20.6 / 24.6 us, MX 16.3 / 15.3, 18.5 / 16.6,
   // 18.6 / 20.7; K 6144 NV 19.7 / 26.2, 21.7 / 28.8, 22.5 / 30.9, MX 18.7 / 24.8, 22.0 / 26.7,
-  // 22.4 / 26.9: the border is where long rows no longer lose and short ones begin to gain. Replayed
-  // in a graph, without the host's launch, spreading is ahead from 1 Mi on (K 2048 NV 10.3 / 12.8).
+  // 22.4 / 26.9: at K 2048 the two meet about 4 Mi. Replayed in a graph, without the host's launch,
+  // spreading is ahead from 1 Mi on (K 2048 NV 10.3 / 12.8).
   const bool spread = pair_ws && gather_div > 1 &&
                       ((long)d->live_limit - src_rows) * d->K >= kSpreadElements;
   // Gathered rows skip pads by their ids. Rows that are in dispatch order already are quantised as
