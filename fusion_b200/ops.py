@@ -107,7 +107,8 @@ def router_split_weight(wg: torch.Tensor) -> torch.Tensor:
     """fp32 [E, H] -> bf16 planes [E, 3H] (hi | mid | lo)."""
     E, H = wg.shape
     wa = torch.empty(E, 3 * H, dtype=torch.bfloat16, device=wg.device)
-    L.call("fus_router_split_weight", _p(wg.contiguous()), _p(wa), E, H, _stream())
+    wg = wg.contiguous()  # held until the launch has returned
+    L.call("fus_router_split_weight", _p(wg), _p(wa), E, H, _stream())
     return wa
 
 
@@ -115,7 +116,8 @@ def router_transpose_weight(wgt: torch.Tensor) -> torch.Tensor:
     """bf16 [H, E] -> bf16 [E, H]."""
     H, E = wgt.shape
     wa = torch.empty(E, H, dtype=torch.bfloat16, device=wgt.device)
-    L.call("fus_router_transpose_weight", _p(wgt.contiguous()), _p(wa), H, E, _stream())
+    wgt = wgt.contiguous()  # held until the launch has returned
+    L.call("fus_router_transpose_weight", _p(wgt), _p(wa), H, E, _stream())
     return wa
 
 

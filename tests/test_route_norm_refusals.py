@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import contextlib
+import weakref
 from types import SimpleNamespace
 
 import pytest
@@ -112,3 +113,15 @@ def test_one_status_word_for_two_first_calls(monkeypatch):
     monkeypatch.setattr(ops, "_status", {})
     monkeypatch.setattr(torch, "zeros", zeros)
     assert ops.status_tensor(7) is first and ops._status[7] is first
+
+
+@pytest.mark.parametrize("entry", [ops.router_split_weight, ops.router_transpose_weight])
+def test_copied_weights_outlive_the_launch(monkeypatch, entry):
+    """A router weight that is copied to be contiguous: the copy is there when the kernel is launched."""
+    passed, alive = [], []
+    address = ops._p
+    monkeypatch.setattr(ops, "_p", lambda t: passed.append(weakref.ref(t)) or address(t))
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(L, "call", lambda *args: alive.extend(r() is not None for r in passed))
+    entry(torch.zeros(8, 16).T)
+    assert alive == [True, True]
